@@ -53,6 +53,17 @@ class HeadConfig(ctypes.Structure):
     ]
 
 
+class PagedConfig(ctypes.Structure):
+    _fields_ = [
+        ("kind", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("first", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("inv_unit", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -105,6 +116,12 @@ SIGNATURES = {
     "algx_swiglu_bwd": ([_P, _P, _P, _I64, _I64, _P], ctypes.c_int),
     "algx_aluglu_fwd": ([_P, _P, _I64, _I64, _F, _P], ctypes.c_int),
     "algx_aluglu_bwd": ([_P, _P, _P, _I64, _I64, _F, _P], ctypes.c_int),
+    "algx_cache_append": ([_P] * 5 + [_I64] + [_P] * 8 + [_I64] * 8 + [_I32, _F, _P], ctypes.c_int),
+    "algx_paged_attn_workspace_size": ([_I64] * 8 + [_I32], _SZ),
+    "algx_paged_attn": ([ctypes.POINTER(PagedConfig)] + [_P] * 9 + [_I64] * 8 + [_I32, _P, _SZ, _P], ctypes.c_int),
+    "algx_cache_evict_workspace_size": ([_I64] * 3, _SZ),
+    "algx_cache_evict": ([_P] * 6 + [_I64] * 3 + [_P] * 4 + [_I64] * 6 + [_I32, _P, _SZ, _P], ctypes.c_int),
+    "algx_verify_draft": ([_I32, _I32, _F] + [_P] * 8 + [_I64] * 3 + [_I32, _P], ctypes.c_int),
 }
 
 _lib = None

@@ -30,6 +30,7 @@ enum DeviceError : int {
   DEV_ERR_MBAR_TIMEOUT = 1,
   DEV_ERR_TMEM_ALLOC = 2,
   DEV_ERR_BAD_LABEL = 4,
+  DEV_ERR_BAD_PAGE = 8,  // a page table entry, a length or a position outside its range
 };
 
 // Programmatic dependent launch: a kernel launched with launch_dependent() may

@@ -1,0 +1,123 @@
+// What the paged-cache kernels share: the cache's layout and the two score
+// weights, asinh-power (algebraic.py:186-204) and softmax.
+#pragma once
+
+#include "algx_common.cuh"
+
+namespace algx {
+
+// Keys and values live in pages: k_pages, v_pages (num_pages, Hkv, page_size,
+// 64). Slot s of sequence b lies in page table[b * max_pages + s / page_size] at
+// row s % page_size. page_size is a power of two of at least 16, so an aligned
+// group of 16 slots never straddles two pages.
+struct PagedView {
+  const int32_t* table;
+  const int32_t* lens;
+  int32_t num_pages;
+  int32_t max_pages;
+  int32_t page_shift;  // log2(page_size)
+  int32_t heads;       // Hkv
+};
+
+// The view of a call's arguments, or an error status (cache.cu).
+int paged_view(PagedView* pv, const void* table, const void* lens, int64_t B, int64_t Hkv, int64_t num_pages,
+               int64_t page_size, int64_t max_pages, int64_t D);
+int* device_error_word();
+
+// First element of the row that holds slot `s` for head h in page `pid`.
+__device__ __forceinline__ int64_t paged_row(const PagedView& pv, int pid, int h, int s) {
+  const int64_t in_page = s & ((1 << pv.page_shift) - 1);
+  return ((((int64_t)pid * pv.heads + h) << pv.page_shift) + in_page) * 64;
+}
+
+// Slots of sequence b that the table can address, 0 for a negative length.
+__device__ __forceinline__ int paged_len(const PagedView& pv, int b, int* err) {
+  const int len = pv.lens[b];
+  const int64_t cap = (int64_t)pv.max_pages << pv.page_shift;
+  if (len > cap) {
+    if (threadIdx.x == 0) atomicOr(err, DEV_ERR_BAD_PAGE);
+    return (int)cap;
+  }
+  return len < 0 ? 0 : len;
+}
+
+// rho(x) for either sign (kernels/flash.py:76-80): |x| + sqrt(1 + x^2), or its
+// reciprocal for x < 0. EXACT uses correctly rounded square root and division
+// (float32 I/O); otherwise the MUFU forms with about 2^-22 relative error,
+// 16 times that in a 16th power, far below bf16's 2^-9.
+template <bool EXACT>
+__device__ __forceinline__ float rho_any(float x) {
+  const float rad = fmaf(x, x, 1.f);
+  if constexpr (EXACT) {
+    const float t = fabsf(x) + sqrtf(rad);
+    return x >= 0.f ? t : 1.f / t;
+  } else {
+    float s;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(rad));
+    const float t = fabsf(x) + s;
+    return x >= 0.f ? t : rcp_fast(t);
+  }
+}
+
+__device__ __forceinline__ float pow_log2(float x, int log2n) {
+  for (int i = 0; i < log2n; ++i) x *= x;
+  return x;
+}
+
+// Weight of a score x against a reference score m: (rho(x) rho(-m))^n for the
+// asinh kind, exp(x - m) for softmax. `turn` is the reference's part, computed
+// once per reference. m = -inf (no score seen yet) gives an infinite weight to
+// any finite x.
+constexpr int kAsinh = ALGX_ATTN_ASINH, kSoftmax = ALGX_ATTN_SOFTMAX;
+
+template <int KIND, bool EXACT>
+__device__ __forceinline__ float weight_turn(float m) {
+  if constexpr (KIND == kAsinh) return rho_any<EXACT>(-m);
+  else return m;
+}
+template <int KIND, bool EXACT>
+__device__ __forceinline__ float weight_of(float x, float turn, int log2n) {
+  if constexpr (KIND == kSoftmax) return EXACT ? expf(x - turn) : __expf(x - turn);
+  else return pow_log2(rho_any<EXACT>(x) * turn, log2n);
+}
+
+// Which slots a query sees. Query token t of T new ones stands at slot
+// last = len - T + t and sees slots s <= last with s > last - window or
+// s < first (window 0: no window).
+struct Sight {
+  int window;
+  int first;
+  __device__ __forceinline__ bool sees(int s, int last) const {
+    return s <= last && (window == 0 || s > last - window || s < first);
+  }
+  // Whether every query with lo <= last <= hi sees every slot of s .. s + 15.
+  __device__ __forceinline__ bool sees_group(int s, int lo, int hi) const {
+    return s + 15 <= lo && (window == 0 || s > hi - window || s + 15 < first);
+  }
+};
+
+// The aligned groups of 16 slots that queries with lo <= last <= hi look at: the
+// groups of the first visible slots, then those from the window's left end on.
+struct Span {
+  int head_groups;  // groups before the gap
+  int skip;         // groups in the gap
+  int total;        // groups to visit
+  __device__ __forceinline__ Span(const Sight& w, int lo, int hi) {
+    const int end = max(0, hi + 1);
+    const int groups = (end + 15) >> 4;
+    head_groups = 0;
+    skip = 0;
+    if (w.window != 0) {
+      const int left = max(0, lo - w.window + 1) >> 4;
+      const int head = (min(w.first, end) + 15) >> 4;
+      if (head < left) {
+        head_groups = head;
+        skip = min(left, groups) - head;
+      }
+    }
+    total = groups - skip;
+  }
+  __device__ __forceinline__ int slot(int i) const { return (i < head_groups ? i : i + skip) << 4; }
+};
+
+}  // namespace algx

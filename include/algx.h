@@ -335,6 +335,104 @@ ALGX_API int algx_aluglu_fwd(const void* gu, void* y, int64_t rows, int64_t ff, 
 ALGX_API int algx_aluglu_bwd(const void* gu, const void* dy, void* dgu, int64_t rows, int64_t ff, float beta,
                              void* stream);
 
+/* ------------------------------------------------------------------- serving */
+/* Keys and values of served sequences live in pages: k_pages, v_pages
+ * (num_pages, Hkv, page_size, D), D = 64, page_size a power of two from 16 to
+ * 256. table (B, max_pages) int32 names each sequence's pages, lens (B) int32
+ * its cached slots; slot s lies in page table[b][s / page_size] at row
+ * s % page_size. Entries of the table beyond a sequence's slots are not read.
+ * S = max_pages * page_size below. A page number, a length or a rotary position
+ * outside its range never leads to an access out of bounds: what it would have
+ * touched is skipped (a length is cut to S, a position to the tables' rows) and
+ * the device error word gets bit 8. The reference trains only; none of these
+ * entries has a counterpart there beyond the formulas cited. */
+
+/* New tokens into the cache: qkv (B, T, Hq + 2 Hkv, D) holds [q | k | v] heads
+ * per token. Token t of sequence b goes to slot lens[b] + t (lens: slots held
+ * before the call, not changed by it) and is rotated to position positions[b] + t
+ * (positions NULL: lens[b] + t). counts (B) or NULL: tokens t >= counts[b] are
+ * padding, stored nowhere and given zero queries. q (B, T, Hq, D) receives the
+ * queries. gain_q, gain_k (64) fp32 or both NULL: QK RMS norm (qk_norm.py:29-43,
+ * algebraic.py:76-83); rope_cos, rope_sin (rope_rows, 32) fp32 or both NULL
+ * (algebraic.py:172-179). Norm and rotation are evaluated in fp32 and rounded
+ * once. slot_positions (B, Hkv, S) int32 or NULL receives the positions of the
+ * new slots. Bytes: each row is read once and written once. */
+ALGX_API int algx_cache_append(const void* qkv, const float* gain_q, const float* gain_k, const float* rope_cos,
+                               const float* rope_sin, int64_t rope_rows, const int32_t* table, const int32_t* lens,
+                               const int32_t* positions, const int32_t* counts, void* q, void* k_pages,
+                               void* v_pages, int32_t* slot_positions, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                               int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t D, int32_t dtype,
+                               float eps, void* stream);
+
+typedef struct algx_paged_config {
+  int32_t kind;   /* ALGX_ATTN_ASINH or ALGX_ATTN_SOFTMAX */
+  int32_t n;      /* asinh weight power, a power of two >= 2 */
+  int32_t window; /* 0, or the newest slots a query sees, its own among them */
+  int32_t first;  /* first slots that stay visible under a window */
+  float scale;    /* 1/(sqrt(D)*unit), unit = c (asinh) or 1 (softmax) */
+  float inv_unit; /* 1/unit, multiplies the sink logits */
+} algx_paged_config;
+
+/* Bytes of workspace algx_paged_attn needs (no initialisation needed); scored:
+ * whether scores are given. No counterpart in the reference. */
+ALGX_API size_t algx_paged_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t page_size,
+                                               int64_t max_pages, int64_t window, int64_t first, int32_t scored);
+
+/* Attention of the T newest tokens of every sequence over its cached slots.
+ * q, o (B, T, Hq, D); Hq a multiple of Hkv, query head j reads kv head
+ * j / (Hq / Hkv). lens (B): cached slots, the T new ones included; query t sees
+ * slots up to lens[b] - T + t, under a window only those within it and the first
+ * ones. sink (Hq) fp32 logits or NULL. The asinh kind evaluates the dense function
+ * of algebraic.py:186-216 (the shifted branch of kernels/flash.py:240-284, any
+ * score range), the softmax kind standard.py:24-38. A row with nothing visible
+ * gives zeros. scores, scores_out (B, Hkv, S) fp32 or both NULL (they may be
+ * the same buffer): scores_out = scores + this call's normalised weights summed
+ * over the queries of each kv head; slots of the T new tokens start from 0, and
+ * slots beyond lens get 0. No counterpart in the reference for the cache. */
+ALGX_API int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_pages, const void* v_pages,
+                             const int32_t* table, const int32_t* lens, const float* sink, const float* scores,
+                             float* scores_out, void* o, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                             int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t D, int32_t dtype,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace algx_cache_evict needs. No counterpart in the reference. */
+ALGX_API size_t algx_cache_evict_workspace_size(int64_t B, int64_t Hkv, int64_t budget);
+
+/* Brings every sequence of more than `budget` slots down to it, per kv head:
+ * kept are the slots whose position (positions (B, Hkv, S) int32) is below
+ * `first` or among the newest `recent` positions, and of the others those with
+ * the highest scores ((B, Hkv, S) fp32; ties: the lower slot; NaN lowest). Kept
+ * rows at or above the budget move, in slot order, into the holes below it; all
+ * other rows stay where they are. new_lens (B), new_scores and new_positions
+ * (B, Hkv, S; 0 and -1 beyond the new length) describe the result, kept
+ * (B, Hkv, budget) the old slot of every new one (-1: none). The new arrays are
+ * buffers of their own, so a call repeated on the same inputs gives the same
+ * result. No counterpart in the reference. */
+ALGX_API int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const int32_t* lens,
+                              const float* scores, const int32_t* positions, int64_t budget, int64_t first,
+                              int64_t recent, int32_t* new_lens, float* new_scores, int32_t* new_positions,
+                              int32_t* kept, int64_t B, int64_t Hkv, int64_t num_pages, int64_t page_size,
+                              int64_t max_pages, int64_t D, int32_t dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Verification of K <= 31 drafted tokens per sequence and the draw of the next
+ * one. target (B, K + 1, V) and draft (B, K, V) logits (draft NULL: every draft
+ * is a certain proposal, q = 1 at its token); probabilities by softmax of
+ * scale * z (ALGX_HEAD_CE) or rho(scale * z)^n normalised (ALGX_HEAD_ALG_CE,
+ * algebraic.py:266-301), -inf and NaN logits having none. Token i is accepted
+ * while u[b][i] q_i(x_i) < p_i(x_i). The next token is
+ * argmax_v weight_v / race[b][v], the lowest index on ties, with weight
+ * max(p - q, 0) of the refused row, p where that is zero everywhere or every
+ * draft was accepted; race (B, V) holds exponential variates. counts (B) or
+ * NULL: drafts of each sequence, K at most. out (B, K + 1): accepted tokens,
+ * the next one, then -1; accepted (B). A draft token outside [0, V) is refused
+ * and sets bit 4 of the device error word. No counterpart in the reference
+ * (probabilities: algebraic.py:266-301). */
+ALGX_API int algx_verify_draft(int32_t kind, int32_t n, float scale, const void* target, const void* draft,
+                               const int32_t* tokens, const int32_t* counts, const float* u, const float* race,
+                               int32_t* out, int32_t* accepted, int64_t B, int64_t K, int64_t V, int32_t dtype,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,128 @@
+"""Draft verification against its 64-bit restatement (oracle/serving_math.py)."""
+
+import math
+
+import pytest
+import torch
+
+from algx import _lib as L
+from algx.kernels.verify import verify_draft
+from oracle import serving_math as O
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+BAD_LABEL = 4
+
+
+def inputs(B, K, V, dtype, kind, c, seed, spread=0.7, n=8):
+    """Drafts are drawn from the draft model's own probabilities, as the operator's contract says."""
+    g = torch.Generator().manual_seed(seed)
+    unit = c if kind == "alg_ce" else 1.0
+    base = 2 * torch.randn((B, K + 1, V), generator=g)
+    draft = base[:, :K] + spread * torch.randn((B, K, V), generator=g)
+    target, draft = (base * unit).to(dtype), (draft * unit).to(dtype)
+    logq = draft.float() if kind == "ce" else n * torch.asinh(draft.float() / c)
+    tokens = torch.empty((B, 0), dtype=torch.int32)
+    if K:
+        tokens = torch.multinomial(torch.softmax(logq, -1).reshape(-1, V), 1, generator=g).reshape(B, K).to(torch.int32)
+    u = torch.rand((B, K), generator=g)
+    race = (-torch.log1p(-torch.rand((B, V), generator=g))).clamp_min(1e-30)
+    return target, tokens, draft, u, race
+
+
+def check(target, tokens, draft, u, race, counts=None, **kw):
+    want, acc = O.verify_draft(target, tokens, draft, u, race, counts=counts, **kw)
+    dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    cd = None if counts is None else torch.tensor(counts, dtype=torch.int32).cuda()
+    out, got = verify_draft(dev(target), dev(tokens), dev(draft), dev(u), dev(race), counts=cd, **kw)
+    assert out.dtype == got.dtype == torch.int32
+    assert got.tolist() == acc and out.tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind,n,c", [("ce", 16, 16.0), ("alg_ce", 8, 2.0), ("alg_ce", 32, 16.0)])
+@pytest.mark.parametrize("B,K,V", [(1, 1, 1), (2, 4, 7), (3, 3, 257), (5, 7, 1000), (2, 31, 130), (2, 4, 50304),
+                                   (1, 5, 32001), (300, 2, 33)])
+def test_verify(B, K, V, kind, n, c, dtype):
+    check(*inputs(B, K, V, dtype, kind, c, 60 + V, n=n), kind=kind, n=n, c=c)
+
+
+@pytest.mark.parametrize("kind", ["ce", "alg_ce"])
+def test_sampling_without_drafts(kind):
+    target, tokens, _, u, race = inputs(6, 0, 999, F32, kind, 2.0, 1)
+    check(target, tokens, None, u, race, kind=kind, n=8, c=2.0)
+
+
+def test_certain_proposals_ragged_counts_and_temperature():
+    target, tokens, draft, u, race = inputs(6, 5, 300, BF16, "ce", 1.0, 2)
+    tokens = target[:, :5].float().argmax(-1).to(torch.int32)
+    check(target, tokens, None, u * 0.5, race)
+    check(target, tokens, draft, u, race, counts=[0, 1, 2, 3, 4, 5])
+    check(target, tokens, draft, u, race, counts=[5, 0, 99, -3, 1, 1])  # cut to 0 .. K
+    for t in (0.25, 3.0):
+        check(target, tokens, draft, u, race, temperature=t)
+
+
+def test_equal_models_accept_everything():
+    target, tokens, _, u, race = inputs(8, 6, 5000, BF16, "ce", 1.0, 3)
+    draft = target[:, :6].clone()
+    tokens = torch.multinomial(torch.softmax(draft.float(), -1).reshape(-1, 5000), 1).reshape(8, 6).to(torch.int32)
+    check(target, tokens, draft, u, race)
+    out, acc = verify_draft(target.cuda(), tokens.cuda(), draft.cuda(), u.cuda(), race.cuda())
+    assert acc.tolist() == [6] * 8
+
+
+def test_nothing_left_of_the_residual_falls_back_to_p():
+    """u = 1 refuses a draft of equal models, whose residual is zero everywhere."""
+    target, tokens, _, u, race = inputs(2, 2, 500, F32, "ce", 1.0, 4)
+    check(target, tokens, target[:, :2].clone(), torch.ones_like(u), race)
+
+
+@pytest.mark.parametrize("kind", ["ce", "alg_ce"])
+def test_masked_and_odd_logits(kind):
+    target, tokens, draft, u, race = inputs(4, 3, 600, F32, kind, 2.0, 5)
+    target[:, :, 100:] = -math.inf
+    draft[:, :, ::2] = -math.inf
+    target[1, :, 7] = math.nan
+    target[2] = -math.inf              # no probability anywhere: token 0
+    target[3, :, 50] = 1e4 if kind == "ce" else 1e15  # one token has it all
+    tokens[3] = 50
+    check(target, tokens, draft, u, race, kind=kind, n=16, c=2.0)
+
+
+def test_draft_tokens_outside_the_vocabulary_are_refused():
+    target, tokens, draft, u, race = inputs(3, 3, 400, BF16, "ce", 1.0, 6)
+    tokens[0, 0], tokens[1, 2] = -1, 400
+    L.device_error()
+    check(target, tokens, draft, u, race)
+    assert L.device_error() & BAD_LABEL
+
+
+def test_strided_logits_and_no_sequences():
+    target, tokens, draft, u, race = inputs(3, 2, 129, BF16, "ce", 1.0, 7)
+    wide = torch.zeros((3, 3, 200), dtype=BF16, device="cuda")
+    wide[..., :129] = target.cuda()
+    rest = [t.cuda() for t in (tokens, draft, u, race)]
+    a = verify_draft(wide[..., :129], *rest)
+    b = verify_draft(target.cuda(), *rest)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    out, acc = verify_draft(wide[:0, :, :129], *(t[:0] for t in rest))
+    assert out.shape == (0, 3) and acc.shape == (0,)
+
+
+def test_tokens_have_the_target_distribution():
+    """Over many seeds the first token is distributed as p, whatever the draft: each frequency
+    within six standard deviations of its probability."""
+    V, B = 8, 40000
+    g = torch.Generator().manual_seed(8)
+    p, q = torch.randn(V, generator=g), torch.randn(V, generator=g)
+    target = p.expand(B, 2, V).contiguous().cuda()
+    draft = q.expand(B, 1, V).contiguous().cuda()
+    tokens = torch.multinomial(torch.softmax(q, -1), B, replacement=True, generator=g).reshape(B, 1).to(torch.int32)
+    u = torch.rand((B, 1), generator=g)
+    race = torch.empty((B, V)).exponential_(generator=g)
+    out, _ = verify_draft(target, tokens.cuda(), draft, u.cuda(), race.cuda())
+    freq = torch.bincount(out[:, 0].cpu().long(), minlength=V) / B
+    prob = torch.softmax(p, -1)
+    assert bool(((freq - prob).abs() < 6 * torch.sqrt(prob * (1 - prob) / B)).all())
