@@ -193,12 +193,13 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
     q, table, lens = q.contiguous(), table.contiguous(), lens.contiguous()
     lib = L.lib()
     o = torch.empty_like(q)
-    nbytes = lib.algx_paged_attn_workspace_size(B, T, Hq, Hkv, size, maxp, cfg.window, first, scores is not None)
+    code = L.dtype_code(q.dtype)
+    nbytes = lib.algx_paged_attn_workspace_size(B, T, Hq, Hkv, size, maxp, cfg.window, first, scores is not None, code)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
     L.check(lib.algx_paged_attn(
         cfg, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.ptr(sink),
-        L.ptr(scores), L.ptr(scores_out), o.data_ptr(), B, T, Hq, Hkv, num, size, maxp, 64, L.dtype_code(q.dtype),
-        ws.data_ptr(), nbytes, L.stream_of(q)), "algx_paged_attn")
+        L.ptr(scores), L.ptr(scores_out), o.data_ptr(), B, T, Hq, Hkv, num, size, maxp, 64, code, ws.data_ptr(),
+        nbytes, L.stream_of(q)), "algx_paged_attn")
     return o if scores is None else (o, scores_out)
 
 

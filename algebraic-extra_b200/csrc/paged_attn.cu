@@ -4,7 +4,7 @@
 // Row (t, g) of kv head h is query token t of T under query head h G + g, with
 // G = Hq / Hkv. For its scores x_s = scale (q . k_s) over the visible slots,
 //
-//   asinh    w_s = rho(x_s)^n          softmax   w_s = exp(x_s)
+//   asinh    w_s = rho(x_s)^n          softmax   w_s = exp(x_s)   (2^x_s, log2(e) in scale)
 //   l = sum_s w_s + w(sink)            o = sum_s w_s v_s / l
 //
 // with every weight taken relative to a running reference score, so that no sum
@@ -22,7 +22,6 @@ constexpr int kD = 64;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMinGroups = 8;  // groups of 16 slots a split takes at least
-constexpr float kNegInf = -INFINITY;
 
 struct PagedAttnArgs {
   const void *q, *k, *v;
@@ -34,13 +33,73 @@ struct PagedAttnArgs {
   float* xs;        // (B, Hkv, rows, S) scores, when weights are accumulated
   int* err;
   int64_t slots;    // S: slots of one sequence's table
-  int T, G, rows, tiles, splits, log2n;
+  int T, G, rows, tile_rows, tiles, splits, log2n;
+  bool direct;      // one split and no scores: outputs are written without a join
   float scale, inv_unit;
   Sight sight;
 };
 
 // Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
 __device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// What one CTA works on.
+struct Work {
+  int b, h, split, r0, nr, len, lo, hi;
+  __device__ __forceinline__ Work(const PagedAttnArgs& a, const PagedView& pv) {
+    unsigned idx = blockIdx.x;
+    const unsigned tile = idx % (unsigned)a.tiles;
+    idx /= (unsigned)a.tiles;
+    split = (int)(idx % (unsigned)a.splits);
+    idx /= (unsigned)a.splits;
+    b = (int)(idx / (unsigned)pv.heads);
+    h = (int)(idx - (unsigned)b * (unsigned)pv.heads);
+    len = paged_len(pv, b, a.err);
+    r0 = (int)tile * a.tile_rows;
+    nr = min(a.tile_rows, a.rows - r0);
+    lo = len - a.T + r0 / a.G;
+    hi = len - a.T + (r0 + nr - 1) / a.G;
+  }
+  __device__ __forceinline__ int64_t kv(const PagedView& pv) const { return (int64_t)b * pv.heads + h; }
+  // Element offset / 64 of a row of q or o.
+  __device__ __forceinline__ int64_t q_row(const PagedAttnArgs& a, const PagedView& pv, int row) const {
+    const int t = row / a.G;
+    return (((int64_t)b * a.T + t) * pv.heads + h) * a.G + (row - t * a.G);
+  }
+};
+
+__device__ __forceinline__ float sink_score(const PagedAttnArgs& a, int h, int row) {
+  return a.sink ? a.sink[h * a.G + row % a.G] * a.inv_unit : kNegInf;
+}
+
+// Joins the CTA's PARTS partial results of each row: into the workspace, or, when
+// no other split has a share, into the output.
+template <typename T, int KIND, int PARTS>
+__device__ __forceinline__ void merge_parts(const PagedAttnArgs& a, const PagedView& pv, const Work& w,
+                                            const float* s_o, const float2* s_ml) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  for (int i = threadIdx.x; i < w.nr * kD; i += kThreads) {
+    const int r = i / kD, d = i % kD;
+    const float sink = a.direct ? sink_score(a, w.h, w.r0 + r) : kNegInf;
+    float M = sink;
+    for (int p = 0; p < PARTS; ++p) M = fmaxf(M, s_ml[r * PARTS + p].x);
+    const float t = weight_turn<KIND, EXACT>(M);
+    float L = sink == kNegInf ? 0.f : weight_of<KIND, EXACT>(sink, t, a.log2n), O = 0.f;
+    for (int p = 0; p < PARTS; ++p) {
+      const float2 ml = s_ml[r * PARTS + p];
+      if (ml.x == kNegInf && ml.y == 0.f) continue;
+      const float f = weight_of<KIND, EXACT>(ml.x, t, a.log2n);
+      L = fmaf(ml.y, f, L);
+      O = fmaf(s_o[(r * PARTS + p) * kD + d], f, O);
+    }
+    if (a.direct) {
+      static_cast<T*>(a.o)[w.q_row(a, pv, w.r0 + r) * kD + d] = from_f32<T>(O * row_scale(L));
+    } else {
+      const int64_t at = (w.kv(pv) * a.rows + w.r0 + r) * a.splits + w.split;
+      if (d == 0) a.part_ml[at] = make_float2(M, L);
+      a.part_o[at * kD + d] = O;
+    }
+  }
+}
 
 // ------------------------------------------------------- any I/O type, FMA units
 // One CTA per (split, row tile, kv head, sequence); a warp takes every fourth
@@ -55,50 +114,43 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
   __shared__ float s_o[R][kParts][kD];
   __shared__ float2 s_ml[R][kParts];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % V::TPR, rl = lane / V::TPR;
-  int64_t idx = blockIdx.x;
-  const int tile = (int)(idx % a.tiles);
-  idx /= a.tiles;
-  const int split = (int)(idx % a.splits);
-  idx /= a.splits;
-  const int h = (int)(idx % pv.heads), b = (int)(idx / pv.heads);
-  const int len = paged_len(pv, b, a.err);
-  const int r0 = tile * R, nr = min(R, a.rows - r0);
-  const int lo = len - a.T + r0 / a.G, hi = len - a.T + (r0 + nr - 1) / a.G;
-  const Span span(a.sight, lo, hi);
+  const Work w(a, pv);
+  const Span span(a.sight, w.lo, w.hi);
   const int per = max(kMinGroups, (span.total + a.splits - 1) / a.splits);
-  const int g_end = (int)min((int64_t)span.total, (int64_t)(split + 1) * per);
+  const int g_end = (int)min((int64_t)span.total, (int64_t)(w.split + 1) * per);
 
   float q[R][V::N];
   int last[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = min(r0 + r, a.rows - 1), t = row / a.G, g = row - t * a.G;
-    last[r] = r < nr ? len - a.T + t : -1;
-    const int64_t at = (((int64_t)b * a.T + t) * pv.heads + h) * a.G + g;
-    unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at * kD + sub * V::N), q[r]);
+    const int row = min(w.r0 + r, a.rows - 1);
+    last[r] = r < w.nr ? w.len - a.T + row / a.G : -1;
+    unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.q_row(a, pv, row) * kD + sub * V::N), q[r]);
   }
   float m[R], turn[R], l[R], acc[R][V::N];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = kNegInf;
-    turn[r] = 0.f;
+    turn[r] = weight_turn<KIND, EXACT>(kNegInf);
     l[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < V::N; ++i) acc[r][i] = 0.f;
   }
-  for (int64_t g = (int64_t)split * per + warp; g < g_end; g += kWarps) {
+  for (int64_t g = (int64_t)w.split * per + warp; g < g_end; g += kWarps) {
     const int base = span.slot((int)g);
-    const int pid = pv.table[(int64_t)b * pv.max_pages + (base >> pv.page_shift)];
+    const int pid = pv.table[(int64_t)w.b * pv.max_pages + (base >> pv.page_shift)];
     if (pid < 0 || pid >= pv.num_pages) {
       if (lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
+      if (a.xs != nullptr && lane < 16)
+        for (int r = 0; r < w.nr; ++r) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + base + lane] = kNegInf;
       continue;
     }
-    const int64_t at = paged_row(pv, pid, h, base) + sub * V::N;
+    const int64_t at = paged_row(pv, pid, w.h, base) + sub * V::N;
 #pragma unroll 2
     for (int j = 0; j < 16; j += V::RPW) {
       const int s = base + j + rl;
       float kf[V::N], vf[V::N];
-      const bool live = s < len;
+      const bool live = s < w.len;
       unpack<T>(live ? ld_stream(static_cast<const T*>(a.k) + at + (j + rl) * kD) : make_uint4(0, 0, 0, 0), kf);
       unpack<T>(live ? ld_stream(static_cast<const T*>(a.v) + at + (j + rl) * kD) : make_uint4(0, 0, 0, 0), vf);
       float xr[R];
@@ -114,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
         const float x = xr[r];
         if (!a.sight.sees(s, last[r])) continue;
         if (a.xs != nullptr && sub == 0)
-          a.xs[(((int64_t)b * pv.heads + h) * a.rows + r0 + r) * a.slots + s] = x;
+          a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + s] = x;
         if (x == kNegInf) continue;  // weight 0
         if (x > m[r]) {
           const float nt = weight_turn<KIND, EXACT>(x);
@@ -125,10 +177,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
 #pragma unroll
           for (int i = 0; i < V::N; ++i) acc[r][i] *= f;
         }
-        const float w = weight_of<KIND, EXACT>(x, turn[r], a.log2n);
-        l[r] += w;
+        const float p = weight_of<KIND, EXACT>(x, turn[r], a.log2n);
+        l[r] += p;
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) acc[r][i] = fmaf(w, vf[i], acc[r][i]);
+        for (int i = 0; i < V::N; ++i) acc[r][i] = fmaf(p, vf[i], acc[r][i]);
       }
     }
   }
@@ -140,23 +192,303 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
     for (int i = 0; i < V::N; ++i) s_o[r][part][sub * V::N + i] = acc[r][i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nr * kD; i += kThreads) {
-    const int r = i / kD, d = i % kD;
-    float M = kNegInf;
-    for (int p = 0; p < kParts; ++p) M = fmaxf(M, s_ml[r][p].x);
-    const float t = weight_turn<KIND, EXACT>(M);
-    float L = 0.f, O = 0.f;
-    for (int p = 0; p < kParts; ++p) {
-      const float2 ml = s_ml[r][p];
-      if (ml.x == kNegInf && ml.y == 0.f) continue;
-      const float f = weight_of<KIND, EXACT>(ml.x, t, a.log2n);
-      L = fmaf(ml.y, f, L);
-      O = fmaf(s_o[r][p][d], f, O);
+  merge_parts<T, KIND, kParts>(a, pv, w, &s_o[0][0][0], &s_ml[0][0]);
+}
+
+// ----------------------------------------------------- bfloat16, matrix units
+// Decoding reads every key and value once and does little with it, so this
+// kernel is built around the loads: keys and values go from memory straight into
+// the registers of the matrix instructions, without shared memory.
+//
+// A warp takes groups of 16 slots. For the scores the keys are the 16-row operand
+// (S^T = K Q^T, up to 8 query rows the other one), and the order of the 64
+// products is free, so each lane loads 16 contiguous bytes of a key where the
+// instruction would have it hold pairs 16 bytes apart: the queries are loaded in
+// the same order. For O^T = V^T P^T the values are the 16-row operand; a lane
+// loads eight contiguous elements of four slots and interleaves pairs of slots
+// with byte permutes, which only renames the output's rows. The scores come out
+// as (slot, row) and go in as (row, slot), one 8 x 8 transposition in registers.
+// mma.sync rather than tcgen05: at 8 to 32 rows the matrix work is a few percent
+// of either unit's rate, and tcgen05 would put keys, values and weights through
+// shared memory and the scores through TMEM.
+//
+// Weights are relative to a per-row reference that moves only when a weight
+// passes 2^8, so most groups need no reduction over lanes at all. Weights are
+// rounded to bf16 for the second product, as the forward kernels round them
+// (kernels/flash.py:262), while their sum keeps the unrounded ones.
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One group's keys and values in registers: k[0], k[1] the lane's 16-byte chunks
+// t and t + 4 of slot g, k[2], k[3] those of slot g + 8; v[i] chunk g of slots
+// 2t, 2t + 1, 2t + 8, 2t + 9 (g = lane / 4, t = lane % 4).
+struct Group {
+  uint4 k[4], v[4];
+  int base;  // first slot
+  int live;  // slots below it exist (0 when the page does not)
+};
+
+constexpr float kMove = 256.f;  // a weight above it moves the row's reference
+
+template <int KIND, int NT, bool ONE>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
+    paged_attn_mma_kernel(const PagedAttnArgs a, const PagedView pv) {
+  using T = __nv_bfloat16;
+  __shared__ float s_o[NT * 8 * kWarps * kD];
+  __shared__ float2 s_ml[NT * 8 * kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const Work w(a, pv);
+  const Span span(a.sight, w.lo, w.hi);
+  const int per = max(kMinGroups, (span.total + a.splits - 1) / a.splits);
+  const int g_end = (int)min((int64_t)span.total, (int64_t)(w.split + 1) * per);
+  const int32_t* table = pv.table + (int64_t)w.b * pv.max_pages;
+
+  // queries: rows 8 nt + g, chunks t and t + 4
+  uint32_t q[NT][8];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    if (r < w.nr) {
+      const T* row = static_cast<const T*>(a.q) + w.q_row(a, pv, w.r0 + r) * kD;
+      x = *reinterpret_cast<const uint4*>(row + t * 8);
+      y = *reinterpret_cast<const uint4*>(row + 32 + t * 8);
     }
-    const int64_t row = ((int64_t)b * pv.heads + h) * a.rows + r0 + r;
-    if (d == 0) a.part_ml[row * a.splits + split] = make_float2(M, L);
-    a.part_o[(row * a.splits + split) * kD + d] = O;
+    q[nt][0] = x.x; q[nt][1] = x.y; q[nt][2] = x.z; q[nt][3] = x.w;
+    q[nt][4] = y.x; q[nt][5] = y.y; q[nt][6] = y.z; q[nt][7] = y.w;
   }
+  // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
+  float m[NT][2], turn[NT][2], l[NT][2], o[NT][4][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      m[nt][c] = kNegInf;
+      turn[nt][c] = weight_turn<KIND, false>(kNegInf);
+      l[nt][c] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
+  }
+
+  auto page_of = [&](int grp) { return grp < g_end ? table[span.slot(grp) >> pv.page_shift] : -1; };
+  auto load = [&](Group& x, int grp, int pid) {
+    x.base = span.slot(grp);
+    const bool known = pid >= 0 && pid < pv.num_pages;
+    x.live = known ? w.len : 0;
+    if (!known && lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
+    const int64_t at = paged_row(pv, known ? pid : 0, w.h, x.base);
+    const T* k = static_cast<const T*>(a.k) + at + t * 8;
+    const T* v = static_cast<const T*>(a.v) + at + g * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int sk = g + (i >> 1) * 8, sv = 2 * t + (i & 1) + (i >> 1) * 8;
+      x.k[i] = x.base + sk < x.live ? ld_stream(k + sk * kD + (i & 1) * 32) : make_uint4(0, 0, 0, 0);
+      x.v[i] = x.base + sv < x.live ? ld_stream(v + sv * kD) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  // O^T += V^T P^T for the weights p (two packed pairs a tile)
+  auto add_values = [&](const uint4 (&v)[4], const uint32_t (&p)[NT][2]) {
+    uint32_t b[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      b[nt][0] = transpose_8x8(p[nt][0]);
+      b[nt][1] = transpose_8x8(p[nt][1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t v0 = reinterpret_cast<const uint32_t*>(&v[0])[j], v1 = reinterpret_cast<const uint32_t*>(&v[1])[j];
+      const uint32_t v2 = reinterpret_cast<const uint32_t*>(&v[2])[j], v3 = reinterpret_cast<const uint32_t*>(&v[3])[j];
+      const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
+      const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][j], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+    }
+  };
+  auto last_of = [&](int r) { return w.len - a.T + (w.r0 + r) / a.G; };
+
+  auto compute = [&](const Group& x) {
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const uint32_t* lo = reinterpret_cast<const uint32_t*>(&x.k[step >> 1]) + (step & 1) * 2;
+        const uint32_t* hi = reinterpret_cast<const uint32_t*>(&x.k[2 + (step >> 1)]) + (step & 1) * 2;
+        mma_16816(s[nt], lo[0], hi[0], lo[1], hi[1], q[nt][2 * step], q[nt][2 * step + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] *= a.scale;
+    }
+    const bool whole = x.base + 16 <= x.live && a.sight.sees_group(x.base, w.lo, w.hi);
+    if (!whole) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int slot = x.base + g + (i >> 1) * 8;
+          if (slot >= x.live || !a.sight.sees(slot, last_of(nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
+        }
+    }
+    if (a.xs != nullptr) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = nt * 8 + 2 * t + (i & 1), slot = x.base + g + (i >> 1) * 8;
+          if (r < w.nr) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + slot] = s[nt][i];
+        }
+    }
+    float p[NT][4];
+    bool move = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (ONE && (i & 1)) {
+          p[nt][i] = 0.f;
+          continue;
+        }
+        p[nt][i] = weight_of<KIND, false>(s[nt][i], turn[nt][i & 1], a.log2n);
+        move = move || p[nt][i] > kMove;
+      }
+    if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (ONE && c) continue;
+          float top = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          if (top > m[nt][c]) {
+            const float nt_turn = weight_turn<KIND, false>(top);
+            const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND, false>(m[nt][c], nt_turn, a.log2n);
+            m[nt][c] = top;
+            turn[nt][c] = nt_turn;
+            l[nt][c] *= f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[nt][j][c] *= f;
+              o[nt][j][c + 2] *= f;
+            }
+            p[nt][c] = weight_of<KIND, false>(s[nt][c], nt_turn, a.log2n);
+            p[nt][c + 2] = weight_of<KIND, false>(s[nt][c + 2], nt_turn, a.log2n);
+          }
+        }
+    }
+    uint32_t pk[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt][0] += p[nt][0] + p[nt][2];
+      if (!ONE) l[nt][1] += p[nt][1] + p[nt][3];
+      pk[nt][0] = pack_pair(p[nt][0], p[nt][1]);
+      pk[nt][1] = pack_pair(p[nt][2], p[nt][3]);
+    }
+    if (!whole && w.lo != w.hi) {
+      // Rows of different tokens see different slots of this group. A weight of
+      // zero does not hide an infinity or NaN in a value, so such a group is
+      // added token by token, the values the token does not see set to zero.
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t* v = reinterpret_cast<const uint32_t*>(&x.v[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          odd = odd || (v[j] & 0x7f80u) == 0x7f80u || (v[j] & 0x7f800000u) == 0x7f800000u;
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+        for (int last = w.lo; last <= w.hi; ++last) {
+          uint4 v[4];
+          uint32_t only[NT][2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = a.sight.sees(x.base + 2 * t + (i & 1) + (i >> 1) * 8, last) ? x.v[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t mask = (last_of(nt * 8 + 2 * t) == last ? 0xffffu : 0u) |
+                                  (last_of(nt * 8 + 2 * t + 1) == last ? 0xffff0000u : 0u);
+            only[nt][0] = pk[nt][0] & mask;
+            only[nt][1] = pk[nt][1] & mask;
+          }
+          // rows of other tokens add zero times a finite or an unseen value of
+          // this token: they must not meet its infinities, so their own sums are
+          // put back afterwards
+          float keep[NT][4][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) keep[nt][j][i] = o[nt][j][i];
+          add_values(v, only);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (last_of(nt * 8 + 2 * t + (i & 1)) != last) o[nt][j][i] = keep[nt][j][i];
+        }
+        return;
+      }
+    }
+    add_values(x.v, pk);
+  };
+
+  // Two groups in registers, the next one's loads issued before the current one
+  // is worked on, page numbers one group further ahead.
+  int grp = (int)min((int64_t)g_end, (int64_t)w.split * per + warp);
+  Group x, y;
+  int pid = page_of(grp), next = page_of(grp + kWarps);
+  if (grp < g_end) load(x, grp, pid);
+  while (grp < g_end) {
+    pid = page_of(grp + 2 * kWarps);
+    if (grp + kWarps < g_end) load(y, grp + kWarps, next);
+    compute(x);
+    grp += kWarps;
+    if (grp >= g_end) break;
+    next = page_of(grp + 2 * kWarps);
+    if (grp + kWarps < g_end) load(x, grp + kWarps, pid);
+    compute(y);
+    grp += kWarps;
+  }
+  pdl_trigger();
+
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+      const int r = nt * 8 + 2 * t + c;
+      if (g == 0) s_ml[r * kWarps + warp] = make_float2(m[nt][c], l[nt][c]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float* at = s_o + (r * kWarps + warp) * kD + 8 * g + 2 * j;
+        *reinterpret_cast<float2*>(at) = make_float2(o[nt][j][c], o[nt][j][c + 2]);
+      }
+    }
+  }
+  __syncthreads();
+  merge_parts<T, KIND, kWarps>(a, pv, w, s_o, s_ml);
 }
 
 // ------------------------------------------------------------------------ join
@@ -165,45 +497,55 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
 constexpr int kScoreSlots = 1024;
 constexpr int kRowChunk = 64;
 
+// Reference and sum of one row over its splits and the sink, by one warp.
 template <int KIND, bool EXACT>
-__device__ __forceinline__ void join_row(const PagedAttnArgs& a, int64_t row, float sink, float& M, float& L) {
-  M = sink;  // -inf without a sink
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[row * a.splits + s].x);
-  const float t = weight_turn<KIND, EXACT>(M);
-  L = sink == kNegInf ? 0.f : weight_of<KIND, EXACT>(sink, t, a.log2n);
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[row * a.splits + s];
-    if (ml.x == kNegInf && ml.y == 0.f) continue;
-    L = fmaf(ml.y, weight_of<KIND, EXACT>(ml.x, t, a.log2n), L);
+__device__ __forceinline__ void join_row(const PagedAttnArgs& a, int64_t row, float sink, float& turn, float& L) {
+  const int lane = threadIdx.x & 31;
+  const float2* ml = a.part_ml + row * a.splits;
+  float M = sink;  // -inf without a sink
+  for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, ml[s].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  turn = weight_turn<KIND, EXACT>(M);
+  L = lane == 0 && sink != kNegInf ? weight_of<KIND, EXACT>(sink, turn, a.log2n) : 0.f;
+  for (int s = lane; s < a.splits; s += 32) {
+    const float2 x = ml[s];
+    if (x.x != kNegInf || x.y != 0.f) L = fmaf(x.y, weight_of<KIND, EXACT>(x.x, turn, a.log2n), L);
   }
+  L = row_sum<32>(L);
 }
 
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArgs a, const PagedView pv, int blocks) {
   constexpr bool EXACT = sizeof(T) == 4;
-  const int64_t bh = blockIdx.x / blocks;
+  constexpr int kQuads = kD / 4, kGroups = kThreads / kQuads;
+  pdl_wait();
+  const int64_t bh = blockIdx.x / (unsigned)blocks;
   const int which = (int)(blockIdx.x - bh * blocks);
   const int h = (int)(bh % pv.heads), b = (int)(bh / pv.heads);
   if (which < a.rows) {
-    __shared__ float s_half[kD];
+    __shared__ float4 s_part[kGroups][kQuads];
     const int64_t row = bh * a.rows + which;
-    const int t = which / a.G, g = which - t * a.G;
-    const float sink = a.sink ? a.sink[h * a.G + g] * a.inv_unit : kNegInf;
-    float M, L, O = 0.f;
-    join_row<KIND, EXACT>(a, row, sink, M, L);
-    const float turn = weight_turn<KIND, EXACT>(M);
-    const int d = threadIdx.x % kD, half = threadIdx.x / kD;
-    for (int s = half; s < a.splits; s += kThreads / kD) {
+    float turn, L;
+    join_row<KIND, EXACT>(a, row, sink_score(a, h, which), turn, L);
+    const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = grp; s < a.splits; s += kGroups) {
       const float2 ml = a.part_ml[row * a.splits + s];
-      if (ml.x == kNegInf && ml.y == 0.f) continue;
-      O = fmaf(a.part_o[(row * a.splits + s) * kD + d], weight_of<KIND, EXACT>(ml.x, turn, a.log2n), O);
+      const float4 x = reinterpret_cast<const float4*>(a.part_o)[(row * a.splits + s) * kQuads + quad];
+      const float f = ml.x == kNegInf && ml.y == 0.f ? 0.f : weight_of<KIND, EXACT>(ml.x, turn, a.log2n);
+      O.x = fmaf(x.x, f, O.x); O.y = fmaf(x.y, f, O.y); O.z = fmaf(x.z, f, O.z); O.w = fmaf(x.w, f, O.w);
     }
-    if (half == 1) s_half[d] = O;
+    s_part[grp][quad] = O;
     __syncthreads();
-    if (half == 0) {
-      O = (O + s_half[d]) * row_scale(L);
+    if (threadIdx.x < kD) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) sum += reinterpret_cast<const float*>(s_part[i])[threadIdx.x];
+      const int t = which / a.G, g = which - t * a.G;
       const int64_t at = (((int64_t)b * a.T + t) * pv.heads + h) * a.G + g;
-      static_cast<T*>(a.o)[at * kD + d] = from_f32<T>(O);
+      static_cast<T*>(a.o)[at * kD + threadIdx.x] = from_f32<T>(sum * row_scale(L));
     }
     return;
   }
@@ -216,12 +558,10 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
   for (int r0 = 0; r0 < a.rows; r0 += kRowChunk) {
     const int nr = min(kRowChunk, a.rows - r0);
     __syncthreads();
-    for (int r = threadIdx.x; r < nr; r += kThreads) {
-      const int g = (r0 + r) % a.G;
-      const float sink = a.sink ? a.sink[h * a.G + g] * a.inv_unit : kNegInf;
-      float M, L;
-      join_row<KIND, EXACT>(a, bh * a.rows + r0 + r, sink, M, L);
-      s_turn[r] = weight_turn<KIND, EXACT>(M);
+    for (int r = threadIdx.x >> 5; r < nr; r += kWarps) {
+      float turn, L;
+      join_row<KIND, EXACT>(a, bh * a.rows + r0 + r, sink_score(a, h, r0 + r), turn, L);
+      s_turn[r] = turn;
       s_inv[r] = row_scale(L);
     }
     __syncthreads();
@@ -258,10 +598,14 @@ int64_t visible_groups(int64_t S, int64_t T, int64_t window, int64_t first) {
   return std::min(all, (window + T + 15) / 16 + 1 + (std::min(first, S) + 15) / 16);
 }
 
-Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, int64_t window, int64_t first, bool scored) {
+Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, int64_t window, int64_t first, bool scored,
+               bool wide) {
   Plan p = {};
   p.rows = T * (Hq / Hkv);
-  p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
+  if (wide)  // bf16: tiles of up to 32 rows, as even as they come
+    p.tile_rows = (((p.rows + 31) / 32 - 1 + p.rows) / ((p.rows + 31) / 32) + 7) / 8 * 8;
+  else
+    p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t groups = visible_groups(S, T, window, first);
   const int64_t base = std::max<int64_t>(1, B * Hkv * p.tiles);
@@ -279,15 +623,25 @@ template <typename T, int KIND>
 int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int64_t B, cudaStream_t st) {
   const int64_t grid = B * pv.heads * p.splits * p.tiles;
   ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
-  auto* kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
-               : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>
-               : p.tile_rows == 4 ? paged_attn_kernel<T, KIND, 4>
-                                  : paged_attn_kernel<T, KIND, 8>;
+  void (*kern)(PagedAttnArgs, PagedView);
+  if constexpr (sizeof(T) == 2)
+    kern = p.rows == 1         ? paged_attn_mma_kernel<KIND, 1, true>
+           : p.tile_rows == 8  ? paged_attn_mma_kernel<KIND, 1, false>
+           : p.tile_rows == 16 ? paged_attn_mma_kernel<KIND, 2, false>
+           : p.tile_rows == 24 ? paged_attn_mma_kernel<KIND, 3, false>
+                               : paged_attn_mma_kernel<KIND, 4, false>;
+  else
+    kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
+           : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>
+           : p.tile_rows == 4 ? paged_attn_kernel<T, KIND, 4>
+                              : paged_attn_kernel<T, KIND, 8>;
   kern<<<(unsigned)grid, kThreads, 0, st>>>(a, pv);
   ALGX_LAUNCHED("paged_attn_kernel");
+  if (a.direct) return ALGX_OK;
   const int64_t blocks = a.rows + (a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0);
   ALGX_REQUIRE(blocks * B * pv.heads <= INT32_MAX, "too many rows");
-  paged_join_kernel<T, KIND><<<(unsigned)(blocks * B * pv.heads), kThreads, 0, st>>>(a, pv, (int)blocks);
+  ALGX_CUDA(launch_dependent(paged_join_kernel<T, KIND>, dim3((unsigned)(blocks * B * pv.heads)), dim3(kThreads), 0, st,
+                             a, pv, (int)blocks));
   ALGX_LAUNCHED("paged_join_kernel");
   return ALGX_OK;
 }
@@ -298,9 +652,11 @@ int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int
 extern "C" {
 
 size_t algx_paged_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t page_size,
-                                      int64_t max_pages, int64_t window, int64_t first, int32_t scored) {
+                                      int64_t max_pages, int64_t window, int64_t first, int32_t scored,
+                                      int32_t dtype) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || page_size <= 0 || max_pages <= 0) return 0;
-  return algx::make_plan(B, T, Hq, Hkv, page_size * max_pages, window, first, scored != 0).bytes;
+  return algx::make_plan(B, T, Hq, Hkv, page_size * max_pages, window, first, scored != 0,
+                         dtype == ALGX_BF16).bytes;
 }
 
 int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_pages, const void* v_pages,
@@ -325,7 +681,7 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
                "tensors must be 16-byte aligned");
   ALGX_REQUIRE(T * (Hq / Hkv) <= INT32_MAX / 64, "too many rows");
   const int64_t S = page_size * max_pages;
-  const Plan p = make_plan(B, T, Hq, Hkv, S, cfg->window, cfg->first, scores != nullptr);
+  const Plan p = make_plan(B, T, Hq, Hkv, S, cfg->window, cfg->first, scores != nullptr, dtype == ALGX_BF16);
   ALGX_REQUIRE(workspace && workspace_bytes >= p.bytes, "workspace too small");
   PagedAttnArgs a = {};
   a.q = q; a.k = k_pages; a.v = v_pages; a.sink = sink; a.scores = scores; a.scores_out = scores_out; a.o = o;
@@ -338,10 +694,13 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   a.slots = S; a.T = (int)T; a.G = (int)(Hq / Hkv); a.rows = (int)p.rows; a.tiles = (int)p.tiles;
   a.splits = (int)p.splits;
   while ((1 << a.log2n) < cfg->n) ++a.log2n;
-  a.scale = cfg->scale; a.inv_unit = cfg->inv_unit;
+  const bool soft = cfg->kind == ALGX_ATTN_SOFTMAX;
+  a.scale = soft ? cfg->scale * kLog2e : cfg->scale;
+  a.inv_unit = soft ? cfg->inv_unit * kLog2e : cfg->inv_unit;
+  a.tile_rows = (int)p.tile_rows;
+  a.direct = p.splits == 1 && scores == nullptr;
   a.sight = {cfg->window, cfg->first};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool soft = cfg->kind == ALGX_ATTN_SOFTMAX;
   if (dtype == ALGX_BF16)
     return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, p, B, st)
                 : paged_launch<__nv_bfloat16, kAsinh>(a, pv, p, B, st);

@@ -65,20 +65,29 @@ __device__ __forceinline__ float pow_log2(float x, int log2n) {
 }
 
 // Weight of a score x against a reference score m: (rho(x) rho(-m))^n for the
-// asinh kind, exp(x - m) for softmax. `turn` is the reference's part, computed
-// once per reference. m = -inf (no score seen yet) gives an infinite weight to
-// any finite x.
+// asinh kind, 2^(x - m) for softmax, whose scores carry a factor log2(e). `turn`
+// is the reference's part, computed once per reference; before any score is seen
+// (m = -inf) it is so large that every finite score has a huge weight, and a
+// masked one (x = -inf) none.
 constexpr int kAsinh = ALGX_ATTN_ASINH, kSoftmax = ALGX_ATTN_SOFTMAX;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -INFINITY;
 
 template <int KIND, bool EXACT>
 __device__ __forceinline__ float weight_turn(float m) {
-  if constexpr (KIND == kAsinh) return rho_any<EXACT>(-m);
-  else return m;
+  if constexpr (KIND == kAsinh) return m == kNegInf ? 3e38f : rho_any<EXACT>(-m);
+  else return m == kNegInf ? -3e38f : m;
 }
 template <int KIND, bool EXACT>
 __device__ __forceinline__ float weight_of(float x, float turn, int log2n) {
-  if constexpr (KIND == kSoftmax) return EXACT ? expf(x - turn) : __expf(x - turn);
-  else return pow_log2(rho_any<EXACT>(x) * turn, log2n);
+  if constexpr (KIND == kSoftmax) {
+    if constexpr (EXACT) return exp2f(x - turn);
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x - turn));
+    return y;
+  } else {
+    return pow_log2(rho_any<EXACT>(x) * turn, log2n);
+  }
 }
 
 // Which slots a query sees. Query token t of T new ones stands at slot

@@ -29,7 +29,6 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
 constexpr int kMaxDraft = 32;
-constexpr float kNegInf = -INFINITY;
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -39,7 +38,7 @@ struct VerifyArgs {
   int* err;
   int64_t V, slice;  // slice: vocabulary columns of one CTA, a multiple of 8
   int K, log2n;
-  float scale;  // 1 / temperature (ce) or 1 / c (alg_ce)
+  float scale;  // log2(e) / temperature (ce) or 1 / c (alg_ce)
 };
 
 // Running reference and sum of one lane over one row's elements.
@@ -217,7 +216,8 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   ALGX_REQUIRE((((uintptr_t)target | (uintptr_t)draft) & 3) == 0, "logits must be 4-byte aligned");
   VerifyArgs a = {};
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
-  a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K; a.scale = scale;
+  a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;
+  a.scale = kind == ALGX_HEAD_CE ? scale * kLog2e : scale;
   a.slice = ((V + kCluster - 1) / kCluster + 7) / 8 * 8;
   while ((1 << a.log2n) < n) ++a.log2n;
   a.err = device_error_word();
