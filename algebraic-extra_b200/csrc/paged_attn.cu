@@ -11,6 +11,7 @@
 // overflows (algebraic.py:186-204; the shifted form of kernels/flash.py:240-284).
 // A row that sees no slot, or whose weights are all zero, gives zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_common.cuh"
 #include "vec_io.cuh"
@@ -243,10 +244,13 @@ struct Group {
 
 constexpr float kMove = 256.f;  // a weight above it moves the row's reference
 
-template <int KIND, int NT, bool ONE>
+template <int KIND, int LOG2N, int NT, bool ONE>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
     paged_attn_mma_kernel(const PagedAttnArgs a, const PagedView pv) {
   using T = __nv_bfloat16;
+  // Scores are worked on in pairs: of both columns of a lane, or, with a single
+  // row (only the first column counts), of its two slots.
+  constexpr int NP = ONE ? 1 : 2;
   __shared__ float s_o[NT * 8 * kWarps * kD];
   __shared__ float2 s_ml[NT * 8 * kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -271,39 +275,48 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
     q[nt][4] = y.x; q[nt][5] = y.y; q[nt][6] = y.z; q[nt][7] = y.w;
   }
   // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
-  float m[NT][2], turn[NT][2], l[NT][2], o[NT][4][4];
+  float m[NT][2], o[NT][4][4];
+  float2 turn[NT], l[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      m[nt][c] = kNegInf;
-      turn[nt][c] = weight_turn<KIND, false>(kNegInf);
-      l[nt][c] = 0.f;
-    }
+    m[nt][0] = m[nt][1] = kNegInf;
+    turn[nt].x = turn[nt].y = weight_turn<KIND, false>(kNegInf);
+    l[nt] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
   }
 
+  const int64_t kv_lane = g * kD + t * 8, v_lane = 2 * t * kD + g * 8;
   auto page_of = [&](int grp) { return grp < g_end ? table[span.slot(grp) >> pv.page_shift] : -1; };
   auto load = [&](Group& x, int grp, int pid) {
     x.base = span.slot(grp);
-    const bool known = pid >= 0 && pid < pv.num_pages;
+    const bool known = (unsigned)pid < (unsigned)pv.num_pages;
     x.live = known ? w.len : 0;
-    if (!known && lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
     const int64_t at = paged_row(pv, known ? pid : 0, w.h, x.base);
-    const T* k = static_cast<const T*>(a.k) + at + t * 8;
-    const T* v = static_cast<const T*>(a.v) + at + g * 8;
+    const T* k = static_cast<const T*>(a.k) + at + kv_lane;
+    const T* v = static_cast<const T*>(a.v) + at + v_lane;
+    if (x.base + 16 <= x.live) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x.k[i] = ld_stream(k + (i >> 1) * 8 * kD + (i & 1) * 32);
+        x.v[i] = ld_stream(v + ((i & 1) + (i >> 1) * 8) * kD);
+      }
+      return;
+    }
+    if (!known && lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int sk = g + (i >> 1) * 8, sv = 2 * t + (i & 1) + (i >> 1) * 8;
-      x.k[i] = x.base + sk < x.live ? ld_stream(k + sk * kD + (i & 1) * 32) : make_uint4(0, 0, 0, 0);
-      x.v[i] = x.base + sv < x.live ? ld_stream(v + sv * kD) : make_uint4(0, 0, 0, 0);
+      x.k[i] = x.base + sk < x.live ? ld_stream(k + (i >> 1) * 8 * kD + (i & 1) * 32) : make_uint4(0, 0, 0, 0);
+      x.v[i] = x.base + sv < x.live ? ld_stream(v + ((i & 1) + (i >> 1) * 8) * kD) : make_uint4(0, 0, 0, 0);
     }
   };
-  // O^T += V^T P^T for the weights p (two packed pairs a tile)
-  auto add_values = [&](const uint4 (&v)[4], const uint32_t (&p)[NT][2]) {
+  auto last_of = [&](int r) { return w.len - a.T + (w.r0 + r) / a.G; };
+  // O^T += V^T P^T for the weights p (two packed pairs a tile); with `only`, for
+  // the rows of the token whose last visible slot it is.
+  auto add_values = [&](const uint4 (&v)[4], const uint32_t (&p)[NT][2], auto one_token, int only) {
     uint32_t b[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -317,25 +330,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
       const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][j], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (decltype(one_token)::value) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16816(sum, a0, a1, a2, a3, b[nt][0], b[nt][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (last_of(nt * 8 + 2 * t + (i & 1)) == only) o[nt][j][i] += sum[i];
+        } else {
+          mma_16816(o[nt][j], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+        }
+      }
     }
   };
-  auto last_of = [&](int r) { return w.len - a.T + (w.r0 + r) / a.G; };
+  // pair i of a tile's four scores, and its reference
+  auto pair = [&](const float (&s)[4], int i) { return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]); };
+  auto turns = [&](int nt) { return ONE ? make_float2(turn[nt].x, turn[nt].x) : turn[nt]; };
 
   auto compute = [&](const Group& x) {
     float s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      float s2[4];  // a second chain of products, for a shorter one
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[nt][i] = s2[i] = 0.f;
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
         const uint32_t* lo = reinterpret_cast<const uint32_t*>(&x.k[step >> 1]) + (step & 1) * 2;
         const uint32_t* hi = reinterpret_cast<const uint32_t*>(&x.k[2 + (step >> 1)]) + (step & 1) * 2;
-        mma_16816(s[nt], lo[0], hi[0], lo[1], hi[1], q[nt][2 * step], q[nt][2 * step + 1]);
+        mma_16816(step & 1 ? s2 : s[nt], lo[0], hi[0], lo[1], hi[1], q[nt][2 * step], q[nt][2 * step + 1]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] *= a.scale;
+      for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[i]) * a.scale;
     }
     const bool whole = x.base + 16 <= x.live && a.sight.sees_group(x.base, w.lo, w.hi);
     if (!whole) {
@@ -356,51 +382,48 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
           if (r < w.nr) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + slot] = s[nt][i];
         }
     }
-    float p[NT][4];
-    bool move = false;
+    float2 p[NT][NP];
+    float high = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (ONE && (i & 1)) {
-          p[nt][i] = 0.f;
-          continue;
-        }
-        p[nt][i] = weight_of<KIND, false>(s[nt][i], turn[nt][i & 1], a.log2n);
-        move = move || p[nt][i] > kMove;
+      for (int i = 0; i < NP; ++i) {
+        p[nt][i] = weight_pair<KIND, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
+        high = fmaxf(high, fmaxf(p[nt][i].x, p[nt][i].y));
       }
-    if (__any_sync(0xffffffffu, move)) {
+    if (__any_sync(0xffffffffu, high > kMove)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (ONE && c) continue;
+        for (int c = 0; c < NP; ++c) {
           float top = fmaxf(s[nt][c], s[nt][c + 2]);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           if (top > m[nt][c]) {
-            const float nt_turn = weight_turn<KIND, false>(top);
-            const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND, false>(m[nt][c], nt_turn, a.log2n);
+            const float to = weight_turn<KIND, false>(top);
+            const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND, false>(m[nt][c], to, a.log2n);
             m[nt][c] = top;
-            turn[nt][c] = nt_turn;
-            l[nt][c] *= f;
+            (c ? turn[nt].y : turn[nt].x) = to;
+            (c ? l[nt].y : l[nt].x) *= f;
+            if (ONE) l[nt].y *= f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               o[nt][j][c] *= f;
               o[nt][j][c + 2] *= f;
             }
-            p[nt][c] = weight_of<KIND, false>(s[nt][c], nt_turn, a.log2n);
-            p[nt][c + 2] = weight_of<KIND, false>(s[nt][c + 2], nt_turn, a.log2n);
           }
         }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) p[nt][i] = weight_pair<KIND, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
+      }
     }
     uint32_t pk[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      l[nt][0] += p[nt][0] + p[nt][2];
-      if (!ONE) l[nt][1] += p[nt][1] + p[nt][3];
-      pk[nt][0] = pack_pair(p[nt][0], p[nt][1]);
-      pk[nt][1] = pack_pair(p[nt][2], p[nt][3]);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) l[nt] = add2(l[nt], p[nt][i]);
+      pk[nt][0] = ONE ? pack_pair(p[nt][0].x, 0.f) : pack_pair(p[nt][0].x, p[nt][0].y);
+      pk[nt][1] = ONE ? pack_pair(p[nt][0].y, 0.f) : pack_pair(p[nt][NP - 1].x, p[nt][NP - 1].y);
     }
     if (!whole && w.lo != w.hi) {
       // Rows of different tokens see different slots of this group. A weight of
@@ -417,40 +440,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       if (__any_sync(0xffffffffu, odd)) {
         for (int last = w.lo; last <= w.hi; ++last) {
           uint4 v[4];
-          uint32_t only[NT][2];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             v[i] = a.sight.sees(x.base + 2 * t + (i & 1) + (i >> 1) * 8, last) ? x.v[i] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t mask = (last_of(nt * 8 + 2 * t) == last ? 0xffffu : 0u) |
-                                  (last_of(nt * 8 + 2 * t + 1) == last ? 0xffff0000u : 0u);
-            only[nt][0] = pk[nt][0] & mask;
-            only[nt][1] = pk[nt][1] & mask;
-          }
-          // rows of other tokens add zero times a finite or an unseen value of
-          // this token: they must not meet its infinities, so their own sums are
-          // put back afterwards
-          float keep[NT][4][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) keep[nt][j][i] = o[nt][j][i];
-          add_values(v, only);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (last_of(nt * 8 + 2 * t + (i & 1)) != last) o[nt][j][i] = keep[nt][j][i];
+          add_values(v, pk, std::true_type{}, last);
         }
         return;
       }
     }
-    add_values(x.v, pk);
+    add_values(x.v, pk, std::false_type{}, 0);
   };
 
   // Two groups in registers, the next one's loads issued before the current one
@@ -476,10 +474,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      float sum = c ? (ONE ? 0.f : l[nt].y) : (ONE ? l[nt].x + l[nt].y : l[nt].x);
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+      for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       const int r = nt * 8 + 2 * t + c;
-      if (g == 0) s_ml[r * kWarps + warp] = make_float2(m[nt][c], l[nt][c]);
+      if (g == 0) s_ml[r * kWarps + warp] = make_float2(m[nt][c], sum);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float* at = s_o + (r * kWarps + warp) * kD + 8 * g + 2 * j;
@@ -619,17 +618,22 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, int64_t
   return p;
 }
 
+template <int KIND, int LOG2N>
+auto mma_kernel(const Plan& p) -> void (*)(PagedAttnArgs, PagedView) {
+  return p.rows == 1         ? paged_attn_mma_kernel<KIND, LOG2N, 1, true>
+         : p.tile_rows == 8  ? paged_attn_mma_kernel<KIND, LOG2N, 1, false>
+         : p.tile_rows == 16 ? paged_attn_mma_kernel<KIND, LOG2N, 2, false>
+         : p.tile_rows == 24 ? paged_attn_mma_kernel<KIND, LOG2N, 3, false>
+                             : paged_attn_mma_kernel<KIND, LOG2N, 4, false>;
+}
+
 template <typename T, int KIND>
 int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int64_t B, cudaStream_t st) {
   const int64_t grid = B * pv.heads * p.splits * p.tiles;
   ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
   void (*kern)(PagedAttnArgs, PagedView);
   if constexpr (sizeof(T) == 2)
-    kern = p.rows == 1         ? paged_attn_mma_kernel<KIND, 1, true>
-           : p.tile_rows == 8  ? paged_attn_mma_kernel<KIND, 1, false>
-           : p.tile_rows == 16 ? paged_attn_mma_kernel<KIND, 2, false>
-           : p.tile_rows == 24 ? paged_attn_mma_kernel<KIND, 3, false>
-                               : paged_attn_mma_kernel<KIND, 4, false>;
+    kern = KIND == kAsinh && a.log2n == 4 ? mma_kernel<KIND, 4>(p) : mma_kernel<KIND, 0>(p);
   else
     kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
            : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>

@@ -90,6 +90,35 @@ __device__ __forceinline__ float weight_of(float x, float turn, int log2n) {
   }
 }
 
+// The same weights for two scores at once on packed fp32 pairs, MUFU forms.
+// LOG2N > 0: the power is known when compiling.
+template <int KIND, int LOG2N>
+__device__ __forceinline__ float2 weight_pair(float2 x, float2 turn, int log2n) {
+  float2 y;
+  if constexpr (KIND == kSoftmax) {
+    y = sub2(x, turn);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(y.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(y.y));
+    return y;
+  } else {
+    y = fma2(x, x, make_float2(1.f, 1.f));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(y.x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(y.y));
+    y.x += fabsf(x.x);
+    y.y += fabsf(x.y);
+    y.x = x.x >= 0.f ? y.x : rcp_fast(y.x);
+    y.y = x.y >= 0.f ? y.y : rcp_fast(y.y);
+    y = mul2(y, turn);
+    if constexpr (LOG2N > 0) {
+#pragma unroll
+      for (int i = 0; i < LOG2N; ++i) y = mul2(y, y);
+    } else {
+      for (int i = 0; i < log2n; ++i) y = mul2(y, y);
+    }
+    return y;
+  }
+}
+
 // Which slots a query sees. Query token t of T new ones stands at slot
 // last = len - T + t and sees slots s <= last with s > last - window or
 // s < first (window 0: no window).
