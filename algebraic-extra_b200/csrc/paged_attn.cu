@@ -11,9 +11,12 @@
 // overflows (algebraic.py:186-204; the shifted form of kernels/flash.py:240-284).
 // A row that sees no slot, or whose weights are all zero, gives zeros.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "paged_common.cuh"
+#include "sm100.cuh"
+#include "tmap.h"
 #include "vec_io.cuh"
 
 namespace algx {
@@ -198,20 +201,20 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
 
 // ----------------------------------------------------- bfloat16, matrix units
 // Decoding reads every key and value once and does little with it, so this
-// kernel is built around the loads: keys and values go from memory straight into
-// the registers of the matrix instructions, without shared memory.
+// kernel is built around the loads. Every warp works for itself: one lane asks
+// TMA for groups of 16 slots (2 KB of keys, 2 KB of values, contiguous in a
+// page) into the warp's ring, kStages - 1 groups ahead, and the warp takes them
+// from there in the registers of the matrix instructions. The boxes are swizzled
+// by 128 bytes, so reading eight rows at once meets no bank twice.
 //
-// A warp takes groups of 16 slots. For the scores the keys are the 16-row operand
-// (S^T = K Q^T, up to 8 query rows the other one), and the order of the 64
-// products is free, so each lane loads 16 contiguous bytes of a key where the
-// instruction would have it hold pairs 16 bytes apart: the queries are loaded in
-// the same order. For O^T = V^T P^T the values are the 16-row operand; a lane
-// loads eight contiguous elements of four slots and interleaves pairs of slots
-// with byte permutes, which only renames the output's rows. The scores come out
-// as (slot, row) and go in as (row, slot), one 8 x 8 transposition in registers.
-// mma.sync rather than tcgen05: at 8 to 32 rows the matrix work is a few percent
-// of either unit's rate, and tcgen05 would put keys, values and weights through
-// shared memory and the scores through TMEM.
+// Scores: the keys are the 16-row operand, up to 8 query rows the other one
+// (S^T = K Q^T). Output: O^T = V^T P^T, the values transposed on the way from
+// shared memory. The scores come out as (slot, row) and go in as (row, slot),
+// one 8 x 8 transposition in registers. mma.sync rather than tcgen05: at 8 to 32
+// rows the matrix work is a few percent of either unit's rate, and tcgen05 would
+// put the weights through shared memory and the scores through TMEM and give up
+// the independence of the warps, which hides the latency of one group's chain
+// (products, weights, products) behind those of the others.
 //
 // Weights are relative to a per-row reference that moves only when a weight
 // passes 2^8, so most groups need no reduction over lanes at all. Weights are
@@ -233,47 +236,97 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One group's keys and values in registers: k[0], k[1] the lane's 16-byte chunks
-// t and t + 4 of slot g, k[2], k[3] those of slot g + 8; v[i] chunk g of slots
-// 2t, 2t + 1, 2t + 8, 2t + 9 (g = lane / 4, t = lane % 4).
-struct Group {
-  uint4 k[4], v[4];
-  int base;  // first slot
-  int live;  // slots below it exist (0 when the page does not)
-};
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void load_matrices_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
 
+constexpr int kGroupBytes = 2 * 16 * kD * 2;  // keys and values of 16 slots
+__host__ __device__ constexpr int mma_ctas(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
+__host__ __device__ constexpr int mma_stages(int nt) { return nt == 1 ? 3 : nt == 2 ? 4 : 6; }
+__host__ __device__ constexpr int mma_smem(int nt) {
+  return 1024 + kWarps * mma_stages(nt) * (kGroupBytes + (int)sizeof(uint64_t));
+}
 constexpr float kMove = 256.f;  // a weight above it moves the row's reference
 
 template <int KIND, int LOG2N, int NT, bool ONE>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
-    paged_attn_mma_kernel(const PagedAttnArgs a, const PagedView pv) {
+__global__ void __launch_bounds__(kThreads, mma_ctas(NT))
+    paged_attn_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                          const PagedAttnArgs a, const PagedView pv) {
   using T = __nv_bfloat16;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
   // row (only the first column counts), of its two slots.
-  constexpr int NP = ONE ? 1 : 2;
-  __shared__ float s_o[NT * 8 * kWarps * kD];
-  __shared__ float2 s_ml[NT * 8 * kWarps];
+  constexpr int NP = ONE ? 1 : 2, kStages = mma_stages(NT);
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ int abort_flag;
+  unsigned char* const smem = smem_raw + (1024 - (sm100::smem_u32(smem_raw) & 1023));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  unsigned char* const ring = smem + warp * kStages * kGroupBytes;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kGroupBytes) + warp * kStages;
+  float* const s_o = reinterpret_cast<float*>(smem);  // takes the rings' place once the groups are done
+  float2* const s_ml = reinterpret_cast<float2*>(s_o + NT * 8 * kWarps * kD);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&full[i], 1);
+    sm100::fence_mbar_init();
+  }
+  if (threadIdx.x == 0) abort_flag = 0;
   const Work w(a, pv);
   const Span span(a.sight, w.lo, w.hi);
   const int per = max(kMinGroups, (span.total + a.splits - 1) / a.splits);
   const int g_end = (int)min((int64_t)span.total, (int64_t)(w.split + 1) * per);
   const int32_t* table = pv.table + (int64_t)w.b * pv.max_pages;
 
-  // queries: rows 8 nt + g, chunks t and t + 4
+  // One lane fetches; a page that does not exist is replaced by page 0 and its
+  // slots are masked.
+  auto page_of = [&](int grp) { return grp < g_end ? table[span.slot(grp) >> pv.page_shift] : 0; };
+  uint32_t missing = 0;  // stages whose page does not exist
+  auto issue = [&](int stage, int grp, int pid) {
+    if (grp >= g_end) return;
+    missing &= ~(1u << stage);
+    if ((unsigned)pid >= (unsigned)pv.num_pages) {
+      missing |= 1u << stage;
+      if (lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
+      pid = 0;
+    }
+    if (lane != 0) return;
+    const int row = (int)(paged_row(pv, pid, w.h, span.slot(grp)) / kD);
+    sm100::mbar_expect_tx(&full[stage], kGroupBytes);
+    sm100::tma_load_2d(ring + stage * kGroupBytes, &k_map, &full[stage], 0, row);
+    sm100::tma_load_2d(ring + stage * kGroupBytes + kGroupBytes / 2, &v_map, &full[stage], 0, row);
+  };
+  int grp = (int)min((int64_t)g_end, (int64_t)w.split * per + warp);
+  int ahead = page_of(grp);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    const int pid = ahead;
+    ahead = page_of(grp + (i + 1) * kWarps);
+    issue(i, grp + i * kWarps, pid);
+  }
+
+  // queries: row 8 nt + g, elements 16 s + 2 t and 16 s + 8 + 2 t of every step
   uint32_t q[NT][8];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g;
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (r < w.nr) {
-      const T* row = static_cast<const T*>(a.q) + w.q_row(a, pv, w.r0 + r) * kD;
-      x = *reinterpret_cast<const uint4*>(row + t * 8);
-      y = *reinterpret_cast<const uint4*>(row + 32 + t * 8);
-    }
-    q[nt][0] = x.x; q[nt][1] = x.y; q[nt][2] = x.z; q[nt][3] = x.w;
-    q[nt][4] = y.x; q[nt][5] = y.y; q[nt][6] = y.z; q[nt][7] = y.w;
+    const uint32_t* row = reinterpret_cast<const uint32_t*>(
+        static_cast<const T*>(a.q) + w.q_row(a, pv, w.r0 + min(r, w.nr - 1)) * kD) + t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[nt][i] = r < w.nr ? row[i * 4] : 0u;
   }
+  // what this lane points ldmatrix at: keys by (row, chunk), values by (chunk, row)
+  const uint32_t ring_at = sm100::smem_u32(ring);
+  const int r8 = lane & 7, mi = lane >> 3;
+  const uint32_t k_at = ring_at + (r8 + (mi & 1) * 8) * 128 + (((mi >> 1) ^ r8) << 4);
+  const uint32_t v_at = ring_at + kGroupBytes / 2 + (r8 + (mi >> 1) * 8) * 128 + (((mi & 1) ^ r8) << 4);
   // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
   float m[NT][2], o[NT][4][4];
   float2 turn[NT], l[NT];
@@ -288,35 +341,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
   }
 
-  const int64_t kv_lane = g * kD + t * 8, v_lane = 2 * t * kD + g * 8;
-  auto page_of = [&](int grp) { return grp < g_end ? table[span.slot(grp) >> pv.page_shift] : -1; };
-  auto load = [&](Group& x, int grp, int pid) {
-    x.base = span.slot(grp);
-    const bool known = (unsigned)pid < (unsigned)pv.num_pages;
-    x.live = known ? w.len : 0;
-    const int64_t at = paged_row(pv, known ? pid : 0, w.h, x.base);
-    const T* k = static_cast<const T*>(a.k) + at + kv_lane;
-    const T* v = static_cast<const T*>(a.v) + at + v_lane;
-    if (x.base + 16 <= x.live) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x.k[i] = ld_stream(k + (i >> 1) * 8 * kD + (i & 1) * 32);
-        x.v[i] = ld_stream(v + ((i & 1) + (i >> 1) * 8) * kD);
-      }
-      return;
-    }
-    if (!known && lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int sk = g + (i >> 1) * 8, sv = 2 * t + (i & 1) + (i >> 1) * 8;
-      x.k[i] = x.base + sk < x.live ? ld_stream(k + (i >> 1) * 8 * kD + (i & 1) * 32) : make_uint4(0, 0, 0, 0);
-      x.v[i] = x.base + sv < x.live ? ld_stream(v + ((i & 1) + (i >> 1) * 8) * kD) : make_uint4(0, 0, 0, 0);
-    }
-  };
   auto last_of = [&](int r) { return w.len - a.T + (w.r0 + r) / a.G; };
-  // O^T += V^T P^T for the weights p (two packed pairs a tile); with `only`, for
-  // the rows of the token whose last visible slot it is.
-  auto add_values = [&](const uint4 (&v)[4], const uint32_t (&p)[NT][2], auto one_token, int only) {
+  // O^T += V^T P^T for the weights p (two packed pairs a tile) and the group's
+  // values. keep(i): bits of the values of slots 2 t, 2 t + 1 (i = 0) or 2 t + 8,
+  // 2 t + 9 that exist. With one_token, only for the rows whose last visible slot
+  // is `only`.
+  auto add_values = [&](int stage, const uint32_t (&p)[NT][2], auto masked, uint32_t keep0, uint32_t keep1,
+                        auto one_token, int only) {
     uint32_t b[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -325,20 +356,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t v0 = reinterpret_cast<const uint32_t*>(&v[0])[j], v1 = reinterpret_cast<const uint32_t*>(&v[1])[j];
-      const uint32_t v2 = reinterpret_cast<const uint32_t*>(&v[2])[j], v3 = reinterpret_cast<const uint32_t*>(&v[3])[j];
-      const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
-      const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+      uint32_t v[4];
+      load_matrices_trans(v, (v_at + stage * kGroupBytes) ^ (j << 5));
+      if constexpr (decltype(masked)::value) {
+        v[0] &= keep0; v[1] &= keep0; v[2] &= keep1; v[3] &= keep1;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if constexpr (decltype(one_token)::value) {
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16816(sum, a0, a1, a2, a3, b[nt][0], b[nt][1]);
+          mma_16816(sum, v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (last_of(nt * 8 + 2 * t + (i & 1)) == only) o[nt][j][i] += sum[i];
         } else {
-          mma_16816(o[nt][j], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+          mma_16816(o[nt][j], v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
         }
       }
     }
@@ -347,30 +379,32 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
   auto pair = [&](const float (&s)[4], int i) { return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]); };
   auto turns = [&](int nt) { return ONE ? make_float2(turn[nt].x, turn[nt].x) : turn[nt]; };
 
-  auto compute = [&](const Group& x) {
-    float s[NT][4];
+  auto compute = [&](int stage, int base, int live) {
+    float s[NT][4], s2[NT][4];  // two chains of products, for shorter ones
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float s2[4];  // a second chain of products, for a shorter one
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = s2[i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const uint32_t* lo = reinterpret_cast<const uint32_t*>(&x.k[step >> 1]) + (step & 1) * 2;
-        const uint32_t* hi = reinterpret_cast<const uint32_t*>(&x.k[2 + (step >> 1)]) + (step & 1) * 2;
-        mma_16816(step & 1 ? s2 : s[nt], lo[0], hi[0], lo[1], hi[1], q[nt][2 * step], q[nt][2 * step + 1]);
-      }
+    for (int step = 0; step < 4; ++step) {
+      uint32_t k[4];
+      load_matrices(k, (k_at + stage * kGroupBytes) ^ (step << 5));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[i]) * a.scale;
+      for (int nt = 0; nt < NT; ++nt)
+        mma_16816(step & 1 ? s2[nt] : s[nt], k[0], k[1], k[2], k[3], q[nt][2 * step], q[nt][2 * step + 1]);
     }
-    const bool whole = x.base + 16 <= x.live && a.sight.sees_group(x.base, w.lo, w.hi);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * a.scale;
+    const bool whole = base + 16 <= live && a.sight.sees_group(base, w.lo, w.hi);
     if (!whole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int slot = x.base + g + (i >> 1) * 8;
-          if (slot >= x.live || !a.sight.sees(slot, last_of(nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
+          const int slot = base + g + (i >> 1) * 8;
+          if (slot >= live || !a.sight.sees(slot, last_of(nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
         }
     }
     if (a.xs != nullptr) {
@@ -378,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = nt * 8 + 2 * t + (i & 1), slot = x.base + g + (i >> 1) * 8;
+          const int r = nt * 8 + 2 * t + (i & 1), slot = base + g + (i >> 1) * 8;
           if (r < w.nr) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + slot] = s[nt][i];
         }
     }
@@ -425,50 +459,53 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       pk[nt][0] = ONE ? pack_pair(p[nt][0].x, 0.f) : pack_pair(p[nt][0].x, p[nt][0].y);
       pk[nt][1] = ONE ? pack_pair(p[nt][0].y, 0.f) : pack_pair(p[nt][NP - 1].x, p[nt][NP - 1].y);
     }
-    if (!whole && w.lo != w.hi) {
-      // Rows of different tokens see different slots of this group. A weight of
-      // zero does not hide an infinity or NaN in a value, so such a group is
-      // added token by token, the values the token does not see set to zero.
-      bool odd = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t* v = reinterpret_cast<const uint32_t*>(&x.v[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          odd = odd || (v[j] & 0x7f80u) == 0x7f80u || (v[j] & 0x7f800000u) == 0x7f800000u;
-      }
-      if (__any_sync(0xffffffffu, odd)) {
-        for (int last = w.lo; last <= w.hi; ++last) {
-          uint4 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = a.sight.sees(x.base + 2 * t + (i & 1) + (i >> 1) * 8, last) ? x.v[i] : make_uint4(0, 0, 0, 0);
-          add_values(v, pk, std::true_type{}, last);
-        }
-        return;
-      }
+    if (whole) {
+      add_values(stage, pk, std::false_type{}, 0u, 0u, std::false_type{}, 0);
+      return;
     }
-    add_values(x.v, pk, std::false_type{}, 0);
+    // Slots beyond the sequence hold anything: a weight of zero does not hide an
+    // infinity or NaN in a value, so their values are cleared. Where the rows of
+    // different tokens see different slots, the group is added token by token.
+    auto keep = [&](int i, int last) {
+      const int slot = base + 2 * t + i * 8;
+      return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
+             (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
+    };
+    if (w.lo == w.hi) {
+      add_values(stage, pk, std::true_type{}, keep(0, w.hi), keep(1, w.hi), std::false_type{}, 0);
+    } else {
+      for (int last = w.lo; last <= w.hi; ++last)
+        add_values(stage, pk, std::true_type{}, keep(0, last), keep(1, last), std::true_type{}, last);
+    }
   };
 
-  // Two groups in registers, the next one's loads issued before the current one
-  // is worked on, page numbers one group further ahead.
-  int grp = (int)min((int64_t)g_end, (int64_t)w.split * per + warp);
-  Group x, y;
-  int pid = page_of(grp), next = page_of(grp + kWarps);
-  if (grp < g_end) load(x, grp, pid);
+  // Page numbers are read one group further ahead than the copies that need them.
+  volatile int* const abort_v = &abort_flag;
+  uint32_t parity = 0;
+  int stage = 0, in = kStages - 1;
+  bool ok = true;
+  __syncthreads();
   while (grp < g_end) {
-    pid = page_of(grp + 2 * kWarps);
-    if (grp + kWarps < g_end) load(y, grp + kWarps, next);
-    compute(x);
+    __syncwarp();  // every lane has taken the group whose place this copy gets
+    issue(in, grp + (kStages - 1) * kWarps, ahead);
+    ahead = page_of(grp + kStages * kWarps);
+    ok = sm100::mbar_wait_warp(&full[stage], parity, abort_v, a.err);
+    if (!ok) break;
+    compute(stage, span.slot(grp), missing >> stage & 1 ? 0 : w.len);
     grp += kWarps;
-    if (grp >= g_end) break;
-    next = page_of(grp + 2 * kWarps);
-    if (grp + kWarps < g_end) load(x, grp + kWarps, pid);
-    compute(y);
-    grp += kWarps;
+    in = stage;
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  if (!ok) {  // a copy did not arrive in time: let those on their way land, within limits, before the CTA ends
+    volatile int quiet = 0;
+    for (int i = 0; i < kStages && grp + i * kWarps < g_end; ++i)
+      sm100::mbar_wait(&full[(stage + i) % kStages], parity ^ (stage + i >= kStages), &quiet, nullptr);
   }
   pdl_trigger();
+  __syncthreads();  // the rings are free
 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -481,8 +518,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2)
       if (g == 0) s_ml[r * kWarps + warp] = make_float2(m[nt][c], sum);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float* at = s_o + (r * kWarps + warp) * kD + 8 * g + 2 * j;
-        *reinterpret_cast<float2*>(at) = make_float2(o[nt][j][c], o[nt][j][c + 2]);
+        s_o[(r * kWarps + warp) * kD + 16 * j + g] = o[nt][j][c];
+        s_o[(r * kWarps + warp) * kD + 16 * j + 8 + g] = o[nt][j][c + 2];
       }
     }
   }
@@ -618,28 +655,51 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, int64_t
   return p;
 }
 
+template <int KIND, int LOG2N, int NT, bool ONE>
+int mma_launch(const PagedAttnArgs& a, const PagedView& pv, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
+               cudaStream_t st) {
+  auto* kern = paged_attn_mma_kernel<KIND, LOG2N, NT, ONE>;
+  static std::atomic<uint64_t> ready{0};  // one bit per device: its shared memory limit is raised
+  int dev = 0;
+  ALGX_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    ALGX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, mma_smem(NT)));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  kern<<<grid, kThreads, mma_smem(NT), st>>>(k, v, a, pv);
+  return ALGX_OK;
+}
+
 template <int KIND, int LOG2N>
-auto mma_kernel(const Plan& p) -> void (*)(PagedAttnArgs, PagedView) {
-  return p.rows == 1         ? paged_attn_mma_kernel<KIND, LOG2N, 1, true>
-         : p.tile_rows == 8  ? paged_attn_mma_kernel<KIND, LOG2N, 1, false>
-         : p.tile_rows == 16 ? paged_attn_mma_kernel<KIND, LOG2N, 2, false>
-         : p.tile_rows == 24 ? paged_attn_mma_kernel<KIND, LOG2N, 3, false>
-                             : paged_attn_mma_kernel<KIND, LOG2N, 4, false>;
+int mma_launch_rows(const PagedAttnArgs& a, const PagedView& pv, unsigned grid, cudaStream_t st) {
+  const int64_t rows = ((int64_t)pv.num_pages * pv.heads) << pv.page_shift;
+  ALGX_REQUIRE(rows <= INT32_MAX, "paged cache too large");
+  CUtensorMap k, v;
+  if (int e = make_tmap_2d(&k, a.k, ALGX_BF16, kD, (uint64_t)rows, kD * 2, kD, 16, true)) return e;
+  if (int e = make_tmap_2d(&v, a.v, ALGX_BF16, kD, (uint64_t)rows, kD * 2, kD, 16, true)) return e;
+  return a.rows == 1         ? mma_launch<KIND, LOG2N, 1, true>(a, pv, k, v, grid, st)
+         : a.tile_rows == 8  ? mma_launch<KIND, LOG2N, 1, false>(a, pv, k, v, grid, st)
+         : a.tile_rows == 16 ? mma_launch<KIND, LOG2N, 2, false>(a, pv, k, v, grid, st)
+         : a.tile_rows == 24 ? mma_launch<KIND, LOG2N, 3, false>(a, pv, k, v, grid, st)
+                             : mma_launch<KIND, LOG2N, 4, false>(a, pv, k, v, grid, st);
 }
 
 template <typename T, int KIND>
 int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int64_t B, cudaStream_t st) {
   const int64_t grid = B * pv.heads * p.splits * p.tiles;
   ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
-  void (*kern)(PagedAttnArgs, PagedView);
-  if constexpr (sizeof(T) == 2)
-    kern = KIND == kAsinh && a.log2n == 4 ? mma_kernel<KIND, 4>(p) : mma_kernel<KIND, 0>(p);
-  else
-    kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
-           : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>
-           : p.tile_rows == 4 ? paged_attn_kernel<T, KIND, 4>
-                              : paged_attn_kernel<T, KIND, 8>;
-  kern<<<(unsigned)grid, kThreads, 0, st>>>(a, pv);
+  if constexpr (sizeof(T) == 2) {
+    const int e = KIND == kAsinh && a.log2n == 4 ? mma_launch_rows<KIND, 4>(a, pv, (unsigned)grid, st)
+                                                 : mma_launch_rows<KIND, 0>(a, pv, (unsigned)grid, st);
+    if (e) return e;
+  } else {
+    auto* kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
+                 : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>
+                 : p.tile_rows == 4 ? paged_attn_kernel<T, KIND, 4>
+                                    : paged_attn_kernel<T, KIND, 8>;
+    kern<<<(unsigned)grid, kThreads, 0, st>>>(a, pv);
+  }
   ALGX_LAUNCHED("paged_attn_kernel");
   if (a.direct) return ALGX_OK;
   const int64_t blocks = a.rows + (a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0);
