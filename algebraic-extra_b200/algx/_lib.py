@@ -117,7 +117,7 @@ SIGNATURES = {
     "algx_aluglu_fwd": ([_P, _P, _I64, _I64, _F, _P], ctypes.c_int),
     "algx_aluglu_bwd": ([_P, _P, _P, _I64, _I64, _F, _P], ctypes.c_int),
     "algx_cache_append": ([_P] * 5 + [_I64] + [_P] * 8 + [_I64] * 8 + [_I32, _F, _P], ctypes.c_int),
-    "algx_paged_attn_workspace_size": ([_I64] * 8 + [_I32] * 2, _SZ),
+    "algx_paged_attn_workspace_size": ([_I64] * 6 + [_I32] * 2, _SZ),
     "algx_paged_attn": ([ctypes.POINTER(PagedConfig)] + [_P] * 9 + [_I64] * 8 + [_I32, _P, _SZ, _P], ctypes.c_int),
     "algx_cache_evict_workspace_size": ([_I64] * 3, _SZ),
     "algx_cache_evict": ([_P] * 6 + [_I64] * 3 + [_P] * 4 + [_I64] * 6 + [_I32, _P, _SZ, _P], ctypes.c_int),

@@ -194,7 +194,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
     lib = L.lib()
     o = torch.empty_like(q)
     code = L.dtype_code(q.dtype)
-    nbytes = lib.algx_paged_attn_workspace_size(B, T, Hq, Hkv, size, maxp, cfg.window, first, scores is not None, code)
+    nbytes = lib.algx_paged_attn_workspace_size(B, T, Hq, Hkv, size, maxp, scores is not None, code)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
     L.check(lib.algx_paged_attn(
         cfg, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.ptr(sink),

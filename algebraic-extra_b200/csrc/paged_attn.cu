@@ -25,188 +25,280 @@ namespace {
 constexpr int kD = 64;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMinGroups = 8;  // groups of 16 slots a split takes at least
+constexpr int kSms = 148;
+constexpr int kMinShare = 4;  // groups of 16 slots a warp takes at least
 
 struct PagedAttnArgs {
   const void *q, *k, *v;
   const float *sink, *scores;
   float* scores_out;
   void* o;
-  float2* part_ml;  // (B, Hkv, rows, splits): reference score, sum of weights
-  float* part_o;    // (B, Hkv, rows, splits, 64)
+  float2* part_ml;  // (warps + items, tile_rows): reference score, sum of weights
+  float* part_o;    // (warps + items, tile_rows, 64)
   float* xs;        // (B, Hkv, rows, S) scores, when weights are accumulated
   int* err;
   int64_t slots;    // S: slots of one sequence's table
-  int T, G, rows, tile_rows, tiles, splits, log2n;
-  bool direct;      // one split and no scores: outputs are written without a join
+  int B, T, G, rows, tile_rows, tiles, warps, log2n;
   float scale, inv_unit;
   Sight sight;
 };
 
-// Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
-__device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// ------------------------------------------------------------- division of work
+// An item is one tile of up to tile_rows rows of one kv head of one sequence; its
+// work is the groups of 16 slots that its rows look at. All items' groups stand in
+// one line, (sequence, head, tile, group), which is cut into equal shares, one a
+// warp, whatever the sequences' lengths: a share can end one item and begin the
+// next ones. Every warp writes one partial result for every item it touches, at
+// index warp + item, which is different for every pair that occurs because along
+// the line either the warp or the item moves on.
 
-// What one CTA works on.
-struct Work {
-  int b, h, split, r0, nr, len, lo, hi;
-  __device__ __forceinline__ Work(const PagedAttnArgs& a, const PagedView& pv) {
-    unsigned idx = blockIdx.x;
-    const unsigned tile = idx % (unsigned)a.tiles;
-    idx /= (unsigned)a.tiles;
-    split = (int)(idx % (unsigned)a.splits);
-    idx /= (unsigned)a.splits;
-    b = (int)(idx / (unsigned)pv.heads);
-    h = (int)(idx - (unsigned)b * (unsigned)pv.heads);
-    len = paged_len(pv, b, a.err);
-    r0 = (int)tile * a.tile_rows;
+// Rows of an item, and the span of slots they look at.
+struct Rows {
+  int r0, nr, lo, hi;
+  __device__ __forceinline__ Rows(const PagedAttnArgs& a, int len, int tile) {
+    r0 = tile * a.tile_rows;
     nr = min(a.tile_rows, a.rows - r0);
     lo = len - a.T + r0 / a.G;
     hi = len - a.T + (r0 + nr - 1) / a.G;
   }
-  __device__ __forceinline__ int64_t kv(const PagedView& pv) const { return (int64_t)b * pv.heads + h; }
-  // Element offset / 64 of a row of q or o.
-  __device__ __forceinline__ int64_t q_row(const PagedAttnArgs& a, const PagedView& pv, int row) const {
-    const int t = row / a.G;
-    return (((int64_t)b * a.T + t) * pv.heads + h) * a.G + (row - t * a.G);
+};
+__device__ __forceinline__ Span item_span(const PagedAttnArgs& a, int len, int tile) {
+  const Rows r(a, len, tile);
+  return Span(a.sight, r.lo, r.hi);
+}
+// Groups of one kv head of a sequence: all tiles', or those before `tiles`.
+__device__ __forceinline__ int64_t head_groups(const PagedAttnArgs& a, int len, int tiles) {
+  int64_t n = 0;
+  for (int i = 0; i < tiles; ++i) n += item_span(a, len, i).total;
+  return n;
+}
+
+// Groups before sequence `upto` and in all, by the whole block.
+struct Line {
+  int64_t before, total, share;
+};
+__device__ __forceinline__ int64_t warp_sum64(int64_t x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+__device__ __forceinline__ int64_t share_of(const PagedAttnArgs& a, int64_t total) {
+  const int64_t even = (total + a.warps - 1) / a.warps;
+  return even < kMinShare ? kMinShare : even;
+}
+__device__ __forceinline__ Line line_before(const PagedAttnArgs& a, const PagedView& pv, int upto) {
+  __shared__ int64_t s_sum[2][kWarps];
+  int64_t before = 0, total = 0;
+  for (int b = threadIdx.x; b < a.B; b += kThreads) {
+    const int64_t n = head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
+    total += n;
+    if (b < upto) before += n;
+  }
+  before = warp_sum64(before);
+  total = warp_sum64(total);
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[0][threadIdx.x >> 5] = before;
+    s_sum[1][threadIdx.x >> 5] = total;
+  }
+  __syncthreads();
+  Line l = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    l.before += s_sum[0][i];
+    l.total += s_sum[1][i];
+  }
+  l.share = share_of(a, l.total);
+  return l;
+}
+
+// A place on the line.
+struct Cursor {
+  int b, h, tile, item, grp, len;
+  Span span;
+
+  // The `at`-th group, for a warp; `excl` (kThreads) holds the groups before each
+  // thread's run of `run` sequences.
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, const int64_t* excl, int run,
+                                    int64_t at) : span(a.sight, -1, -1) {
+    int lo = 0;
+    for (int step = kThreads / 2; step > 0; step >>= 1)
+      if (excl[lo + step] <= at) lo += step;
+    b = lo * run;
+    at -= excl[lo];
+    int64_t per;
+    for (;;) {
+      len = paged_len(pv, b, a.err);
+      per = head_groups(a, len, a.tiles);
+      if (at < per * pv.heads) break;
+      at -= per * pv.heads;
+      ++b;
+    }
+    h = (int)(at / per);
+    at -= h * per;
+    tile = 0;
+    for (;;) {
+      span = item_span(a, len, tile);
+      if (at < span.total) break;
+      at -= span.total;
+      ++tile;
+    }
+    grp = (int)at;
+    item = (b * pv.heads + h) * a.tiles + tile;
+  }
+  // On to the next group, if there is one.
+  __device__ __forceinline__ void next(const PagedAttnArgs& a, const PagedView& pv) {
+    if (++grp < span.total) return;
+    grp = 0;
+    do {
+      ++item;
+      if (++tile == a.tiles) {
+        tile = 0;
+        if (++h == pv.heads) {
+          h = 0;
+          if (++b == a.B) return;
+          len = paged_len(pv, b, a.err);
+        }
+      }
+      span = item_span(a, len, tile);
+    } while (span.total == 0);
   }
 };
 
-__device__ __forceinline__ float sink_score(const PagedAttnArgs& a, int h, int row) {
-  return a.sink ? a.sink[h * a.G + row % a.G] * a.inv_unit : kNegInf;
-}
-
-// Joins the CTA's PARTS partial results of each row: into the workspace, or, when
-// no other split has a share, into the output.
-template <typename T, int KIND, int PARTS>
-__device__ __forceinline__ void merge_parts(const PagedAttnArgs& a, const PagedView& pv, const Work& w,
-                                            const float* s_o, const float2* s_ml) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  for (int i = threadIdx.x; i < w.nr * kD; i += kThreads) {
-    const int r = i / kD, d = i % kD;
-    const float sink = a.direct ? sink_score(a, w.h, w.r0 + r) : kNegInf;
-    float M = sink;
-    for (int p = 0; p < PARTS; ++p) M = fmaxf(M, s_ml[r * PARTS + p].x);
-    const float t = weight_turn<KIND, EXACT>(M);
-    float L = sink == kNegInf ? 0.f : weight_of<KIND, EXACT>(sink, t, a.log2n), O = 0.f;
-    for (int p = 0; p < PARTS; ++p) {
-      const float2 ml = s_ml[r * PARTS + p];
-      if (ml.x == kNegInf && ml.y == 0.f) continue;
-      const float f = weight_of<KIND, EXACT>(ml.x, t, a.log2n);
-      L = fmaf(ml.y, f, L);
-      O = fmaf(s_o[(r * PARTS + p) * kD + d], f, O);
-    }
-    if (a.direct) {
-      static_cast<T*>(a.o)[w.q_row(a, pv, w.r0 + r) * kD + d] = from_f32<T>(O * row_scale(L));
-    } else {
-      const int64_t at = (w.kv(pv) * a.rows + w.r0 + r) * a.splits + w.split;
-      if (d == 0) a.part_ml[at] = make_float2(M, L);
-      a.part_o[at * kD + d] = O;
-    }
+// What a warp needs to know of the item it works on.
+struct Item {
+  int b, h, len, r0, nr, lo, hi;
+  __device__ __forceinline__ Item(const PagedAttnArgs& a, const PagedView& pv, int item) {
+    const int tile = item % a.tiles, bh = item / a.tiles;
+    b = bh / pv.heads;
+    h = bh - b * pv.heads;
+    len = paged_len(pv, b, a.err);
+    const Rows r(a, len, tile);
+    r0 = r.r0; nr = r.nr; lo = r.lo; hi = r.hi;
   }
-}
+  // Row of q or o (in units of 64 elements), and of xs (in units of S).
+  __device__ __forceinline__ int64_t q_row(const PagedAttnArgs& a, const PagedView& pv, int r) const {
+    const int t = (r0 + r) / a.G;
+    return (((int64_t)b * a.T + t) * pv.heads + h) * a.G + (r0 + r - t * a.G);
+  }
+  __device__ __forceinline__ float* x_row(const PagedAttnArgs& a, const PagedView& pv, int r) const {
+    return a.xs + (((int64_t)b * pv.heads + h) * a.rows + r0 + r) * a.slots;
+  }
+  __device__ __forceinline__ int last_of(const PagedAttnArgs& a, int r) const { return len - a.T + (r0 + r) / a.G; }
+};
 
-// ------------------------------------------------------- any I/O type, FMA units
-// One CTA per (split, row tile, kv head, sequence); a warp takes every fourth
-// group of the split. A row of 64 elements lies across TPR lanes, so a warp
-// reads 32 / TPR slots at once, and each such lane group keeps its own running
-// reference, sum and output, merged over the CTA at the end.
-template <typename T, int KIND, int R>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArgs a, const PagedView pv) {
-  using V = Vec<T>;
-  constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int kParts = kWarps * V::RPW;
-  __shared__ float s_o[R][kParts][kD];
-  __shared__ float2 s_ml[R][kParts];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % V::TPR, rl = lane / V::TPR;
-  const Work w(a, pv);
-  const Span span(a.sight, w.lo, w.hi);
-  const int per = max(kMinGroups, (span.total + a.splits - 1) / a.splits);
-  const int g_end = (int)min((int64_t)span.total, (int64_t)(w.split + 1) * per);
+// Weights are relative to a per-row reference that moves only when a weight
+// passes 2^8, so most groups need no reduction over lanes at all.
+constexpr float kMove = 256.f;
 
-  float q[R][V::N];
+// ------------------------------------------------------- float32, FMA units
+// A row of 64 elements lies across 16 lanes, two slots a step. The 8 partial
+// products of a lane are summed over the 16 lanes by exchanging halves (8
+// shuffles for 16 slots), which leaves every slot's score in a pair of lanes, so
+// each weight is evaluated once, and handed back by one shuffle a step.
+template <int KIND_, int R>
+struct FmaEngine {
+  using T = float;
+  static constexpr int kStages = 2, kCtas = 3, kRowBytes = kD * 4;
+  static constexpr bool kSwizzle = false;
+  float4 q[R], acc[R];
+  float m[R], turn[R], l[R];
   int last[R];
+
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedView& pv, const Item& w) {
+    const int sub = threadIdx.x & 15;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = min(w.r0 + r, a.rows - 1);
-    last[r] = r < w.nr ? w.len - a.T + row / a.G : -1;
-    unpack<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.q_row(a, pv, row) * kD + sub * V::N), q[r]);
-  }
-  float m[R], turn[R], l[R], acc[R][V::N];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = kNegInf;
-    turn[r] = weight_turn<KIND, EXACT>(kNegInf);
-    l[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < V::N; ++i) acc[r][i] = 0.f;
-  }
-  for (int64_t g = (int64_t)w.split * per + warp; g < g_end; g += kWarps) {
-    const int base = span.slot((int)g);
-    const int pid = pv.table[(int64_t)w.b * pv.max_pages + (base >> pv.page_shift)];
-    if (pid < 0 || pid >= pv.num_pages) {
-      if (lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
-      if (a.xs != nullptr && lane < 16)
-        for (int r = 0; r < w.nr; ++r) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + base + lane] = kNegInf;
-      continue;
+    for (int r = 0; r < R; ++r) {
+      const float* row = static_cast<const float*>(a.q) + w.q_row(a, pv, min(r, w.nr - 1)) * kD;
+      q[r] = reinterpret_cast<const float4*>(row)[sub];
+      acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      m[r] = kNegInf;
+      turn[r] = weight_turn<KIND_, true>(kNegInf);
+      l[r] = 0.f;
+      last[r] = r < w.nr ? w.last_of(a, r) : -1;
     }
-    const int64_t at = paged_row(pv, pid, w.h, base) + sub * V::N;
-#pragma unroll 2
-    for (int j = 0; j < 16; j += V::RPW) {
-      const int s = base + j + rl;
-      float kf[V::N], vf[V::N];
-      const bool live = s < w.len;
-      unpack<T>(live ? ld_stream(static_cast<const T*>(a.k) + at + (j + rl) * kD) : make_uint4(0, 0, 0, 0), kf);
-      unpack<T>(live ? ld_stream(static_cast<const T*>(a.v) + at + (j + rl) * kD) : make_uint4(0, 0, 0, 0), vf);
-      float xr[R];
+  }
+  __device__ __forceinline__ void compute(const PagedAttnArgs& a, const PagedView& pv, const Item& w,
+                                          const unsigned char* group, int base, int live) {
+    const int lane = threadIdx.x & 31, sub = lane & 15, rl = lane >> 4;
+    const float4* k = reinterpret_cast<const float4*>(group) + lane;
+    const float4* v = k + 16 * kRowBytes / 16;
+    const int slot = base + (sub & ~1) + rl;  // whose score this lane ends up with
+    float p[R];
+    float high = 0.f;
+    float x[R][8];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float x = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const float4 kv = k[i * 32];
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) x = fmaf(q[r][i], kf[i], x);
-        xr[r] = row_sum<V::TPR>(x) * a.scale;
-      }
+      for (int r = 0; r < R; ++r) x[r][i] = fmaf(q[r].w, kv.w, fmaf(q[r].z, kv.z, fmaf(q[r].y, kv.y, q[r].x * kv.x)));
+    }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float x = xr[r];
-        if (!a.sight.sees(s, last[r])) continue;
-        if (a.xs != nullptr && sub == 0)
-          a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + s] = x;
-        if (x == kNegInf) continue;  // weight 0
-        if (x > m[r]) {
-          const float nt = weight_turn<KIND, EXACT>(x);
-          const float f = m[r] == kNegInf ? 0.f : weight_of<KIND, EXACT>(m[r], nt, a.log2n);
-          m[r] = x;
-          turn[r] = nt;
-          l[r] *= f;
+    for (int r = 0; r < R; ++r) {
 #pragma unroll
-          for (int i = 0; i < V::N; ++i) acc[r][i] *= f;
+      for (int half = 4; half > 0; half >>= 1) {
+        const bool upper = sub & (2 * half);
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+          const float give = upper ? x[r][i] : x[r][i + half], hold = upper ? x[r][i + half] : x[r][i];
+          x[r][i] = hold + __shfl_xor_sync(0xffffffffu, give, 2 * half);
         }
-        const float p = weight_of<KIND, EXACT>(x, turn[r], a.log2n);
-        l[r] += p;
+      }
+      float s = (x[r][0] + __shfl_xor_sync(0xffffffffu, x[r][0], 1)) * a.scale;
+      if (slot >= live || !a.sight.sees(slot, last[r])) s = kNegInf;
+      if (a.xs != nullptr && r < w.nr && !(sub & 1)) w.x_row(a, pv, r)[slot] = s;
+      x[r][0] = s;
+      p[r] = weight_of<KIND_, true>(s, turn[r], a.log2n);
+      high = fmaxf(high, p[r]);
+    }
+    if (__any_sync(0xffffffffu, high > kMove)) {
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) acc[r][i] = fmaf(p, vf[i], acc[r][i]);
+      for (int r = 0; r < R; ++r) {
+        float top = x[r][0];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (top > m[r]) {
+          turn[r] = weight_turn<KIND_, true>(top);
+          const float f = m[r] == kNegInf ? 0.f : weight_of<KIND_, true>(m[r], turn[r], a.log2n);
+          m[r] = top;
+          l[r] *= f;
+          acc[r].x *= f; acc[r].y *= f; acc[r].z *= f; acc[r].w *= f;
+          p[r] = weight_of<KIND_, true>(x[r][0], turn[r], a.log2n);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) l[r] += p[r];
+    const bool whole = base + 16 <= live && a.sight.sees_group(base, w.lo, w.hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 vv = v[i * 32];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float f = __shfl_sync(0xffffffffu, p[r], (lane & 16) + 2 * i);
+        if (whole || f != 0.f) {  // a weight of zero does not hide an infinity or NaN in a value
+          acc[r].x = fmaf(f, vv.x, acc[r].x); acc[r].y = fmaf(f, vv.y, acc[r].y);
+          acc[r].z = fmaf(f, vv.z, acc[r].z); acc[r].w = fmaf(f, vv.w, acc[r].w);
+        }
       }
     }
   }
-  const int part = warp * V::RPW + rl;
+  __device__ __forceinline__ void flush(const Item& w, float2* ml, float* o) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (sub == 0) s_ml[r][part] = make_float2(m[r], l[r]);
-#pragma unroll
-    for (int i = 0; i < V::N; ++i) s_o[r][part][sub * V::N + i] = acc[r][i];
+    for (int r = 0; r < R; ++r) {
+      const float sum = 0.5f * row_sum<32>(l[r]);  // every slot's weight stands in two lanes
+      float4 y = acc[r];
+      y.x += __shfl_xor_sync(0xffffffffu, y.x, 16); y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+      y.z += __shfl_xor_sync(0xffffffffu, y.z, 16); y.w += __shfl_xor_sync(0xffffffffu, y.w, 16);
+      if (r < w.nr) {
+        if (lane == 0) ml[r] = make_float2(m[r], sum);
+        if (lane < 16) reinterpret_cast<float4*>(o + r * kD)[lane] = y;
+      }
+    }
   }
-  __syncthreads();
-  merge_parts<T, KIND, kParts>(a, pv, w, &s_o[0][0][0], &s_ml[0][0]);
-}
+};
 
 // ----------------------------------------------------- bfloat16, matrix units
-// Decoding reads every key and value once and does little with it, so this
-// kernel is built around the loads. Every warp works for itself: one lane asks
-// TMA for groups of 16 slots (2 KB of keys, 2 KB of values, contiguous in a
-// page) into the warp's ring, kStages - 1 groups ahead, and the warp takes them
-// from there in the registers of the matrix instructions. The boxes are swizzled
-// by 128 bytes, so reading eight rows at once meets no bank twice.
-//
 // Scores: the keys are the 16-row operand, up to 8 query rows the other one
 // (S^T = K Q^T). Output: O^T = V^T P^T, the values transposed on the way from
 // shared memory. The scores come out as (slot, row) and go in as (row, slot),
@@ -216,10 +308,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
 // the independence of the warps, which hides the latency of one group's chain
 // (products, weights, products) behind those of the others.
 //
-// Weights are relative to a per-row reference that moves only when a weight
-// passes 2^8, so most groups need no reduction over lanes at all. Weights are
-// rounded to bf16 for the second product, as the forward kernels round them
-// (kernels/flash.py:262), while their sum keeps the unrounded ones.
+// Weights are rounded to bf16 for the second product, as the forward kernels
+// round them (kernels/flash.py:262), while their sum keeps the unrounded ones.
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -249,105 +339,47 @@ __device__ __forceinline__ void load_matrices_trans(uint32_t (&r)[4], uint32_t a
                : "memory");
 }
 
-constexpr int kGroupBytes = 2 * 16 * kD * 2;  // keys and values of 16 slots
-__host__ __device__ constexpr int mma_ctas(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
-__host__ __device__ constexpr int mma_stages(int nt) { return nt == 1 ? 3 : nt == 2 ? 4 : 6; }
-__host__ __device__ constexpr int mma_smem(int nt) {
-  return 1024 + kWarps * mma_stages(nt) * (kGroupBytes + (int)sizeof(uint64_t));
-}
-constexpr float kMove = 256.f;  // a weight above it moves the row's reference
 
-template <int KIND, int LOG2N, int NT, bool ONE>
-__global__ void __launch_bounds__(kThreads, mma_ctas(NT))
-    paged_attn_mma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                          const PagedAttnArgs a, const PagedView pv) {
+template <int KIND_, int LOG2N, int NT, bool ONE>
+struct MmaEngine {
   using T = __nv_bfloat16;
+  static constexpr int kStages = NT == 1 ? 3 : NT == 2 ? 4 : 6, kCtas = NT == 1 ? 4 : NT == 2 ? 3 : 2,
+                       kRowBytes = kD * 2;
+  static constexpr bool kSwizzle = true;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
   // row (only the first column counts), of its two slots.
-  constexpr int NP = ONE ? 1 : 2, kStages = mma_stages(NT);
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ int abort_flag;
-  unsigned char* const smem = smem_raw + (1024 - (sm100::smem_u32(smem_raw) & 1023));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  unsigned char* const ring = smem + warp * kStages * kGroupBytes;
-  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kGroupBytes) + warp * kStages;
-  float* const s_o = reinterpret_cast<float*>(smem);  // takes the rings' place once the groups are done
-  float2* const s_ml = reinterpret_cast<float2*>(s_o + NT * 8 * kWarps * kD);
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&full[i], 1);
-    sm100::fence_mbar_init();
-  }
-  if (threadIdx.x == 0) abort_flag = 0;
-  const Work w(a, pv);
-  const Span span(a.sight, w.lo, w.hi);
-  const int per = max(kMinGroups, (span.total + a.splits - 1) / a.splits);
-  const int g_end = (int)min((int64_t)span.total, (int64_t)(w.split + 1) * per);
-  const int32_t* table = pv.table + (int64_t)w.b * pv.max_pages;
-
-  // One lane fetches; a page that does not exist is replaced by page 0 and its
-  // slots are masked.
-  auto page_of = [&](int grp) { return grp < g_end ? table[span.slot(grp) >> pv.page_shift] : 0; };
-  uint32_t missing = 0;  // stages whose page does not exist
-  auto issue = [&](int stage, int grp, int pid) {
-    if (grp >= g_end) return;
-    missing &= ~(1u << stage);
-    if ((unsigned)pid >= (unsigned)pv.num_pages) {
-      missing |= 1u << stage;
-      if (lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
-      pid = 0;
-    }
-    if (lane != 0) return;
-    const int row = (int)(paged_row(pv, pid, w.h, span.slot(grp)) / kD);
-    sm100::mbar_expect_tx(&full[stage], kGroupBytes);
-    sm100::tma_load_2d(ring + stage * kGroupBytes, &k_map, &full[stage], 0, row);
-    sm100::tma_load_2d(ring + stage * kGroupBytes + kGroupBytes / 2, &v_map, &full[stage], 0, row);
-  };
-  int grp = (int)min((int64_t)g_end, (int64_t)w.split * per + warp);
-  int ahead = page_of(grp);
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    const int pid = ahead;
-    ahead = page_of(grp + (i + 1) * kWarps);
-    issue(i, grp + i * kWarps, pid);
-  }
-
-  // queries: row 8 nt + g, elements 16 s + 2 t and 16 s + 8 + 2 t of every step
+  static constexpr int NP = ONE ? 1 : 2;
   uint32_t q[NT][8];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g;
-    const uint32_t* row = reinterpret_cast<const uint32_t*>(
-        static_cast<const T*>(a.q) + w.q_row(a, pv, w.r0 + min(r, w.nr - 1)) * kD) + t;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[nt][i] = r < w.nr ? row[i * 4] : 0u;
-  }
-  // what this lane points ldmatrix at: keys by (row, chunk), values by (chunk, row)
-  const uint32_t ring_at = sm100::smem_u32(ring);
-  const int r8 = lane & 7, mi = lane >> 3;
-  const uint32_t k_at = ring_at + (r8 + (mi & 1) * 8) * 128 + (((mi >> 1) ^ r8) << 4);
-  const uint32_t v_at = ring_at + kGroupBytes / 2 + (r8 + (mi >> 1) * 8) * 128 + (((mi & 1) ^ r8) << 4);
   // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
   float m[NT][2], o[NT][4][4];
   float2 turn[NT], l[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = kNegInf;
-    turn[nt].x = turn[nt].y = weight_turn<KIND, false>(kNegInf);
-    l[nt] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
-  }
 
-  auto last_of = [&](int r) { return w.len - a.T + (w.r0 + r) / a.G; };
-  // O^T += V^T P^T for the weights p (two packed pairs a tile) and the group's
-  // values. keep(i): bits of the values of slots 2 t, 2 t + 1 (i = 0) or 2 t + 8,
-  // 2 t + 9 that exist. With one_token, only for the rows whose last visible slot
-  // is `only`.
-  auto add_values = [&](int stage, const uint32_t (&p)[NT][2], auto masked, uint32_t keep0, uint32_t keep1,
-                        auto one_token, int only) {
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedView& pv, const Item& w) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // row 8 nt + g, elements 16 s + 2 t and 16 s + 8 + 2 t of every step s
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const uint32_t* row =
+          reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + w.q_row(a, pv, min(r, w.nr - 1)) * kD) + t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[nt][i] = r < w.nr ? row[i * 4] : 0u;
+      m[nt][0] = m[nt][1] = kNegInf;
+      turn[nt].x = turn[nt].y = weight_turn<KIND_, false>(kNegInf);
+      l[nt] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
+    }
+  }
+  // O^T += V^T P^T. PART: values outside keep0, keep1 (bits of slots 2 t, 2 t + 1
+  // and 2 t + 8, 2 t + 9) are taken as zero, and only the rows whose last visible
+  // slot is `only` receive the sum.
+  template <bool PART>
+  __device__ __forceinline__ void add_values(const PagedAttnArgs& a, const Item& w, uint32_t v_at,
+                                             const uint32_t (&p)[NT][2], uint32_t keep0, uint32_t keep1, int only) {
+    const int t = threadIdx.x & 3;
     uint32_t b[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -357,46 +389,55 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t v[4];
-      load_matrices_trans(v, (v_at + stage * kGroupBytes) ^ (j << 5));
-      if constexpr (decltype(masked)::value) {
+      load_matrices_trans(v, v_at ^ (j << 5));
+      if constexpr (PART) {
         v[0] &= keep0; v[1] &= keep0; v[2] &= keep1; v[3] &= keep1;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (decltype(one_token)::value) {
+        if constexpr (PART) {
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
           mma_16816(sum, v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (last_of(nt * 8 + 2 * t + (i & 1)) == only) o[nt][j][i] += sum[i];
+            if (w.last_of(a, nt * 8 + 2 * t + (i & 1)) == only) o[nt][j][i] += sum[i];
         } else {
           mma_16816(o[nt][j], v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
         }
       }
     }
-  };
-  // pair i of a tile's four scores, and its reference
-  auto pair = [&](const float (&s)[4], int i) { return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]); };
-  auto turns = [&](int nt) { return ONE ? make_float2(turn[nt].x, turn[nt].x) : turn[nt]; };
+  }
+  __device__ __forceinline__ float2 pair(const float (&s)[4], int i) const {
+    return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]);
+  }
+  __device__ __forceinline__ float2 turns(int nt) const { return ONE ? make_float2(turn[nt].x, turn[nt].x) : turn[nt]; }
 
-  auto compute = [&](int stage, int base, int live) {
-    float s[NT][4], s2[NT][4];  // two chains of products, for shorter ones
+  __device__ __forceinline__ void compute(const PagedAttnArgs& a, const PagedView& pv, const Item& w,
+                                          const unsigned char* group, int base, int live) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // what this lane points ldmatrix at: keys by (row, chunk), values by (chunk, row)
+    const int r8 = lane & 7, mi = lane >> 3;
+    const uint32_t at = sm100::smem_u32(group);
+    const uint32_t k_at = at + (r8 + (mi & 1) * 8) * 128 + (((mi >> 1) ^ r8) << 4);
+    const uint32_t v_at = at + 16 * kRowBytes + (r8 + (mi >> 1) * 8) * 128 + (((mi & 1) ^ r8) << 4);
+    constexpr int kChains = NT == 1 ? 2 : 1;  // a second chain of products, for shorter ones
+    float s[NT][4], s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       uint32_t k[4];
-      load_matrices(k, (k_at + stage * kGroupBytes) ^ (step << 5));
+      load_matrices(k, k_at ^ (step << 5));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        mma_16816(step & 1 ? s2[nt] : s[nt], k[0], k[1], k[2], k[3], q[nt][2 * step], q[nt][2 * step + 1]);
+        mma_16816(kChains == 2 && (step & 1) ? s2 : s[nt], k[0], k[1], k[2], k[3], q[nt][2 * step], q[nt][2 * step + 1]);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * a.scale;
+      for (int i = 0; i < 4; ++i) s[nt][i] = (kChains == 2 ? s[nt][i] + s2[i] : s[nt][i]) * a.scale;
     const bool whole = base + 16 <= live && a.sight.sees_group(base, w.lo, w.hi);
     if (!whole) {
 #pragma unroll
@@ -404,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int slot = base + g + (i >> 1) * 8;
-          if (slot >= live || !a.sight.sees(slot, last_of(nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
+          if (slot >= live || !a.sight.sees(slot, w.last_of(a, nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
         }
     }
     if (a.xs != nullptr) {
@@ -412,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = nt * 8 + 2 * t + (i & 1), slot = base + g + (i >> 1) * 8;
-          if (r < w.nr) a.xs[(w.kv(pv) * a.rows + w.r0 + r) * a.slots + slot] = s[nt][i];
+          const int r = nt * 8 + 2 * t + (i & 1);
+          if (r < w.nr) w.x_row(a, pv, r)[base + g + (i >> 1) * 8] = s[nt][i];
         }
     }
     float2 p[NT][NP];
@@ -422,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        p[nt][i] = weight_pair<KIND, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
+        p[nt][i] = weight_pair<KIND_, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
         high = fmaxf(high, fmaxf(p[nt][i].x, p[nt][i].y));
       }
     if (__any_sync(0xffffffffu, high > kMove)) {
@@ -434,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           if (top > m[nt][c]) {
-            const float to = weight_turn<KIND, false>(top);
-            const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND, false>(m[nt][c], to, a.log2n);
+            const float to = weight_turn<KIND_, false>(top);
+            const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND_, false>(m[nt][c], to, a.log2n);
             m[nt][c] = top;
             (c ? turn[nt].y : turn[nt].x) = to;
             (c ? l[nt].y : l[nt].x) *= f;
@@ -448,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
           }
         }
 #pragma unroll
-        for (int i = 0; i < NP; ++i) p[nt][i] = weight_pair<KIND, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
+        for (int i = 0; i < NP; ++i) p[nt][i] = weight_pair<KIND_, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
       }
     }
     uint32_t pk[NT][2];
@@ -460,116 +501,235 @@ __global__ void __launch_bounds__(kThreads, mma_ctas(NT))
       pk[nt][1] = ONE ? pack_pair(p[nt][0].y, 0.f) : pack_pair(p[nt][NP - 1].x, p[nt][NP - 1].y);
     }
     if (whole) {
-      add_values(stage, pk, std::false_type{}, 0u, 0u, std::false_type{}, 0);
+      add_values<false>(a, w, v_at, pk, 0u, 0u, 0);
       return;
     }
-    // Slots beyond the sequence hold anything: a weight of zero does not hide an
-    // infinity or NaN in a value, so their values are cleared. Where the rows of
-    // different tokens see different slots, the group is added token by token.
-    auto keep = [&](int i, int last) {
-      const int slot = base + 2 * t + i * 8;
-      return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
-             (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
-    };
-    if (w.lo == w.hi) {
-      add_values(stage, pk, std::true_type{}, keep(0, w.hi), keep(1, w.hi), std::false_type{}, 0);
-    } else {
-      for (int last = w.lo; last <= w.hi; ++last)
-        add_values(stage, pk, std::true_type{}, keep(0, last), keep(1, last), std::true_type{}, last);
+    // Slots that a row does not see hold anything: a weight of zero does not hide
+    // an infinity or NaN in a value, so such a group is added token by token with
+    // the values that the token does not see cleared.
+    for (int last = w.lo; last <= w.hi; ++last) {
+      auto keep = [&](int slot) {
+        return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
+               (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
+      };
+      add_values<true>(a, w, v_at, pk, keep(base + 2 * t), keep(base + 2 * t + 8), last);
     }
-  };
+  }
+  __device__ __forceinline__ void flush(const Item& w, float2* ml, float* dst) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < NP; ++c) {
+        float sum = ONE ? l[nt].x + l[nt].y : c ? l[nt].y : l[nt].x;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const int r = nt * 8 + 2 * t + c;
+        if (r >= w.nr) continue;
+        if (g == 0) ml[r] = make_float2(m[nt][c], sum);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dst[r * kD + 16 * j + g] = o[nt][j][c];
+          dst[r * kD + 16 * j + 8 + g] = o[nt][j][c + 2];
+        }
+      }
+  }
+};
 
-  // Page numbers are read one group further ahead than the copies that need them.
+// ------------------------------------------------------------------ the kernel
+// Decoding reads every key and value once and does little with it, so the kernel
+// is built around the loads. Every warp works for itself: one lane asks TMA for
+// the groups of the warp's share, 16 rows of keys and 16 of values, contiguous in
+// a page, kStages - 1 groups ahead into the warp's ring, across the ends of items;
+// the warp takes them from there. (bf16 boxes are swizzled by 128 bytes, so that
+// ldmatrix meets no bank twice.)
+template <typename E>
+constexpr int group_bytes() { return 2 * 16 * E::kRowBytes; }
+template <typename E>
+constexpr int ring_smem() { return 1024 + kWarps * E::kStages * group_bytes<E>(); }
+
+template <typename E>
+__global__ void __launch_bounds__(kThreads, E::kCtas)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                      const PagedAttnArgs a, const PagedView pv) {
+  constexpr int kStages = E::kStages, kBytes = group_bytes<E>();
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t s_full[kWarps][kStages];
+  __shared__ int4 s_meta[kWarps][kStages];  // item, first slot, live slots
+  __shared__ int64_t s_excl[kThreads];
+  __shared__ int64_t s_warp[kWarps];
+  __shared__ int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned char* const ring =
+      smem_raw + (1024 - (sm100::smem_u32(smem_raw) & 1023)) + warp * kStages * kBytes;
+  uint64_t* const full = s_full[warp];
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&full[i], 1);
+    sm100::fence_mbar_init();
+    if (warp == 0) abort_flag = 0;
+  }
+  // the line: every thread counts a run of sequences
+  const int run = (a.B + kThreads - 1) / kThreads;
+  int64_t mine = 0;
+  for (int i = 0; i < run; ++i) {
+    const int b = threadIdx.x * run + i;
+    if (b < a.B) mine += head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
+  }
+  int64_t sum = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, sum, off);
+    if (lane >= off) sum += up;
+  }
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += s_warp[i];
+    total += s_warp[i];
+  }
+  s_excl[threadIdx.x] = before + sum - mine;
+  __syncthreads();
+  const int64_t share = share_of(a, total);
+  const int wid = warp * gridDim.x + blockIdx.x;  // neighbours in the line sit on different SMs
+  const int64_t start = wid * share;
+  if (start >= total) return;
+  int left = (int)min(share, total - start), to_issue = left;
+
+  Cursor at(a, pv, s_excl, run, start);
+  auto page_of = [&]() {
+    return to_issue > 0 ? pv.table[(int64_t)at.b * pv.max_pages + (at.span.slot(at.grp) >> pv.page_shift)] : 0;
+  };
+  int pid = page_of();
+  // One lane fetches. A page that does not exist is replaced by page 0 and its
+  // slots are masked.
+  auto issue = [&](int stage) {
+    if (to_issue <= 0) return;
+    const bool known = (unsigned)pid < (unsigned)pv.num_pages;
+    const int slot = at.span.slot(at.grp);
+    if (lane == 0) {
+      if (!known) atomicOr(a.err, DEV_ERR_BAD_PAGE);
+      const int row = (int)(paged_row(pv, known ? pid : 0, at.h, slot) / kD);
+      s_meta[warp][stage] = make_int4(at.item, slot, known ? at.len : 0, 0);
+      sm100::mbar_expect_tx(&full[stage], kBytes);
+      sm100::tma_load_2d(ring + stage * kBytes, &k_map, &full[stage], 0, row);
+      sm100::tma_load_2d(ring + stage * kBytes + kBytes / 2, &v_map, &full[stage], 0, row);
+    }
+    if (--to_issue > 0) at.next(a, pv);
+    pid = page_of();  // read one group further ahead than the copy that needs it
+  };
+  int item = at.item;
+  Item w(a, pv, item);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+  E e;
+  e.begin(a, pv, w);
+
   volatile int* const abort_v = &abort_flag;
   uint32_t parity = 0;
   int stage = 0, in = kStages - 1;
-  bool ok = true;
-  __syncthreads();
-  while (grp < g_end) {
+  while (left > 0) {
     __syncwarp();  // every lane has taken the group whose place this copy gets
-    issue(in, grp + (kStages - 1) * kWarps, ahead);
-    ahead = page_of(grp + kStages * kWarps);
-    ok = sm100::mbar_wait_warp(&full[stage], parity, abort_v, a.err);
-    if (!ok) break;
-    compute(stage, span.slot(grp), missing >> stage & 1 ? 0 : w.len);
-    grp += kWarps;
+    issue(in);
+    if (!sm100::mbar_wait_warp(&full[stage], parity, abort_v, a.err)) break;
+    const int4 meta = s_meta[warp][stage];
+    if (meta.x != item) {
+      e.flush(w, a.part_ml + (int64_t)(wid + item) * a.tile_rows, a.part_o + (int64_t)(wid + item) * a.tile_rows * kD);
+      item = meta.x;
+      w = Item(a, pv, item);
+      e.begin(a, pv, w);
+    }
+    e.compute(a, pv, w, ring + stage * kBytes, meta.y, meta.z);
+    --left;
     in = stage;
     if (++stage == kStages) {
       stage = 0;
       parity ^= 1;
     }
   }
-  if (!ok) {  // a copy did not arrive in time: let those on their way land, within limits, before the CTA ends
+  pdl_trigger();
+  e.flush(w, a.part_ml + (int64_t)(wid + item) * a.tile_rows, a.part_o + (int64_t)(wid + item) * a.tile_rows * kD);
+  if (left > 0) {  // a copy did not arrive in time: let those on their way land, within limits, before the CTA ends
     volatile int quiet = 0;
-    for (int i = 0; i < kStages && grp + i * kWarps < g_end; ++i)
+    for (int i = 0; i < kStages && i < left - to_issue; ++i)
       sm100::mbar_wait(&full[(stage + i) % kStages], parity ^ (stage + i >= kStages), &quiet, nullptr);
   }
-  pdl_trigger();
-  __syncthreads();  // the rings are free
-
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float sum = c ? (ONE ? 0.f : l[nt].y) : (ONE ? l[nt].x + l[nt].y : l[nt].x);
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      const int r = nt * 8 + 2 * t + c;
-      if (g == 0) s_ml[r * kWarps + warp] = make_float2(m[nt][c], sum);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s_o[(r * kWarps + warp) * kD + 16 * j + g] = o[nt][j][c];
-        s_o[(r * kWarps + warp) * kD + 16 * j + 8 + g] = o[nt][j][c + 2];
-      }
-    }
-  }
-  __syncthreads();
-  merge_parts<T, KIND, kWarps>(a, pv, w, s_o, s_ml);
 }
 
 // ------------------------------------------------------------------------ join
-// Blocks below `rows` join one row's splits; the others add the weights of their
-// slots over the rows of one kv head.
-constexpr int kScoreSlots = 1024;
+// Blocks below `rows` join one row's partial results; the others add the weights
+// of their slots over the rows of one kv head.
+constexpr int kScoreSlots = 512;
 constexpr int kRowChunk = 64;
 
-// Reference and sum of one row over its splits and the sink, by one warp.
+// Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
+__device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// The partial results of one item: indices first .. first + count - 1, and the row
+// in its tile.
+struct Parts {
+  int64_t first;
+  int count, row;
+  __device__ __forceinline__ Parts(const PagedAttnArgs& a, const PagedView& pv, const Line& line, int b, int h, int len,
+                                   int r) {
+    const int tile = r / a.tile_rows;
+    row = r - tile * a.tile_rows;
+    const int64_t begin = line.before + h * head_groups(a, len, a.tiles) + head_groups(a, len, tile);
+    const int groups = item_span(a, len, tile).total;
+    const int64_t lo = begin / line.share, hi = (begin + groups - 1) / line.share;
+    first = lo + ((int64_t)b * pv.heads + h) * a.tiles + tile;
+    count = groups ? (int)(hi - lo) + 1 : 0;
+  }
+};
+
+// Reference and sum of one row over its parts and the sink, by one warp.
 template <int KIND, bool EXACT>
-__device__ __forceinline__ void join_row(const PagedAttnArgs& a, int64_t row, float sink, float& turn, float& L) {
+__device__ __forceinline__ void join_row(const PagedAttnArgs& a, const Parts& p, float sink, float& turn, float& L) {
   const int lane = threadIdx.x & 31;
-  const float2* ml = a.part_ml + row * a.splits;
+  const float2* ml = a.part_ml + p.first * a.tile_rows + p.row;
   float M = sink;  // -inf without a sink
-  for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, ml[s].x);
+  for (int s = lane; s < p.count; s += 32) M = fmaxf(M, ml[(int64_t)s * a.tile_rows].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   turn = weight_turn<KIND, EXACT>(M);
   L = lane == 0 && sink != kNegInf ? weight_of<KIND, EXACT>(sink, turn, a.log2n) : 0.f;
-  for (int s = lane; s < a.splits; s += 32) {
-    const float2 x = ml[s];
+  for (int s = lane; s < p.count; s += 32) {
+    const float2 x = ml[(int64_t)s * a.tile_rows];
     if (x.x != kNegInf || x.y != 0.f) L = fmaf(x.y, weight_of<KIND, EXACT>(x.x, turn, a.log2n), L);
   }
   L = row_sum<32>(L);
+}
+
+__device__ __forceinline__ float sink_score(const PagedAttnArgs& a, int h, int row) {
+  return a.sink ? a.sink[h * a.G + row % a.G] * a.inv_unit : kNegInf;
 }
 
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArgs a, const PagedView pv, int blocks) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int kQuads = kD / 4, kGroups = kThreads / kQuads;
-  pdl_wait();
   const int64_t bh = blockIdx.x / (unsigned)blocks;
   const int which = (int)(blockIdx.x - bh * blocks);
   const int h = (int)(bh % pv.heads), b = (int)(bh / pv.heads);
+  // lengths and sinks were there before the kernel that this one waits for
+  const int len = paged_len(pv, b, a.err);
+  const Line line = line_before(a, pv, b);
   if (which < a.rows) {
     __shared__ float4 s_part[kGroups][kQuads];
-    const int64_t row = bh * a.rows + which;
+    const Parts p(a, pv, line, b, h, len, which);
+    const float sink = sink_score(a, h, which);
+    pdl_wait();
     float turn, L;
-    join_row<KIND, EXACT>(a, row, sink_score(a, h, which), turn, L);
+    join_row<KIND, EXACT>(a, p, sink, turn, L);
     const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = grp; s < a.splits; s += kGroups) {
-      const float2 ml = a.part_ml[row * a.splits + s];
-      const float4 x = reinterpret_cast<const float4*>(a.part_o)[(row * a.splits + s) * kQuads + quad];
+    for (int s = grp; s < p.count; s += kGroups) {
+      const int64_t at = (p.first + s) * a.tile_rows + p.row;
+      const float2 ml = a.part_ml[at];
+      const float4 x = reinterpret_cast<const float4*>(a.part_o)[at * kQuads + quad];
       const float f = ml.x == kNegInf && ml.y == 0.f ? 0.f : weight_of<KIND, EXACT>(ml.x, turn, a.log2n);
       O.x = fmaf(x.x, f, O.x); O.y = fmaf(x.y, f, O.y); O.z = fmaf(x.z, f, O.z); O.w = fmaf(x.w, f, O.w);
     }
@@ -585,127 +745,126 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
     }
     return;
   }
+  constexpr int kEach = kScoreSlots / kThreads;
   __shared__ float s_turn[kRowChunk], s_inv[kRowChunk];
-  const int len = paged_len(pv, b, a.err);
-  const int64_t s0 = (int64_t)(which - a.rows) * kScoreSlots;
-  float sum[kScoreSlots / kThreads];
+  const int64_t s0 = (int64_t)(which - a.rows) * kScoreSlots + threadIdx.x;
+  float old[kEach], sum[kEach];
 #pragma unroll
-  for (int i = 0; i < kScoreSlots / kThreads; ++i) sum[i] = 0.f;
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t s = s0 + i * kThreads;
+    old[i] = s < len - a.T ? a.scores[bh * a.slots + s] : 0.f;
+    sum[i] = 0.f;
+  }
+  pdl_wait();
   for (int r0 = 0; r0 < a.rows; r0 += kRowChunk) {
     const int nr = min(kRowChunk, a.rows - r0);
     __syncthreads();
     for (int r = threadIdx.x >> 5; r < nr; r += kWarps) {
       float turn, L;
-      join_row<KIND, EXACT>(a, bh * a.rows + r0 + r, sink_score(a, h, r0 + r), turn, L);
+      join_row<KIND, EXACT>(a, Parts(a, pv, line, b, h, len, r0 + r), sink_score(a, h, r0 + r), turn, L);
       s_turn[r] = turn;
       s_inv[r] = row_scale(L);
     }
     __syncthreads();
+    for (int r = 0; r < nr; ++r) {
+      const float* x = a.xs + (bh * a.rows + r0 + r) * a.slots;
+      const int last = len - a.T + (r0 + r) / a.G;
+      float xv[kEach];
 #pragma unroll
-    for (int i = 0; i < kScoreSlots / kThreads; ++i) {
-      const int64_t s = s0 + threadIdx.x + (int64_t)i * kThreads;
-      if (s >= len) continue;
-      for (int r = 0; r < nr; ++r) {
-        if (!a.sight.sees((int)s, len - a.T + (r0 + r) / a.G)) continue;
-        const float x = a.xs[(bh * a.rows + r0 + r) * a.slots + s];
-        sum[i] += weight_of<KIND, EXACT>(x, s_turn[r], a.log2n) * s_inv[r];
+      for (int i = 0; i < kEach; ++i) {
+        const int64_t s = s0 + i * kThreads;
+        xv[i] = s < len && a.sight.sees((int)s, last) ? x[s] : kNegInf;
       }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (xv[i] != kNegInf) sum[i] += weight_of<KIND, EXACT>(xv[i], s_turn[r], a.log2n) * s_inv[r];
     }
   }
 #pragma unroll
-  for (int i = 0; i < kScoreSlots / kThreads; ++i) {
-    const int64_t s = s0 + threadIdx.x + (int64_t)i * kThreads;
-    if (s >= a.slots) continue;
-    const float old = s < len - a.T ? a.scores[bh * a.slots + s] : 0.f;
-    a.scores_out[bh * a.slots + s] = old + sum[i];
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t s = s0 + i * kThreads;
+    if (s < a.slots) a.scores_out[bh * a.slots + s] = old[i] + sum[i];
   }
 }
 
 // ------------------------------------------------------------------------ host
 struct Plan {
-  int64_t rows, tile_rows, tiles, splits;
-  size_t ml, o, xs, bytes;
+  int64_t rows, tile_rows, tiles, items, warps;
+  size_t o, xs, bytes;
 };
 
-// Slots a query can see at most, in groups of 16.
-int64_t visible_groups(int64_t S, int64_t T, int64_t window, int64_t first) {
-  const int64_t all = (S + 15) / 16;
-  if (window == 0) return all;
-  return std::min(all, (window + T + 15) / 16 + 1 + (std::min(first, S) + 15) / 16);
-}
-
-Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, int64_t window, int64_t first, bool scored,
-               bool wide) {
+Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool scored, bool wide) {
   Plan p = {};
   p.rows = T * (Hq / Hkv);
-  if (wide)  // bf16: tiles of up to 32 rows, as even as they come
-    p.tile_rows = (((p.rows + 31) / 32 - 1 + p.rows) / ((p.rows + 31) / 32) + 7) / 8 * 8;
-  else
+  int ctas;
+  if (wide) {  // bf16: tiles of up to 32 rows, as even as they come
+    const int64_t tiles = (p.rows + 31) / 32;
+    p.tile_rows = ((p.rows + tiles - 1) / tiles + 7) / 8 * 8;
+    ctas = p.tile_rows == 8 ? 4 : p.tile_rows == 16 ? 3 : 2;
+  } else {
     p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
+    ctas = 3;
+  }
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
-  const int64_t groups = visible_groups(S, T, window, first);
-  const int64_t base = std::max<int64_t>(1, B * Hkv * p.tiles);
-  const int64_t want = (148 * 8 + base - 1) / base;
-  p.splits = std::max<int64_t>(1, std::min(want, (groups + kMinGroups - 1) / kMinGroups));
+  p.items = B * Hkv * p.tiles;
+  // one wave of CTAs, fewer where even the full tables hold less than kMinShare groups a warp
+  const int64_t most = (p.items * ((S + 15) / 16) + kMinShare - 1) / kMinShare;
+  p.warps = std::min<int64_t>(kSms * ctas, (most + kWarps - 1) / kWarps) * kWarps;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.ml = 0;
-  p.o = up((size_t)(B * Hkv * p.rows * p.splits) * sizeof(float2));
-  p.xs = p.o + up((size_t)(B * Hkv * p.rows * p.splits) * kD * sizeof(float));
+  const size_t parts = (size_t)((p.warps + p.items) * p.tile_rows);
+  p.o = up(parts * sizeof(float2));
+  p.xs = p.o + up(parts * kD * sizeof(float));
   p.bytes = p.xs + (scored ? up((size_t)(B * Hkv * p.rows * S) * sizeof(float)) : 0);
   return p;
 }
 
-template <int KIND, int LOG2N, int NT, bool ONE>
-int mma_launch(const PagedAttnArgs& a, const PagedView& pv, const CUtensorMap& k, const CUtensorMap& v, unsigned grid,
-               cudaStream_t st) {
-  auto* kern = paged_attn_mma_kernel<KIND, LOG2N, NT, ONE>;
+template <typename E>
+int attn_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+  constexpr int dtype = sizeof(typename E::T) == 2 ? ALGX_BF16 : ALGX_F32;
   static std::atomic<uint64_t> ready{0};  // one bit per device: its shared memory limit is raised
+  auto* kern = paged_attn_kernel<E>;
   int dev = 0;
   ALGX_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    ALGX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, mma_smem(NT)));
+    ALGX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_smem<E>()));
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  kern<<<grid, kThreads, mma_smem(NT), st>>>(k, v, a, pv);
+  const int64_t rows = ((int64_t)pv.num_pages * pv.heads) << pv.page_shift;
+  ALGX_REQUIRE(rows <= INT32_MAX, "paged cache too large");
+  CUtensorMap k, v;
+  if (int e = make_tmap_2d(&k, a.k, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, 16, E::kSwizzle)) return e;
+  if (int e = make_tmap_2d(&v, a.v, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, 16, E::kSwizzle)) return e;
+  kern<<<a.warps / kWarps, kThreads, ring_smem<E>(), st>>>(k, v, a, pv);
+  ALGX_LAUNCHED("paged_attn_kernel");
   return ALGX_OK;
 }
 
 template <int KIND, int LOG2N>
-int mma_launch_rows(const PagedAttnArgs& a, const PagedView& pv, unsigned grid, cudaStream_t st) {
-  const int64_t rows = ((int64_t)pv.num_pages * pv.heads) << pv.page_shift;
-  ALGX_REQUIRE(rows <= INT32_MAX, "paged cache too large");
-  CUtensorMap k, v;
-  if (int e = make_tmap_2d(&k, a.k, ALGX_BF16, kD, (uint64_t)rows, kD * 2, kD, 16, true)) return e;
-  if (int e = make_tmap_2d(&v, a.v, ALGX_BF16, kD, (uint64_t)rows, kD * 2, kD, 16, true)) return e;
-  return a.rows == 1         ? mma_launch<KIND, LOG2N, 1, true>(a, pv, k, v, grid, st)
-         : a.tile_rows == 8  ? mma_launch<KIND, LOG2N, 1, false>(a, pv, k, v, grid, st)
-         : a.tile_rows == 16 ? mma_launch<KIND, LOG2N, 2, false>(a, pv, k, v, grid, st)
-         : a.tile_rows == 24 ? mma_launch<KIND, LOG2N, 3, false>(a, pv, k, v, grid, st)
-                             : mma_launch<KIND, LOG2N, 4, false>(a, pv, k, v, grid, st);
+int mma_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+  return a.rows == 1         ? attn_launch<MmaEngine<KIND, LOG2N, 1, true>>(a, pv, st)
+         : a.tile_rows == 8  ? attn_launch<MmaEngine<KIND, LOG2N, 1, false>>(a, pv, st)
+         : a.tile_rows == 16 ? attn_launch<MmaEngine<KIND, LOG2N, 2, false>>(a, pv, st)
+         : a.tile_rows == 24 ? attn_launch<MmaEngine<KIND, LOG2N, 3, false>>(a, pv, st)
+                             : attn_launch<MmaEngine<KIND, LOG2N, 4, false>>(a, pv, st);
 }
 
 template <typename T, int KIND>
-int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int64_t B, cudaStream_t st) {
-  const int64_t grid = B * pv.heads * p.splits * p.tiles;
-  ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
-  if constexpr (sizeof(T) == 2) {
-    const int e = KIND == kAsinh && a.log2n == 4 ? mma_launch_rows<KIND, 4>(a, pv, (unsigned)grid, st)
-                                                 : mma_launch_rows<KIND, 0>(a, pv, (unsigned)grid, st);
-    if (e) return e;
-  } else {
-    auto* kern = p.tile_rows == 1   ? paged_attn_kernel<T, KIND, 1>
-                 : p.tile_rows == 2 ? paged_attn_kernel<T, KIND, 2>
-                 : p.tile_rows == 4 ? paged_attn_kernel<T, KIND, 4>
-                                    : paged_attn_kernel<T, KIND, 8>;
-    kern<<<(unsigned)grid, kThreads, 0, st>>>(a, pv);
-  }
-  ALGX_LAUNCHED("paged_attn_kernel");
-  if (a.direct) return ALGX_OK;
+int paged_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+  int e;
+  if constexpr (sizeof(T) == 2)
+    e = KIND == kAsinh && a.log2n == 4 ? mma_launch<KIND, 4>(a, pv, st) : mma_launch<KIND, 0>(a, pv, st);
+  else
+    e = a.tile_rows == 1   ? attn_launch<FmaEngine<KIND, 1>>(a, pv, st)
+        : a.tile_rows == 2 ? attn_launch<FmaEngine<KIND, 2>>(a, pv, st)
+        : a.tile_rows == 4 ? attn_launch<FmaEngine<KIND, 4>>(a, pv, st)
+                           : attn_launch<FmaEngine<KIND, 8>>(a, pv, st);
+  if (e) return e;
   const int64_t blocks = a.rows + (a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0);
-  ALGX_REQUIRE(blocks * B * pv.heads <= INT32_MAX, "too many rows");
-  ALGX_CUDA(launch_dependent(paged_join_kernel<T, KIND>, dim3((unsigned)(blocks * B * pv.heads)), dim3(kThreads), 0, st,
-                             a, pv, (int)blocks));
+  const int64_t grid = blocks * a.B * pv.heads;
+  ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
+  ALGX_CUDA(launch_dependent(paged_join_kernel<T, KIND>, dim3((unsigned)grid), dim3(kThreads), 0, st, a, pv,
+                             (int)blocks));
   ALGX_LAUNCHED("paged_join_kernel");
   return ALGX_OK;
 }
@@ -716,11 +875,9 @@ int paged_launch(const PagedAttnArgs& a, const PagedView& pv, const Plan& p, int
 extern "C" {
 
 size_t algx_paged_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t page_size,
-                                      int64_t max_pages, int64_t window, int64_t first, int32_t scored,
-                                      int32_t dtype) {
+                                      int64_t max_pages, int32_t scored, int32_t dtype) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || page_size <= 0 || max_pages <= 0) return 0;
-  return algx::make_plan(B, T, Hq, Hkv, page_size * max_pages, window, first, scored != 0,
-                         dtype == ALGX_BF16).bytes;
+  return algx::make_plan(B, T, Hq, Hkv, page_size * max_pages, scored != 0, dtype == ALGX_BF16).bytes;
 }
 
 int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_pages, const void* v_pages,
@@ -743,32 +900,31 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   ALGX_REQUIRE((scores == nullptr) == (scores_out == nullptr), "give scores and scores_out or neither");
   ALGX_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)workspace) & 15) == 0,
                "tensors must be 16-byte aligned");
-  ALGX_REQUIRE(T * (Hq / Hkv) <= INT32_MAX / 64, "too many rows");
+  ALGX_REQUIRE(T <= INT32_MAX && T * (Hq / Hkv) <= INT32_MAX / 64, "too many rows");
   const int64_t S = page_size * max_pages;
-  const Plan p = make_plan(B, T, Hq, Hkv, S, cfg->window, cfg->first, scores != nullptr, dtype == ALGX_BF16);
+  const Plan p = make_plan(B, T, Hq, Hkv, S, scores != nullptr, dtype == ALGX_BF16);
+  ALGX_REQUIRE(p.items + p.warps <= INT32_MAX, "too many rows");
   ALGX_REQUIRE(workspace && workspace_bytes >= p.bytes, "workspace too small");
   PagedAttnArgs a = {};
   a.q = q; a.k = k_pages; a.v = v_pages; a.sink = sink; a.scores = scores; a.scores_out = scores_out; a.o = o;
   char* ws = static_cast<char*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
+  a.part_ml = reinterpret_cast<float2*>(ws);
   a.part_o = reinterpret_cast<float*>(ws + p.o);
   a.xs = scores ? reinterpret_cast<float*>(ws + p.xs) : nullptr;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  a.slots = S; a.T = (int)T; a.G = (int)(Hq / Hkv); a.rows = (int)p.rows; a.tiles = (int)p.tiles;
-  a.splits = (int)p.splits;
-  while ((1 << a.log2n) < cfg->n) ++a.log2n;
+  a.slots = S; a.B = (int)B; a.T = (int)T; a.G = (int)(Hq / Hkv); a.rows = (int)p.rows;
+  a.tile_rows = (int)p.tile_rows; a.tiles = (int)p.tiles; a.warps = (int)p.warps;
   const bool soft = cfg->kind == ALGX_ATTN_SOFTMAX;
+  if (!soft)
+    while ((1 << a.log2n) < cfg->n) ++a.log2n;
   a.scale = soft ? cfg->scale * kLog2e : cfg->scale;
   a.inv_unit = soft ? cfg->inv_unit * kLog2e : cfg->inv_unit;
-  a.tile_rows = (int)p.tile_rows;
-  a.direct = p.splits == 1 && scores == nullptr;
   a.sight = {cfg->window, cfg->first};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == ALGX_BF16)
-    return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, p, B, st)
-                : paged_launch<__nv_bfloat16, kAsinh>(a, pv, p, B, st);
-  return soft ? paged_launch<float, kSoftmax>(a, pv, p, B, st) : paged_launch<float, kAsinh>(a, pv, p, B, st);
+    return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, st) : paged_launch<__nv_bfloat16, kAsinh>(a, pv, st);
+  return soft ? paged_launch<float, kSoftmax>(a, pv, st) : paged_launch<float, kAsinh>(a, pv, st);
 }
 
 }  // extern "C"

@@ -376,8 +376,7 @@ typedef struct algx_paged_config {
 /* Bytes of workspace algx_paged_attn needs (no initialisation needed); scored:
  * whether scores are given. No counterpart in the reference. */
 ALGX_API size_t algx_paged_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t page_size,
-                                               int64_t max_pages, int64_t window, int64_t first, int32_t scored,
-                                               int32_t dtype);
+                                               int64_t max_pages, int32_t scored, int32_t dtype);
 
 /* Attention of the T newest tokens of every sequence over its cached slots.
  * q, o (B, T, Hq, D); Hq a multiple of Hkv, query head j reads kv head

@@ -127,5 +127,5 @@ def test_c_entries_refuse_without_a_device():
     assert lib.algx_cache_evict(*[None] * 6, 4, 3, 2, *[None] * 4, 0, 1, 1, 16, 1, 64, L.ALGX_BF16, None, 0,
                                 None) == L.ALGX_ERR_INVALID
     assert b"fit the budget" in lib.algx_last_error()
-    assert lib.algx_paged_attn_workspace_size(1, 1, 3, 2, 16, 1, 0, 0, 0, L.ALGX_BF16) == 0
+    assert lib.algx_paged_attn_workspace_size(1, 1, 3, 2, 16, 1, 0, L.ALGX_BF16) == 0
     assert lib.algx_cache_evict_workspace_size(2, 3, 5) >= 2 * 3 * 5 * 4
