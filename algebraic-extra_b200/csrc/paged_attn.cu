@@ -26,7 +26,7 @@ constexpr int kD = 64;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
-constexpr int kMinShare = 4;  // groups of 16 slots a warp takes at least
+constexpr int kMinSlots = 64;  // slots a warp takes at least
 
 struct PagedAttnArgs {
   const void *q, *k, *v;
@@ -39,13 +39,14 @@ struct PagedAttnArgs {
   int* err;
   int64_t slots;    // S: slots of one sequence's table
   int B, T, G, rows, tile_rows, tiles, warps, log2n;
+  int shift;        // log2 of the slots of a group
   float scale, inv_unit;
   Sight sight;
 };
 
 // ------------------------------------------------------------- division of work
 // An item is one tile of up to tile_rows rows of one kv head of one sequence; its
-// work is the groups of 16 slots that its rows look at. All items' groups stand in
+// work is the groups of 16 or 32 slots that its rows look at. All items' groups stand in
 // one line, (sequence, head, tile, group), which is cut into equal shares, one a
 // warp, whatever the sequences' lengths: a share can end one item and begin the
 // next ones. Every warp writes one partial result for every item it touches, at
@@ -64,7 +65,7 @@ struct Rows {
 };
 __device__ __forceinline__ Span item_span(const PagedAttnArgs& a, int len, int tile) {
   const Rows r(a, len, tile);
-  return Span(a.sight, r.lo, r.hi);
+  return Span(a.sight, a.shift, r.lo, r.hi);
 }
 // Groups of one kv head of a sequence: all tiles', or those before `tiles`.
 __device__ __forceinline__ int64_t head_groups(const PagedAttnArgs& a, int len, int tiles) {
@@ -84,7 +85,8 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t x) {
 }
 __device__ __forceinline__ int64_t share_of(const PagedAttnArgs& a, int64_t total) {
   const int64_t even = (total + a.warps - 1) / a.warps;
-  return even < kMinShare ? kMinShare : even;
+  const int least = kMinSlots >> a.shift;
+  return even < least ? least : even;
 }
 __device__ __forceinline__ Line line_before(const PagedAttnArgs& a, const PagedView& pv, int upto) {
   __shared__ int64_t s_sum[2][kWarps];
@@ -119,7 +121,7 @@ struct Cursor {
   // The `at`-th group, for a warp; `excl` (kThreads) holds the groups before each
   // thread's run of `run` sequences.
   __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, const int64_t* excl, int run,
-                                    int64_t at) : span(a.sight, -1, -1) {
+                                    int64_t at) : span(a.sight, a.shift, -1, -1) {
     int lo = 0;
     for (int step = kThreads / 2; step > 0; step >>= 1)
       if (excl[lo + step] <= at) lo += step;
@@ -145,6 +147,7 @@ struct Cursor {
     grp = (int)at;
     item = (b * pv.heads + h) * a.tiles + tile;
   }
+  __device__ __forceinline__ int slot(const PagedAttnArgs& a) const { return span.group(grp) << a.shift; }
   // On to the next group, if there is one.
   __device__ __forceinline__ void next(const PagedAttnArgs& a, const PagedView& pv) {
     if (++grp < span.total) return;
@@ -198,7 +201,7 @@ constexpr float kMove = 256.f;
 template <int KIND_, int R>
 struct FmaEngine {
   using T = float;
-  static constexpr int kStages = 2, kCtas = 3, kRowBytes = kD * 4;
+  static constexpr int kSlots = 16, kStages = 2, kCtas = 3, kRowBytes = kD * 4;
   static constexpr bool kSwizzle = false;
   float4 q[R], acc[R];
   float m[R], turn[R], l[R];
@@ -221,7 +224,7 @@ struct FmaEngine {
                                           const unsigned char* group, int base, int live) {
     const int lane = threadIdx.x & 31, sub = lane & 15, rl = lane >> 4;
     const float4* k = reinterpret_cast<const float4*>(group) + lane;
-    const float4* v = k + 16 * kRowBytes / 16;
+    const float4* v = k + kSlots * kRowBytes / 16;
     const int slot = base + (sub & ~1) + rl;  // whose score this lane ends up with
     float p[R];
     float high = 0.f;
@@ -268,7 +271,7 @@ struct FmaEngine {
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) l[r] += p[r];
-    const bool whole = base + 16 <= live && a.sight.sees_group(base, w.lo, w.hi);
+    const bool whole = base + kSlots <= live && a.sight.sees_all(base, kSlots, w.lo, w.hi);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float4 vv = v[i * 32];
@@ -343,8 +346,10 @@ __device__ __forceinline__ void load_matrices_trans(uint32_t (&r)[4], uint32_t a
 template <int KIND_, int LOG2N, int NT, bool ONE>
 struct MmaEngine {
   using T = __nv_bfloat16;
-  static constexpr int kStages = NT == 1 ? 3 : NT == 2 ? 4 : 6, kCtas = NT == 1 ? 4 : NT == 2 ? 3 : 2,
-                       kRowBytes = kD * 2;
+  // Groups of 32 slots: copies of 4 KB. Read in 2 KB pieces memory gives a tenth
+  // less (6.0 TB/s instead of 6.6 in a bare ring of this form).
+  static constexpr int kSlots = 32, kStages = NT <= 2 ? 2 : 3, kCtas = NT <= 2 ? 3 : 2, kRowBytes = kD * 2;
+  static constexpr int kSub = NT == 1 ? 2 : 1;  // 16-slot steps worked on together
   static constexpr bool kSwizzle = true;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
   // row (only the first column counts), of its two slots.
@@ -373,9 +378,9 @@ struct MmaEngine {
         for (int i = 0; i < 4; ++i) o[nt][j][i] = 0.f;
     }
   }
-  // O^T += V^T P^T. PART: values outside keep0, keep1 (bits of slots 2 t, 2 t + 1
-  // and 2 t + 8, 2 t + 9) are taken as zero, and only the rows whose last visible
-  // slot is `only` receive the sum.
+  // O^T += V^T P^T for 16 slots. PART: values outside keep0, keep1 (bits of slots
+  // 2 t, 2 t + 1 and 2 t + 8, 2 t + 9) are taken as zero, and only the rows whose
+  // last visible slot is `only` receive the sum.
   template <bool PART>
   __device__ __forceinline__ void add_values(const PagedAttnArgs& a, const Item& w, uint32_t v_at,
                                              const uint32_t (&p)[NT][2], uint32_t keep0, uint32_t keep1, int only) {
@@ -414,64 +419,74 @@ struct MmaEngine {
 
   __device__ __forceinline__ void compute(const PagedAttnArgs& a, const PagedView& pv, const Item& w,
                                           const unsigned char* group, int base, int live) {
+    const bool whole = base + kSlots <= live && a.sight.sees_all(base, kSlots, w.lo, w.hi);
+#pragma unroll
+    for (int i = 0; i < kSlots / 16; i += kSub) step(a, pv, w, sm100::smem_u32(group) + i * 16 * kRowBytes, base + i * 16, live, whole);
+  }
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, const PagedView& pv, const Item& w, uint32_t at, int base,
+                                       int live, bool whole) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // what this lane points ldmatrix at: keys by (row, chunk), values by (chunk, row)
     const int r8 = lane & 7, mi = lane >> 3;
-    const uint32_t at = sm100::smem_u32(group);
     const uint32_t k_at = at + (r8 + (mi & 1) * 8) * 128 + (((mi >> 1) ^ r8) << 4);
-    const uint32_t v_at = at + 16 * kRowBytes + (r8 + (mi >> 1) * 8) * 128 + (((mi & 1) ^ r8) << 4);
-    constexpr int kChains = NT == 1 ? 2 : 1;  // a second chain of products, for shorter ones
-    float s[NT][4], s2[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t v_at = at + kSlots * kRowBytes + (r8 + (mi >> 1) * 8) * 128 + (((mi & 1) ^ r8) << 4);
+    float s[kSub][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      uint32_t k[4];
-      load_matrices(k, k_at ^ (step << 5));
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        mma_16816(kChains == 2 && (step & 1) ? s2 : s[nt], k[0], k[1], k[2], k[3], q[nt][2 * step], q[nt][2 * step + 1]);
-    }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 4; ++i) s[u][nt][i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = (kChains == 2 ? s[nt][i] + s2[i] : s[nt][i]) * a.scale;
-    const bool whole = base + 16 <= live && a.sight.sees_group(base, w.lo, w.hi);
-    if (!whole) {
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        uint32_t k[4];
+        load_matrices(k, (k_at + u * 16 * kRowBytes) ^ (c << 5));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16816(s[u][nt], k[0], k[1], k[2], k[3], q[nt][2 * c], q[nt][2 * c + 1]);
+      }
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int slot = base + g + (i >> 1) * 8;
-          if (slot >= live || !a.sight.sees(slot, w.last_of(a, nt * 8 + 2 * t + (i & 1)))) s[nt][i] = kNegInf;
+          s[u][nt][i] *= a.scale;
+          const int slot = base + u * 16 + g + (i >> 1) * 8;
+          if (!whole && (slot >= live || !a.sight.sees(slot, w.last_of(a, nt * 8 + 2 * t + (i & 1)))))
+            s[u][nt][i] = kNegInf;
         }
-    }
     if (a.xs != nullptr) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = nt * 8 + 2 * t + (i & 1);
-          if (r < w.nr) w.x_row(a, pv, r)[base + g + (i >> 1) * 8] = s[nt][i];
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = nt * 8 + 2 * t + (i & 1), slot = base + u * 16 + g + (i >> 1) * 8;
+            if (r < w.nr && slot < a.slots) w.x_row(a, pv, r)[slot] = s[u][nt][i];
+          }
     }
-    float2 p[NT][NP];
+    float2 p[kSub][NT][NP];
     float high = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        p[nt][i] = weight_pair<KIND_, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
-        high = fmaxf(high, fmaxf(p[nt][i].x, p[nt][i].y));
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          p[u][nt][i] = weight_pair<KIND_, LOG2N>(pair(s[u][nt], i), turns(nt), a.log2n);
+          high = fmaxf(high, fmaxf(p[u][nt][i].x, p[u][nt][i].y));
+        }
     if (__any_sync(0xffffffffu, high > kMove)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int c = 0; c < NP; ++c) {
-          float top = fmaxf(s[nt][c], s[nt][c + 2]);
+          float top = kNegInf;
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) top = fmaxf(top, fmaxf(s[u][nt][c], s[u][nt][c + 2]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           if (top > m[nt][c]) {
@@ -489,30 +504,39 @@ struct MmaEngine {
           }
         }
 #pragma unroll
-        for (int i = 0; i < NP; ++i) p[nt][i] = weight_pair<KIND_, LOG2N>(pair(s[nt], i), turns(nt), a.log2n);
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            p[u][nt][i] = weight_pair<KIND_, LOG2N>(pair(s[u][nt], i), turns(nt), a.log2n);
       }
     }
-    uint32_t pk[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int u = 0; u < kSub; ++u) {
+      uint32_t pk[NT][2];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) l[nt] = add2(l[nt], p[nt][i]);
-      pk[nt][0] = ONE ? pack_pair(p[nt][0].x, 0.f) : pack_pair(p[nt][0].x, p[nt][0].y);
-      pk[nt][1] = ONE ? pack_pair(p[nt][0].y, 0.f) : pack_pair(p[nt][NP - 1].x, p[nt][NP - 1].y);
-    }
-    if (whole) {
-      add_values<false>(a, w, v_at, pk, 0u, 0u, 0);
-      return;
-    }
-    // Slots that a row does not see hold anything: a weight of zero does not hide
-    // an infinity or NaN in a value, so such a group is added token by token with
-    // the values that the token does not see cleared.
-    for (int last = w.lo; last <= w.hi; ++last) {
-      auto keep = [&](int slot) {
-        return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
-               (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
-      };
-      add_values<true>(a, w, v_at, pk, keep(base + 2 * t), keep(base + 2 * t + 8), last);
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) l[nt] = add2(l[nt], p[u][nt][i]);
+        const float2 x = p[u][nt][0], y = p[u][nt][NP - 1];
+        pk[nt][0] = ONE ? pack_pair(x.x, 0.f) : pack_pair(x.x, x.y);
+        pk[nt][1] = ONE ? pack_pair(x.y, 0.f) : pack_pair(y.x, y.y);
+      }
+      const uint32_t vu = v_at + u * 16 * kRowBytes;
+      if (whole) {
+        add_values<false>(a, w, vu, pk, 0u, 0u, 0);
+        continue;
+      }
+      // Slots that a row does not see hold anything: a weight of zero does not hide
+      // an infinity or NaN in a value, so such a group is added token by token with
+      // the values that the token does not see cleared.
+      for (int last = w.lo; last <= w.hi; ++last) {
+        auto keep = [&](int slot) {
+          return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
+                 (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
+        };
+        const int slot = base + u * 16 + 2 * t;
+        add_values<true>(a, w, vu, pk, keep(slot), keep(slot + 8), last);
+      }
     }
   }
   __device__ __forceinline__ void flush(const Item& w, float2* ml, float* dst) {
@@ -539,12 +563,12 @@ struct MmaEngine {
 // ------------------------------------------------------------------ the kernel
 // Decoding reads every key and value once and does little with it, so the kernel
 // is built around the loads. Every warp works for itself: one lane asks TMA for
-// the groups of the warp's share, 16 rows of keys and 16 of values, contiguous in
-// a page, kStages - 1 groups ahead into the warp's ring, across the ends of items;
+// the groups of the warp's share, rows of keys and of values contiguous in a page,
+// kStages - 1 groups ahead into the warp's ring, across the ends of items;
 // the warp takes them from there. (bf16 boxes are swizzled by 128 bytes, so that
 // ldmatrix meets no bank twice.)
 template <typename E>
-constexpr int group_bytes() { return 2 * 16 * E::kRowBytes; }
+constexpr int group_bytes() { return 2 * E::kSlots * E::kRowBytes; }
 template <typename E>
 constexpr int ring_smem() { return 1024 + kWarps * E::kStages * group_bytes<E>(); }
 
@@ -599,27 +623,41 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   int left = (int)min(share, total - start), to_issue = left;
 
   Cursor at(a, pv, s_excl, run, start);
-  auto page_of = [&]() {
-    return to_issue > 0 ? pv.table[(int64_t)at.b * pv.max_pages + (at.span.slot(at.grp) >> pv.page_shift)] : 0;
+  // A group lies in one page, or, with pages of 16 slots and groups of 32, in two.
+  const int boxes = (1 << pv.page_shift) < E::kSlots ? 2 : 1;
+  int2 pid = make_int2(0, 0);
+  auto read_pages = [&]() {
+    if (to_issue <= 0) return;
+    const int slot = at.slot(a), page = slot >> pv.page_shift;
+    const int32_t* table = pv.table + (int64_t)at.b * pv.max_pages;
+    pid.x = table[page];
+    pid.y = boxes == 2 && slot + 16 < at.len ? table[page + 1] : pid.x;
   };
-  int pid = page_of();
-  // One lane fetches. A page that does not exist is replaced by page 0 and its
-  // slots are masked.
+  // One lane fetches. A page that does not exist is replaced by page 0 and the
+  // group's slots are masked; a box beyond the sequence is left out.
   auto issue = [&](int stage) {
     if (to_issue <= 0) return;
-    const bool known = (unsigned)pid < (unsigned)pv.num_pages;
-    const int slot = at.span.slot(at.grp);
+    const bool known = (unsigned)pid.x < (unsigned)pv.num_pages && (unsigned)pid.y < (unsigned)pv.num_pages;
+    const int slot = at.slot(a);
     if (lane == 0) {
       if (!known) atomicOr(a.err, DEV_ERR_BAD_PAGE);
-      const int row = (int)(paged_row(pv, known ? pid : 0, at.h, slot) / kD);
       s_meta[warp][stage] = make_int4(at.item, slot, known ? at.len : 0, 0);
-      sm100::mbar_expect_tx(&full[stage], kBytes);
-      sm100::tma_load_2d(ring + stage * kBytes, &k_map, &full[stage], 0, row);
-      sm100::tma_load_2d(ring + stage * kBytes + kBytes / 2, &v_map, &full[stage], 0, row);
+      const bool second = boxes == 2 && slot + 16 < at.len;
+      sm100::mbar_expect_tx(&full[stage], boxes == 1 || second ? kBytes : kBytes / 2);
+      unsigned char* k = ring + stage * kBytes;
+      const int row = (int)(paged_row(pv, known ? pid.x : 0, at.h, slot) / kD);
+      sm100::tma_load_2d(k, &k_map, &full[stage], 0, row);
+      sm100::tma_load_2d(k + kBytes / 2, &v_map, &full[stage], 0, row);
+      if (second) {
+        const int next = (int)(paged_row(pv, known ? pid.y : 0, at.h, slot + 16) / kD);
+        sm100::tma_load_2d(k + kBytes / 4, &k_map, &full[stage], 0, next);
+        sm100::tma_load_2d(k + 3 * kBytes / 4, &v_map, &full[stage], 0, next);
+      }
     }
     if (--to_issue > 0) at.next(a, pv);
-    pid = page_of();  // read one group further ahead than the copy that needs it
+    read_pages();  // one group further ahead than the copy that needs them
   };
+  read_pages();
   int item = at.item;
   Item w(a, pv, item);
 #pragma unroll
@@ -796,19 +834,18 @@ struct Plan {
 Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool scored, bool wide) {
   Plan p = {};
   p.rows = T * (Hq / Hkv);
-  int ctas;
+  int ctas = 3;
   if (wide) {  // bf16: tiles of up to 32 rows, as even as they come
     const int64_t tiles = (p.rows + 31) / 32;
     p.tile_rows = ((p.rows + tiles - 1) / tiles + 7) / 8 * 8;
-    ctas = p.tile_rows == 8 ? 4 : p.tile_rows == 16 ? 3 : 2;
+    ctas = p.tile_rows <= 16 ? 3 : 2;
   } else {
     p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
-    ctas = 3;
   }
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
   p.items = B * Hkv * p.tiles;
-  // one wave of CTAs, fewer where even the full tables hold less than kMinShare groups a warp
-  const int64_t most = (p.items * ((S + 15) / 16) + kMinShare - 1) / kMinShare;
+  // one wave of CTAs, fewer where even the full tables hold less than kMinSlots a warp
+  const int64_t most = (p.items * ((S + 31) / 32 * 32) + kMinSlots - 1) / kMinSlots;
   p.warps = std::min<int64_t>(kSms * ctas, (most + kWarps - 1) / kWarps) * kWarps;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t parts = (size_t)((p.warps + p.items) * p.tile_rows);
@@ -833,8 +870,9 @@ int attn_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
   const int64_t rows = ((int64_t)pv.num_pages * pv.heads) << pv.page_shift;
   ALGX_REQUIRE(rows <= INT32_MAX, "paged cache too large");
   CUtensorMap k, v;
-  if (int e = make_tmap_2d(&k, a.k, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, 16, E::kSwizzle)) return e;
-  if (int e = make_tmap_2d(&v, a.v, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, 16, E::kSwizzle)) return e;
+  const uint32_t box = std::min(E::kSlots, 1 << pv.page_shift);
+  if (int e = make_tmap_2d(&k, a.k, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
+  if (int e = make_tmap_2d(&v, a.v, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
   kern<<<a.warps / kWarps, kThreads, ring_smem<E>(), st>>>(k, v, a, pv);
   ALGX_LAUNCHED("paged_attn_kernel");
   return ALGX_OK;
@@ -921,6 +959,7 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   a.scale = soft ? cfg->scale * kLog2e : cfg->scale;
   a.inv_unit = soft ? cfg->inv_unit * kLog2e : cfg->inv_unit;
   a.sight = {cfg->window, cfg->first};
+  a.shift = dtype == ALGX_BF16 ? 5 : 4;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == ALGX_BF16)
     return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, st) : paged_launch<__nv_bfloat16, kAsinh>(a, pv, st);

@@ -128,26 +128,26 @@ struct Sight {
   __device__ __forceinline__ bool sees(int s, int last) const {
     return s <= last && (window == 0 || s > last - window || s < first);
   }
-  // Whether every query with lo <= last <= hi sees every slot of s .. s + 15.
-  __device__ __forceinline__ bool sees_group(int s, int lo, int hi) const {
-    return s + 15 <= lo && (window == 0 || s > hi - window || s + 15 < first);
+  // Whether every query with lo <= last <= hi sees every slot of s .. s + n - 1.
+  __device__ __forceinline__ bool sees_all(int s, int n, int lo, int hi) const {
+    return s + n - 1 <= lo && (window == 0 || s > hi - window || s + n - 1 < first);
   }
 };
 
-// The aligned groups of 16 slots that queries with lo <= last <= hi look at: the
-// groups of the first visible slots, then those from the window's left end on.
+// The aligned groups of 2^shift slots that queries with lo <= last <= hi look at:
+// the groups of the first visible slots, then those from the window's left end on.
 struct Span {
   int head_groups;  // groups before the gap
   int skip;         // groups in the gap
   int total;        // groups to visit
-  __device__ __forceinline__ Span(const Sight& w, int lo, int hi) {
-    const int end = max(0, hi + 1);
-    const int groups = (end + 15) >> 4;
+  __device__ __forceinline__ Span(const Sight& w, int shift, int lo, int hi) {
+    const int end = max(0, hi + 1), more = (1 << shift) - 1;
+    const int groups = (end + more) >> shift;
     head_groups = 0;
     skip = 0;
     if (w.window != 0) {
-      const int left = max(0, lo - w.window + 1) >> 4;
-      const int head = (min(w.first, end) + 15) >> 4;
+      const int left = max(0, lo - w.window + 1) >> shift;
+      const int head = (min(w.first, end) + more) >> shift;
       if (head < left) {
         head_groups = head;
         skip = min(left, groups) - head;
@@ -155,7 +155,8 @@ struct Span {
     }
     total = groups - skip;
   }
-  __device__ __forceinline__ int slot(int i) const { return (i < head_groups ? i : i + skip) << 4; }
+  // Number of the i-th group to visit.
+  __device__ __forceinline__ int group(int i) const { return i < head_groups ? i : i + skip; }
 };
 
 }  // namespace algx
