@@ -13,6 +13,11 @@
 // vocabulary of every row, the CTAs exchange the rows' partial sums through
 // distributed shared memory, each decides the (same) accepted count, races over
 // its slice of the one row that counts, and the winners meet in CTA 0.
+//
+// Bound by reading the logits once. The sums use the MUFU forms of the weights
+// (2^-22 relative error an element, averaged by the sum); everything a decision
+// compares - the drafted tokens' probabilities and the race's candidates - is
+// evaluated with correctly rounded roots and divisions or expf.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -28,7 +33,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
-constexpr int kMaxDraft = 32;
+constexpr int kMaxRows = 64;  // 32 target rows, 31 draft rows
+constexpr int kUnroll = 4;    // 16-byte loads of a lane on their way together
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -36,55 +42,97 @@ struct VerifyArgs {
   const float *u, *race;
   int32_t *out, *accepted;
   int* err;
-  int64_t V, slice;  // slice: vocabulary columns of one CTA, a multiple of 8
+  int64_t V, slice;  // slice: vocabulary columns of one CTA
   int K, log2n;
-  float scale;  // log2(e) / temperature (ce) or 1 / c (alg_ce)
+  float scale;  // 1 / temperature (ce) or 1 / c (alg_ce)
 };
 
-// Running reference and sum of one lane over one row's elements.
+// The score of a logit: the logit itself for ce, so that differences from the
+// maximum are exact, z / c for alg_ce. NaN counts as -inf.
 template <int KIND>
+__device__ __forceinline__ float score_of(const VerifyArgs& a, float z) {
+  z = fmaxf(z, kNegInf);
+  return KIND == kSoftmax ? z : z * a.scale;
+}
+template <int KIND>
+__device__ __forceinline__ float exact_weight(const VerifyArgs& a, float x, float turn) {
+  if constexpr (KIND == kSoftmax) return expf((x - turn) * a.scale);
+  else return weight_of<kAsinh, true>(x, turn, a.log2n);
+}
+template <int KIND, int LOG2N>
+__device__ __forceinline__ float2 fast_weights(const VerifyArgs& a, float2 x, float2 turn) {
+  if constexpr (KIND == kSoftmax) {
+    const float k = a.scale * kLog2e;
+    return weight_pair<kSoftmax, 0>(mul2(sub2(x, turn), make_float2(k, k)), make_float2(0.f, 0.f), 0);
+  } else {
+    return weight_pair<kAsinh, LOG2N>(x, turn, a.log2n);
+  }
+}
+
+// Running reference (a score) and sum of weights of one lane.
+template <int KIND, int LOG2N>
 struct RowSum {
-  float m = kNegInf, turn = 0.f, l = 0.f;
-  __device__ __forceinline__ void add(float x, int log2n) {
-    if (!(x > kNegInf)) return;  // -inf and NaN logits have no probability
-    if (x > m) {
-      const float t = weight_turn<KIND, true>(x);
-      l = m == kNegInf ? 0.f : l * weight_of<KIND, true>(m, t, log2n);
-      m = x;
+  float m, turn;
+  float2 l;
+  __device__ __forceinline__ void clear() {
+    m = kNegInf;
+    turn = weight_turn<KIND, true>(kNegInf);
+    l = make_float2(0.f, 0.f);
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const VerifyArgs& a, const float (&z)[N]) {
+    float x[N], top = kNegInf;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] = score_of<KIND>(a, z[i]);
+      top = fmaxf(top, x[i]);
+    }
+    if (top > m) {
+      const float t = weight_turn<KIND, true>(top);
+      const float f = m == kNegInf ? 0.f : exact_weight<KIND>(a, m, t);
+      l.x *= f;
+      l.y *= f;
+      m = top;
       turn = t;
     }
-    l += weight_of<KIND, true>(x, turn, log2n);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 w = fast_weights<KIND, LOG2N>(a, make_float2(x[i], i + 1 < N ? x[i + 1] : kNegInf),
+                                                 make_float2(turn, turn));
+      l = add2(l, w);
+    }
   }
 };
-
-// f(column, value) over the columns [begin, end) of a row, 16-byte loads on the
-// aligned middle, spread over `lanes` threads.
-template <typename T, typename F>
-__device__ __forceinline__ void for_columns(const T* row, int64_t begin, int64_t end, int me, int lanes, F f) {
-  using V = Vec<T>;
-  const uintptr_t addr = reinterpret_cast<uintptr_t>(row + begin);
-  int64_t head = (int64_t)(((16 - (addr & 15)) & 15) / sizeof(T));
-  if (head > end - begin) head = end - begin;
-  for (int64_t v = begin + me; v < begin + head; v += lanes) f(v, to_f32(row[v]));
-  const int64_t mid = begin + head, vecs = (end - mid) / V::N;
-#pragma unroll 4
-  for (int64_t i = me; i < vecs; i += lanes) {
-    float x[V::N];
-    unpack<T>(*reinterpret_cast<const uint4*>(row + mid + i * V::N), x);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) f(mid + i * V::N + j, x[j]);
-  }
-  for (int64_t v = mid + vecs * V::N + me; v < end; v += lanes) f(v, to_f32(row[v]));
-}
 
 __device__ __forceinline__ uint64_t pack_best(float value, int64_t v) {
   return ((uint64_t)__float_as_uint(value) << 32) | (uint32_t)~(uint32_t)v;
 }
 
-template <typename T, int KIND>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ float2 s_part[2 * kMaxDraft + 1];  // this CTA's (reference, sum) of every row
-  __shared__ float s_m[2 * kMaxDraft + 1], s_l[2 * kMaxDraft + 1];
+// Columns [begin, end) of a row in blocks of kUnroll 16-byte vectors a lane: the
+// aligned middle, and up to 2 (N - 1) single columns at the ends, which go with
+// the first block.
+template <typename T>
+struct Columns {
+  static constexpr int N = Vec<T>::N, kBlock = 32 * kUnroll;  // vectors of a block
+  const T* row;
+  int64_t begin, end, mid, vecs;
+  __device__ __forceinline__ Columns(const T* r, int64_t b, int64_t e) : row(r), begin(b), end(e) {
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(r + b);
+    mid = min(e, b + (int64_t)(((16 - (addr & 15)) & 15) / sizeof(T)));
+    vecs = (e - mid) / N;
+  }
+  __device__ __forceinline__ int ends() const { return (int)((mid - begin) + (end - mid - vecs * N)); }
+  __device__ __forceinline__ int64_t end_column(int i) const {
+    return i < mid - begin ? begin + i : mid + vecs * N + (i - (mid - begin));
+  }
+};
+
+template <typename T, int KIND, int LOG2N>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs a) {
+  using V = Vec<T>;
+  __shared__ float2 s_part[kWarps + kMaxRows];  // (reference, sum) of every (warp, row) that meets, at warp + row
+  __shared__ float2 s_row[kMaxRows];            // this CTA's (reference, sum) of every row
+  __shared__ float s_turn[kMaxRows], s_l[kMaxRows];
   __shared__ uint64_t s_best[kWarps];
   __shared__ uint64_t s_cta_best;
   __shared__ int s_accepted;
@@ -92,90 +140,180 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
   const int rank = (int)cluster.block_rank();
   const int64_t b = blockIdx.x / kCluster;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
   const int K = a.counts ? min(max(a.counts[b], 0), a.K) : a.K;
   const bool has_draft = a.draft != nullptr;
   const int rows = K + 1 + (has_draft ? K : 0);
   const int64_t begin = min(a.V, rank * a.slice), end = min(a.V, begin + a.slice);
   const T* target = static_cast<const T*>(a.target) + b * (a.K + 1) * a.V;
   const T* draft = static_cast<const T*>(a.draft) + b * a.K * a.V;
+  const float* race = a.race + b * a.V;
   auto row_of = [&](int r) { return r <= K ? target + (int64_t)r * a.V : draft + (int64_t)(r - K - 1) * a.V; };
+  // what the decision will need, asked for early: the drafted tokens, their
+  // logits, and (into L2) the race's variates
+  float u = 0.f, zp = 0.f, zq = 0.f;
+  bool valid = false;
+  if (warp == 0 && lane < K) {
+    const int32_t x = a.tokens[b * a.K + lane];
+    valid = x >= 0 && x < a.V;
+    if (!valid && rank == 0) atomicOr(a.err, DEV_ERR_BAD_LABEL);
+    u = a.u[b * a.K + lane];
+    if (valid) {
+      zp = to_f32(target[(int64_t)lane * a.V + x]);
+      if (has_draft) zq = to_f32(draft[(int64_t)lane * a.V + x]);
+    }
+  }
+  for (int64_t v = begin + threadIdx.x * 32; v < end; v += kThreads * 32)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(race + v));
 
-  for (int r = warp; r < rows; r += kWarps) {
-    RowSum<KIND> sum;
-    for_columns(row_of(r), begin, end, lane, 32, [&](int64_t, float z) { sum.add(z * a.scale, a.log2n); });
+  // The blocks of all rows stand in one line, cut into equal shares of the warps.
+  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Columns<T>::kBlock - 1) / (V::N * Columns<T>::kBlock));
+  const int share = (rows * blocks + kWarps - 1) / kWarps;
+  int at = warp * share;
+  const int stop = min(rows * blocks, at + share);
+  while (at < stop) {
+    const int r = at / blocks;
+    const Columns<T> c(row_of(r), begin, end);
+    const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
+    RowSum<KIND, LOG2N> sum;
+    sum.clear();
+    if (at == r * blocks && lane < c.ends()) {
+      const float z[1] = {to_f32(c.row[c.end_column(lane)])};
+      sum.add(a, z);
+    }
+    for (; at < stop && at < (r + 1) * blocks; ++at) {
+      const int64_t v0 = (int64_t)(at - r * blocks) * Columns<T>::kBlock + lane;
+      uint4 raw[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i)
+        if (v0 + i * 32 < c.vecs) raw[i] = __ldg(mid + v0 + i * 32);
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i)
+        if (v0 + i * 32 < c.vecs) {
+          float z[V::N];
+          unpack<T>(raw[i], z);
+          sum.add(a, z);
+        }
+    }
     float M = sum.m;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    float L = sum.m == kNegInf ? 0.f : sum.l * weight_of<KIND, true>(sum.m, weight_turn<KIND, true>(M), a.log2n);
+    float L = sum.m == kNegInf ? 0.f : (sum.l.x + sum.l.y) * exact_weight<KIND>(a, sum.m, weight_turn<KIND, true>(M));
     L = row_sum<32>(L);
-    if (lane == 0) s_part[r] = make_float2(M, L);
+    if (lane == 0) s_part[warp + r] = make_float2(M, L);
+  }
+  __syncthreads();
+  // joins parts one by one; each has a reference and a sum
+  auto join = [&](int count, auto part) {
+    float M = kNegInf, L = 0.f;
+    for (int i = 0; i < count; ++i) M = fmaxf(M, part(i).x);
+    const float turn = weight_turn<KIND, true>(M);
+    for (int i = 0; i < count; ++i) {
+      const float2 p = part(i);
+      if (p.x != kNegInf) L = fmaf(p.y, exact_weight<KIND>(a, p.x, turn), L);
+    }
+    return make_float2(M, L);
+  };
+  if (threadIdx.x < rows) {
+    const int r = threadIdx.x, lo = r * blocks / share, hi = ((r + 1) * blocks - 1) / share;
+    s_row[r] = join(hi - lo + 1, [&](int i) { return s_part[lo + i + r]; });
   }
   cluster.sync();
-  for (int r = threadIdx.x; r < rows; r += kThreads) {
+  if (threadIdx.x < rows) {
+    const int r = threadIdx.x;
     float2 part[kCluster];
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c) part[c] = *cluster.map_shared_rank(&s_row[r], c);
     float M = kNegInf, L = 0.f;
 #pragma unroll
-    for (int c = 0; c < kCluster; ++c) {
-      part[c] = *cluster.map_shared_rank(&s_part[r], c);
-      M = fmaxf(M, part[c].x);
-    }
+    for (int c = 0; c < kCluster; ++c) M = fmaxf(M, part[c].x);
     const float turn = weight_turn<KIND, true>(M);
 #pragma unroll
     for (int c = 0; c < kCluster; ++c)
-      if (part[c].x != kNegInf) L = fmaf(part[c].y, weight_of<KIND, true>(part[c].x, turn, a.log2n), L);
-    s_m[r] = turn;
+      if (part[c].x != kNegInf) L = fmaf(part[c].y, exact_weight<KIND>(a, part[c].x, turn), L);
+    s_turn[r] = turn;
     s_l[r] = L > 0.f ? L : 1.f;
   }
   __syncthreads();
   auto prob = [&](int r, float z) {
-    const float x = z * a.scale;
-    return x > kNegInf ? weight_of<KIND, true>(x, s_m[r], a.log2n) / s_l[r] : 0.f;
+    const float x = score_of<KIND>(a, z);
+    return x > kNegInf ? exact_weight<KIND>(a, x, s_turn[r]) / s_l[r] : 0.f;
   };
   if (warp == 0) {
     bool refused = false;
-    if (lane < K) {
-      const int32_t x = a.tokens[b * a.K + lane];
-      if (x < 0 || x >= a.V) {
-        refused = true;
-        if (rank == 0) atomicOr(a.err, DEV_ERR_BAD_LABEL);
-      } else {
-        const float p = prob(lane, to_f32(target[(int64_t)lane * a.V + x]));
-        const float q = has_draft ? prob(K + 1 + lane, to_f32(draft[(int64_t)lane * a.V + x])) : 1.f;
-        refused = !(a.u[b * a.K + lane] * q < p);
-      }
-    }
+    if (lane < K) refused = !valid || !(u * (has_draft ? prob(K + 1 + lane, zq) : 1.f) < prob(lane, zp));
     const unsigned mask = __ballot_sync(0xffffffffu, refused);
     if (lane == 0) s_accepted = mask ? __ffs(mask) - 1 : K;
   }
   __syncthreads();
   const int acc = s_accepted;
-  const float* race = a.race + b * a.V;
-  const T* zp = target + (int64_t)acc * a.V;
-  const T* zq = has_draft && acc < K ? draft + (int64_t)acc * a.V : nullptr;
+  const T* row_p = target + (int64_t)acc * a.V;
+  const T* row_q = has_draft && acc < K ? draft + (int64_t)acc * a.V : nullptr;
   const int64_t drafted = !has_draft && acc < K ? a.tokens[b * a.K + acc] : -1;
+  const float turn_p = s_turn[acc], l_p = s_l[acc];
+  const float turn_q = row_q ? s_turn[K + 1 + acc] : 0.f, l_q = row_q ? s_l[K + 1 + acc] : 1.f;
+  const float inv_p = 1.f / l_p, inv_q = 1.f / l_q;
   // pass 0 races over the residual; where nothing of it is left, pass 1 over p
   for (int pass = acc < K ? 0 : 1; pass < 2; ++pass) {
-    uint64_t best = 0;
-    for_columns(zp, begin, end, threadIdx.x, kThreads, [&](int64_t v, float z) {
-      float w = prob(acc, z);
-      if (pass == 0) {
-        const float q = zq ? prob(K + 1 + acc, to_f32(zq[v])) : v == drafted ? 1.f : 0.f;
-        w = fmaxf(w - q, 0.f);
+    float best = 0.f;
+    uint64_t best_at = pack_best(0.f, begin + threadIdx.x);
+    // A column is evaluated exactly only where its fast value could win: the fast
+    // weights err by less than 2^-16 of themselves (2^-22 a factor, 32 factors).
+    auto enter = [&](int64_t v, float z, float zd, float e) {
+      const float xp = score_of<KIND>(a, z), xq = score_of<KIND>(a, zd);
+      const float2 f = fast_weights<KIND, LOG2N>(a, make_float2(xp, xq), make_float2(turn_p, turn_q));
+      const bool rest = pass == 0;
+      const float p = f.x * inv_p, q = !rest ? 0.f : row_q ? f.y * inv_q : v == drafted ? 1.f : 0.f;
+      const float most = (p - q) + (p + q) * 0x1p-16f;
+      if (!(most > 0.f) || !(most * 1.001f >= best * e)) return;
+      float w = xp > kNegInf ? exact_weight<KIND>(a, xp, turn_p) / l_p : 0.f;
+      if (rest) w -= row_q ? (xq > kNegInf ? exact_weight<KIND>(a, xq, turn_q) / l_q : 0.f) : q;
+      const float ratio = w > 0.f ? w / e : 0.f;
+      if (!(ratio > 0.f)) return;
+      const uint64_t here = pack_best(ratio, v);
+      if (here > best_at) {
+        best_at = here;
+        best = ratio;
       }
-      const float ratio = w > 0.f ? w / race[v] : 0.f;
-      const uint64_t at = pack_best(ratio > 0.f ? ratio : 0.f, v);
-      best = best > at ? best : at;
-    });
+    };
+    const bool rest = pass == 0 && row_q;
+    const Columns<T> c(row_p, begin, end);
+    if (threadIdx.x < c.ends()) {
+      const int64_t v = c.end_column(threadIdx.x);
+      enter(v, to_f32(row_p[v]), rest ? to_f32(row_q[v]) : kNegInf, race[v]);
+    }
+    // the three rows need not be aligned alike: vectors where they are
+    const bool vec = ((reinterpret_cast<uintptr_t>(race + c.mid) & 15) == 0) &&
+                     (!rest || (reinterpret_cast<uintptr_t>(row_q + c.mid) & 15) == 0);
+    if (vec) {
+#pragma unroll 2
+      for (int64_t i = threadIdx.x; i < c.vecs; i += kThreads) {
+        const int64_t v = c.mid + i * V::N;
+        float z[V::N], zd[V::N], e[V::N];
+        unpack<T>(__ldg(reinterpret_cast<const uint4*>(row_p + v)), z);
+        if (rest) unpack<T>(__ldg(reinterpret_cast<const uint4*>(row_q + v)), zd);
+#pragma unroll
+        for (int j = 0; j < V::N; j += 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(race + v + j));
+          e[j] = x.x; e[j + 1] = x.y; e[j + 2] = x.z; e[j + 3] = x.w;
+        }
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) enter(v + j, z[j], rest ? zd[j] : kNegInf, e[j]);
+      }
+    } else {
+      for (int64_t v = c.mid + threadIdx.x; v < c.mid + c.vecs * V::N; v += kThreads)
+        enter(v, to_f32(row_p[v]), rest ? to_f32(row_q[v]) : kNegInf, race[v]);
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, best, off);
-      best = best > o ? best : o;
+      const uint64_t o = __shfl_xor_sync(0xffffffffu, best_at, off);
+      best_at = best_at > o ? best_at : o;
     }
-    if (lane == 0) s_best[warp] = best;
+    if (lane == 0) s_best[warp] = best_at;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int i = 1; i < kWarps; ++i) best = best > s_best[i] ? best : s_best[i];
-      s_cta_best = best;
+      for (int i = 1; i < kWarps; ++i) best_at = best_at > s_best[i] ? best_at : s_best[i];
+      s_cta_best = best_at;
     }
     cluster.sync();
     uint64_t all = 0;
@@ -185,11 +323,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
       all = all > o ? all : o;
     }
     const bool empty = (all >> 32) == 0;
-    if (rank == 0 && threadIdx.x == 0 && (pass == 1 || !empty)) {
-      for (int i = 0; i <= a.K; ++i)
-        a.out[b * (a.K + 1) + i] =
-            i < acc ? a.tokens[b * a.K + i] : i == acc ? (int32_t)~(uint32_t)all : -1;
-      a.accepted[b] = acc;
+    if (rank == 0 && (int)threadIdx.x <= a.K && (pass == 1 || !empty)) {
+      const int i = threadIdx.x;
+      a.out[b * (a.K + 1) + i] = i < acc ? a.tokens[b * a.K + i] : i == acc ? (int32_t)~(uint32_t)all : -1;
+      if (i == 0) a.accepted[b] = acc;
     }
     cluster.sync();  // nobody leaves, or writes its best again, while others read it
     if (!empty) break;
@@ -217,16 +354,21 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   VerifyArgs a = {};
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
   a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;
-  a.scale = kind == ALGX_HEAD_CE ? scale * kLog2e : scale;
+  a.scale = scale;
   a.slice = ((V + kCluster - 1) / kCluster + 7) / 8 * 8;
   while ((1 << a.log2n) < n) ++a.log2n;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  auto* kern = dtype == ALGX_BF16 ? (kind == ALGX_HEAD_CE ? verify_kernel<__nv_bfloat16, kSoftmax>
-                                                          : verify_kernel<__nv_bfloat16, kAsinh>)
-                                  : (kind == ALGX_HEAD_CE ? verify_kernel<float, kSoftmax>
-                                                          : verify_kernel<float, kAsinh>);
-  kern<<<(unsigned)(B * kCluster), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  using bf16 = __nv_bfloat16;
+  void (*kern)(VerifyArgs);
+  if (kind == ALGX_HEAD_CE)
+    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kSoftmax, 0> : verify_kernel<float, kSoftmax, 0>;
+  else if (a.log2n == 3)
+    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kAsinh, 3> : verify_kernel<float, kAsinh, 3>;
+  else
+    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kAsinh, 0> : verify_kernel<float, kAsinh, 0>;
+  ALGX_CUDA(launch_dependent(kern, dim3((unsigned)(B * kCluster)), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
+                             a));
   ALGX_LAUNCHED("verify_kernel");
   return ALGX_OK;
 }
