@@ -30,10 +30,8 @@ namespace cg = cooperative_groups;
 namespace algx {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
-constexpr int kMaxRows = 64;  // 32 target rows, 31 draft rows
+constexpr int kMaxRows = 64;  // of one round: 32 target rows, 31 draft rows
 constexpr int kUnroll = 4;    // 16-byte loads of a lane on their way together
 
 struct VerifyArgs {
@@ -44,6 +42,7 @@ struct VerifyArgs {
   int* err;
   int64_t V, slice;  // slice: vocabulary columns of one CTA
   int K, log2n;
+  int round;  // draft positions looked at in one round
   float scale;  // 1 / temperature (ce) or 1 / c (alg_ce)
 };
 
@@ -59,6 +58,11 @@ __device__ __forceinline__ float exact_weight(const VerifyArgs& a, float x, floa
   if constexpr (KIND == kSoftmax) return expf((x - turn) * a.scale);
   else return weight_of<kAsinh, true>(x, turn, a.log2n);
 }
+template <int KIND>
+__device__ __forceinline__ float fast_weight(const VerifyArgs& a, float x, float turn) {
+  if constexpr (KIND == kSoftmax) return weight_of<kSoftmax, false>((x - turn) * (a.scale * kLog2e), 0.f, 0);
+  else return weight_of<kAsinh, false>(x, turn, a.log2n);
+}
 template <int KIND, int LOG2N>
 __device__ __forceinline__ float2 fast_weights(const VerifyArgs& a, float2 x, float2 turn) {
   if constexpr (KIND == kSoftmax) {
@@ -69,7 +73,11 @@ __device__ __forceinline__ float2 fast_weights(const VerifyArgs& a, float2 x, fl
   }
 }
 
-// Running reference (a score) and sum of weights of one lane.
+// Running reference (a score) and sum of weights of one lane. The reference is
+// the first vector's maximum until a weight passes 2^60 of it; smaller moves
+// would cost a warp a rescaling at nearly every vector, for some lane of it.
+constexpr float kFar = 0x1p60f;
+
 template <int KIND, int LOG2N>
 struct RowSum {
   float m, turn;
@@ -81,26 +89,29 @@ struct RowSum {
   }
   template <int N>
   __device__ __forceinline__ void add(const VerifyArgs& a, const float (&z)[N]) {
-    float x[N], top = kNegInf;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = score_of<KIND>(a, z[i]);
-      top = fmaxf(top, x[i]);
-    }
-    if (top > m) {
-      const float t = weight_turn<KIND, true>(top);
-      const float f = m == kNegInf ? 0.f : exact_weight<KIND>(a, m, t);
-      l.x *= f;
-      l.y *= f;
-      m = top;
-      turn = t;
-    }
+    float2 x[(N + 1) / 2], w[(N + 1) / 2];
+    float high = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const float2 w = fast_weights<KIND, LOG2N>(a, make_float2(x[i], i + 1 < N ? x[i + 1] : kNegInf),
-                                                 make_float2(turn, turn));
-      l = add2(l, w);
+      x[i / 2] = make_float2(fmaxf(z[i], kNegInf), i + 1 < N ? fmaxf(z[i + 1], kNegInf) : kNegInf);
+      if (KIND == kAsinh) x[i / 2] = mul2(x[i / 2], make_float2(a.scale, a.scale));
+      w[i / 2] = fast_weights<KIND, LOG2N>(a, x[i / 2], make_float2(turn, turn));
+      high = fmaxf(high, fmaxf(w[i / 2].x, w[i / 2].y));
     }
+    if (high > kFar) {
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < (N + 1) / 2; ++i) top = fmaxf(top, fmaxf(x[i].x, x[i].y));
+      const float to = weight_turn<KIND, true>(top);
+      const float f = m == kNegInf ? 0.f : exact_weight<KIND>(a, m, to);
+      l = mul2(l, make_float2(f, f));
+      m = top;
+      turn = to;
+#pragma unroll
+      for (int i = 0; i < (N + 1) / 2; ++i) w[i] = fast_weights<KIND, LOG2N>(a, x[i], make_float2(turn, turn));
+    }
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) l = add2(l, w[i]);
   }
 };
 
@@ -127,11 +138,13 @@ struct Columns {
   }
 };
 
-template <typename T, int KIND, int LOG2N>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs a) {
+template <typename T, int KIND, int LOG2N, int kThreads>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1024 / kThreads)
+    verify_kernel(const VerifyArgs a) {
   using V = Vec<T>;
+  constexpr int kWarps = kThreads / 32;
   __shared__ float2 s_part[kWarps + kMaxRows];  // (reference, sum) of every (warp, row) that meets, at warp + row
-  __shared__ float2 s_row[kMaxRows];            // this CTA's (reference, sum) of every row
+  __shared__ float2 s_row[2][kMaxRows];         // this CTA's (reference, sum) of every row, for two rounds
   __shared__ float s_turn[kMaxRows], s_l[kMaxRows];
   __shared__ uint64_t s_best[kWarps];
   __shared__ uint64_t s_cta_best;
@@ -143,12 +156,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
   pdl_wait();
   const int K = a.counts ? min(max(a.counts[b], 0), a.K) : a.K;
   const bool has_draft = a.draft != nullptr;
-  const int rows = K + 1 + (has_draft ? K : 0);
   const int64_t begin = min(a.V, rank * a.slice), end = min(a.V, begin + a.slice);
   const T* target = static_cast<const T*>(a.target) + b * (a.K + 1) * a.V;
   const T* draft = static_cast<const T*>(a.draft) + b * a.K * a.V;
   const float* race = a.race + b * a.V;
-  auto row_of = [&](int r) { return r <= K ? target + (int64_t)r * a.V : draft + (int64_t)(r - K - 1) * a.V; };
   // what the decision will need, asked for early: the drafted tokens, their
   // logits, and (into L2) the race's variates
   float u = 0.f, zp = 0.f, zq = 0.f;
@@ -166,43 +177,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
   for (int64_t v = begin + threadIdx.x * 32; v < end; v += kThreads * 32)
     asm volatile("prefetch.global.L2 [%0];" ::"l"(race + v));
 
-  // The blocks of all rows stand in one line, cut into equal shares of the warps.
-  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Columns<T>::kBlock - 1) / (V::N * Columns<T>::kBlock));
-  const int share = (rows * blocks + kWarps - 1) / kWarps;
-  int at = warp * share;
-  const int stop = min(rows * blocks, at + share);
-  while (at < stop) {
-    const int r = at / blocks;
-    const Columns<T> c(row_of(r), begin, end);
-    const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
-    RowSum<KIND, LOG2N> sum;
-    sum.clear();
-    if (at == r * blocks && lane < c.ends()) {
-      const float z[1] = {to_f32(c.row[c.end_column(lane)])};
-      sum.add(a, z);
-    }
-    for (; at < stop && at < (r + 1) * blocks; ++at) {
-      const int64_t v0 = (int64_t)(at - r * blocks) * Columns<T>::kBlock + lane;
-      uint4 raw[kUnroll];
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
-        if (v0 + i * 32 < c.vecs) raw[i] = __ldg(mid + v0 + i * 32);
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
-        if (v0 + i * 32 < c.vecs) {
-          float z[V::N];
-          unpack<T>(raw[i], z);
-          sum.add(a, z);
-        }
-    }
-    float M = sum.m;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    float L = sum.m == kNegInf ? 0.f : (sum.l.x + sum.l.y) * exact_weight<KIND>(a, sum.m, weight_turn<KIND, true>(M));
-    L = row_sum<32>(L);
-    if (lane == 0) s_part[warp + r] = make_float2(M, L);
-  }
-  __syncthreads();
   // joins parts one by one; each has a reference and a sum
   auto join = [&](int count, auto part) {
     float M = kNegInf, L = 0.f;
@@ -210,70 +184,131 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     const float turn = weight_turn<KIND, true>(M);
     for (int i = 0; i < count; ++i) {
       const float2 p = part(i);
-      if (p.x != kNegInf) L = fmaf(p.y, exact_weight<KIND>(a, p.x, turn), L);
+      if (p.x != kNegInf) L = fmaf(p.y, fast_weight<KIND>(a, p.x, turn), L);
     }
     return make_float2(M, L);
   };
-  if (threadIdx.x < rows) {
-    const int r = threadIdx.x, lo = r * blocks / share, hi = ((r + 1) * blocks - 1) / share;
-    s_row[r] = join(hi - lo + 1, [&](int i) { return s_part[lo + i + r]; });
-  }
-  cluster.sync();
-  if (threadIdx.x < rows) {
-    const int r = threadIdx.x;
-    float2 part[kCluster];
-#pragma unroll
-    for (int c = 0; c < kCluster; ++c) part[c] = *cluster.map_shared_rank(&s_row[r], c);
-    float M = kNegInf, L = 0.f;
-#pragma unroll
-    for (int c = 0; c < kCluster; ++c) M = fmaxf(M, part[c].x);
-    const float turn = weight_turn<KIND, true>(M);
-#pragma unroll
-    for (int c = 0; c < kCluster; ++c)
-      if (part[c].x != kNegInf) L = fmaf(part[c].y, exact_weight<KIND>(a, part[c].x, turn), L);
-    s_turn[r] = turn;
-    s_l[r] = L > 0.f ? L : 1.f;
-  }
-  __syncthreads();
   auto prob = [&](int r, float z) {
     const float x = score_of<KIND>(a, z);
     return x > kNegInf ? exact_weight<KIND>(a, x, s_turn[r]) / s_l[r] : 0.f;
   };
-  if (warp == 0) {
-    bool refused = false;
-    if (lane < K) refused = !valid || !(u * (has_draft ? prob(K + 1 + lane, zq) : 1.f) < prob(lane, zp));
-    const unsigned mask = __ballot_sync(0xffffffffu, refused);
-    if (lane == 0) s_accepted = mask ? __ffs(mask) - 1 : K;
+  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Columns<T>::kBlock - 1) / (V::N * Columns<T>::kBlock));
+
+  // Rounds of a.round positions, up to the first refusal: rows after it are not
+  // needed. Row r of a round is target row i0 + r, then draft row i0 + (r - nt).
+  int acc = -1, i0 = 0, nt = 0;
+  for (int turn_no = 0; acc < 0; ++turn_no) {
+    i0 = turn_no * a.round;
+    nt = min(K + 1 - i0, a.round);
+    const int nd = min(K - i0, a.round), rows = nt + (has_draft ? nd : 0);
+    float2* const s_mine = s_row[turn_no & 1];
+    // the blocks of the round's rows stand in one line, cut into equal shares of the warps
+    const int share = (rows * blocks + kWarps - 1) / kWarps;
+    int at = warp * share;
+    const int stop = min(rows * blocks, at + share);
+    while (at < stop) {
+      const int r = at / blocks;
+      const Columns<T> c(r < nt ? target + (int64_t)(i0 + r) * a.V : draft + (int64_t)(i0 + r - nt) * a.V, begin, end);
+      const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
+      const int vecs = (int)c.vecs;
+      RowSum<KIND, LOG2N> sum;
+      sum.clear();
+      if (at == r * blocks && lane < c.ends()) {
+        const float z[1] = {to_f32(c.row[c.end_column(lane)])};
+        sum.add(a, z);
+      }
+      for (; at < stop && at < (r + 1) * blocks; ++at) {
+        const int v0 = (at - r * blocks) * Columns<T>::kBlock + lane;
+        uint4 raw[kUnroll];
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i)
+          if (v0 + i * 32 < vecs) raw[i] = __ldg(mid + v0 + i * 32);
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i)
+          if (v0 + i * 32 < vecs) {
+            float z[V::N];
+            unpack<T>(raw[i], z);
+            sum.add(a, z);
+          }
+      }
+      float M = sum.m;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+      float L = sum.m == kNegInf ? 0.f : (sum.l.x + sum.l.y) * fast_weight<KIND>(a, sum.m, weight_turn<KIND, true>(M));
+      L = row_sum<32>(L);
+      if (lane == 0) s_part[warp + r] = make_float2(M, L);
+    }
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      const int r = threadIdx.x, lo = r * blocks / share, hi = ((r + 1) * blocks - 1) / share;
+      s_mine[r] = join(hi - lo + 1, [&](int i) { return s_part[lo + i + r]; });
+    }
+    cluster.sync();
+    if (threadIdx.x < rows) {
+      const int r = threadIdx.x;
+      float2 part[kCluster];
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) part[c] = *cluster.map_shared_rank(&s_mine[r], c);
+      float M = kNegInf, L = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) M = fmaxf(M, part[c].x);
+      const float turn = weight_turn<KIND, true>(M);
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c)
+        if (part[c].x != kNegInf) L = fmaf(part[c].y, fast_weight<KIND>(a, part[c].x, turn), L);
+      s_turn[r] = turn;
+      s_l[r] = L > 0.f ? L : 1.f;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      bool refused = false;
+      const int i = lane - i0;  // this lane's draft in the round
+      if (i >= 0 && i < nd) refused = !valid || !(u * (has_draft ? prob(nt + i, zq) : 1.f) < prob(i, zp));
+      const unsigned mask = __ballot_sync(0xffffffffu, refused);
+      if (lane == 0) s_accepted = mask ? __ffs(mask) - 1 : i0 + nt > K ? K : -1;
+    }
+    __syncthreads();
+    acc = s_accepted;
   }
-  __syncthreads();
-  const int acc = s_accepted;
   const T* row_p = target + (int64_t)acc * a.V;
   const T* row_q = has_draft && acc < K ? draft + (int64_t)acc * a.V : nullptr;
   const int64_t drafted = !has_draft && acc < K ? a.tokens[b * a.K + acc] : -1;
-  const float turn_p = s_turn[acc], l_p = s_l[acc];
-  const float turn_q = row_q ? s_turn[K + 1 + acc] : 0.f, l_q = row_q ? s_l[K + 1 + acc] : 1.f;
+  const int rp = acc - i0, rq = nt + acc - i0;  // their rows in the last round
+  const float turn_p = s_turn[rp], l_p = s_l[rp];
+  const float turn_q = row_q ? s_turn[rq] : 0.f, l_q = row_q ? s_l[rq] : 1.f;
   const float inv_p = 1.f / l_p, inv_q = 1.f / l_q;
+  // weight / variate of one column, as the result is compared
+  auto exact_ratio = [&](bool rest, int64_t v, float xp, float xq, float e) {
+    float w = xp > kNegInf ? exact_weight<KIND>(a, xp, turn_p) / l_p : 0.f;
+    if (rest) w -= row_q ? (xq > kNegInf ? exact_weight<KIND>(a, xq, turn_q) / l_q : 0.f) : v == drafted ? 1.f : 0.f;
+    const float ratio = w > 0.f ? w / e : 0.f;
+    return ratio > 0.f ? ratio : 0.f;
+  };
   // pass 0 races over the residual; where nothing of it is left, pass 1 over p
   for (int pass = acc < K ? 0 : 1; pass < 2; ++pass) {
-    float best = 0.f;
-    uint64_t best_at = pack_best(0.f, begin + threadIdx.x);
-    // A column is evaluated exactly only where its fast value could win: the fast
-    // weights err by less than 2^-16 of themselves (2^-22 a factor, 32 factors).
+    // The fast weights err by less than 2^-16 of themselves (2^-22 a factor, 32
+    // factors), which bounds every ratio from both sides. A lane keeps the column
+    // that no other can be above; only where two overlap are they evaluated
+    // exactly, and at the end the lanes that could hold the winner.
+    float low = 0.f, up = 0.f, xp_b = kNegInf, xq_b = kNegInf, e_b = 1.f;
+    int64_t v_b = min(begin + threadIdx.x, a.V - 1);
     auto enter = [&](int64_t v, float z, float zd, float e) {
       const float xp = score_of<KIND>(a, z), xq = score_of<KIND>(a, zd);
       const float2 f = fast_weights<KIND, LOG2N>(a, make_float2(xp, xq), make_float2(turn_p, turn_q));
-      const bool rest = pass == 0;
-      const float p = f.x * inv_p, q = !rest ? 0.f : row_q ? f.y * inv_q : v == drafted ? 1.f : 0.f;
-      const float most = (p - q) + (p + q) * 0x1p-16f;
-      if (!(most > 0.f) || !(most * 1.001f >= best * e)) return;
-      float w = xp > kNegInf ? exact_weight<KIND>(a, xp, turn_p) / l_p : 0.f;
-      if (rest) w -= row_q ? (xq > kNegInf ? exact_weight<KIND>(a, xq, turn_q) / l_q : 0.f) : q;
-      const float ratio = w > 0.f ? w / e : 0.f;
-      if (!(ratio > 0.f)) return;
-      const uint64_t here = pack_best(ratio, v);
-      if (here > best_at) {
-        best_at = here;
-        best = ratio;
+      const float p = f.x * inv_p, q = pass == 1 ? 0.f : row_q ? f.y * inv_q : v == drafted ? 1.f : 0.f;
+      const float r = rcp_fast(e), mid = (p - q) * r, off = (p + q) * r * 0x1p-16f;
+      if (!(mid + off > low) || !(mid + off > 0.f)) return;
+      bool take = mid - off > up;
+      float lo = mid - off, hi = mid + off;
+      if (!take) {
+        const float mine = exact_ratio(pass == 0, v, xp, xq, e);
+        const float held = up > 0.f ? exact_ratio(pass == 0, v_b, xp_b, xq_b, e_b) : 0.f;
+        take = mine > held || (mine == held && v < v_b);
+        lo = hi = mine;
+        if (!take) low = up = held;
+      }
+      if (take) {
+        low = lo; up = hi; xp_b = xp; xq_b = xq; e_b = e; v_b = v;
       }
     };
     const bool rest = pass == 0 && row_q;
@@ -304,6 +339,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       for (int64_t v = c.mid + threadIdx.x; v < c.mid + c.vecs * V::N; v += kThreads)
         enter(v, to_f32(row_p[v]), rest ? to_f32(row_q[v]) : kNegInf, race[v]);
     }
+    float sure = low;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sure = fmaxf(sure, __shfl_xor_sync(0xffffffffu, sure, off));
+    uint64_t best_at = pack_best(0.f, v_b);
+    if (up > 0.f && up >= sure) best_at = pack_best(exact_ratio(pass == 0, v_b, xp_b, xq_b, e_b), v_b);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       const uint64_t o = __shfl_xor_sync(0xffffffffu, best_at, off);
@@ -312,6 +352,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     if (lane == 0) s_best[warp] = best_at;
     __syncthreads();
     if (threadIdx.x == 0) {
+#pragma unroll
       for (int i = 1; i < kWarps; ++i) best_at = best_at > s_best[i] ? best_at : s_best[i];
       s_cta_best = best_at;
     }
@@ -331,6 +372,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     cluster.sync();  // nobody leaves, or writes its best again, while others read it
     if (!empty) break;
   }
+}
+
+template <int TH>
+auto pick_kernel(int32_t kind, int log2n, int32_t dtype) -> void (*)(VerifyArgs) {
+  using bf16 = __nv_bfloat16;
+  const bool wide = dtype == ALGX_F32;
+  if (kind == ALGX_HEAD_CE) return wide ? verify_kernel<float, kSoftmax, 0, TH> : verify_kernel<bf16, kSoftmax, 0, TH>;
+  if (log2n == 3) return wide ? verify_kernel<float, kAsinh, 3, TH> : verify_kernel<bf16, kAsinh, 3, TH>;
+  return wide ? verify_kernel<float, kAsinh, 0, TH> : verify_kernel<bf16, kAsinh, 0, TH>;
 }
 
 }  // namespace
@@ -355,19 +405,20 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
   a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;
   a.scale = scale;
+  // Few sequences: all rows in one round, whose time is latency. Where the
+  // clusters fill the device, two positions a round: rows behind a refusal are
+  // mostly not read.
+  a.round = B * kCluster <= 148 ? (int)K + 1 : 2;
   a.slice = ((V + kCluster - 1) / kCluster + 7) / 8 * 8;
   while ((1 << a.log2n) < n) ++a.log2n;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  using bf16 = __nv_bfloat16;
-  void (*kern)(VerifyArgs);
-  if (kind == ALGX_HEAD_CE)
-    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kSoftmax, 0> : verify_kernel<float, kSoftmax, 0>;
-  else if (a.log2n == 3)
-    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kAsinh, 3> : verify_kernel<float, kAsinh, 3>;
-  else
-    kern = dtype == ALGX_BF16 ? verify_kernel<bf16, kAsinh, 0> : verify_kernel<float, kAsinh, 0>;
-  ALGX_CUDA(launch_dependent(kern, dim3((unsigned)(B * kCluster)), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
+  // 512 threads a CTA while the clusters leave SMs to themselves; above two CTAs
+  // an SM smaller ones, four an SM, which leaves less of a last wave.
+  const bool wide = B * kCluster <= 2 * 148;
+  void (*kern)(VerifyArgs) = wide ? pick_kernel<512>(kind, a.log2n, dtype) : pick_kernel<256>(kind, a.log2n, dtype);
+  const int threads = wide ? 512 : 256;
+  ALGX_CUDA(launch_dependent(kern, dim3((unsigned)(B * kCluster)), dim3(threads), 0, static_cast<cudaStream_t>(stream),
                              a));
   ALGX_LAUNCHED("verify_kernel");
   return ALGX_OK;
