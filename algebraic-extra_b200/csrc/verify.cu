@@ -30,9 +30,7 @@ namespace cg = cooperative_groups;
 namespace algx {
 namespace {
 
-constexpr int kCluster = 8;
 constexpr int kMaxRows = 64;  // of one round: 32 target rows, 31 draft rows
-constexpr int kUnroll = 4;    // 16-byte loads of a lane on their way together
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -122,7 +120,7 @@ __device__ __forceinline__ uint64_t pack_best(float value, int64_t v) {
 // Columns [begin, end) of a row in blocks of kUnroll 16-byte vectors a lane: the
 // aligned middle, and up to 2 (N - 1) single columns at the ends, which go with
 // the first block.
-template <typename T>
+template <typename T, int kUnroll>
 struct Columns {
   static constexpr int N = Vec<T>::N, kBlock = 32 * kUnroll;  // vectors of a block
   const T* row;
@@ -138,11 +136,12 @@ struct Columns {
   }
 };
 
-template <typename T, int KIND, int LOG2N, int kThreads>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1024 / kThreads)
-    verify_kernel(const VerifyArgs a) {
+template <typename T, int KIND, int LOG2N, int kCluster, int kThreads>
+__global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads) verify_kernel(const VerifyArgs a) {
   using V = Vec<T>;
   constexpr int kWarps = kThreads / 32;
+  constexpr int kUnroll = kCluster == 16 ? 8 : 4;  // 16-byte loads of a lane on their way together
+  using Cols = Columns<T, kUnroll>;
   __shared__ float2 s_part[kWarps + kMaxRows];  // (reference, sum) of every (warp, row) that meets, at warp + row
   __shared__ float2 s_row[2][kMaxRows];         // this CTA's (reference, sum) of every row, for two rounds
   __shared__ float s_turn[kMaxRows], s_l[kMaxRows];
@@ -192,7 +191,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 102
     const float x = score_of<KIND>(a, z);
     return x > kNegInf ? exact_weight<KIND>(a, x, s_turn[r]) / s_l[r] : 0.f;
   };
-  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Columns<T>::kBlock - 1) / (V::N * Columns<T>::kBlock));
+  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Cols::kBlock - 1) / (V::N * Cols::kBlock));
 
   // Rounds of a.round positions, up to the first refusal: rows after it are not
   // needed. Row r of a round is target row i0 + r, then draft row i0 + (r - nt).
@@ -208,7 +207,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 102
     const int stop = min(rows * blocks, at + share);
     while (at < stop) {
       const int r = at / blocks;
-      const Columns<T> c(r < nt ? target + (int64_t)(i0 + r) * a.V : draft + (int64_t)(i0 + r - nt) * a.V, begin, end);
+      const Cols c(r < nt ? target + (int64_t)(i0 + r) * a.V : draft + (int64_t)(i0 + r - nt) * a.V, begin, end);
       const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
       const int vecs = (int)c.vecs;
       RowSum<KIND, LOG2N> sum;
@@ -218,7 +217,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 102
         sum.add(a, z);
       }
       for (; at < stop && at < (r + 1) * blocks; ++at) {
-        const int v0 = (at - r * blocks) * Columns<T>::kBlock + lane;
+        const int v0 = (at - r * blocks) * Cols::kBlock + lane;
         uint4 raw[kUnroll];
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i)
@@ -312,7 +311,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 102
       }
     };
     const bool rest = pass == 0 && row_q;
-    const Columns<T> c(row_p, begin, end);
+    const Cols c(row_p, begin, end);
     if (threadIdx.x < c.ends()) {
       const int64_t v = c.end_column(threadIdx.x);
       enter(v, to_f32(row_p[v]), rest ? to_f32(row_q[v]) : kNegInf, race[v]);
@@ -374,13 +373,32 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 102
   }
 }
 
-template <int TH>
-auto pick_kernel(int32_t kind, int log2n, int32_t dtype) -> void (*)(VerifyArgs) {
-  using bf16 = __nv_bfloat16;
-  const bool wide = dtype == ALGX_F32;
-  if (kind == ALGX_HEAD_CE) return wide ? verify_kernel<float, kSoftmax, 0, TH> : verify_kernel<bf16, kSoftmax, 0, TH>;
-  if (log2n == 3) return wide ? verify_kernel<float, kAsinh, 3, TH> : verify_kernel<bf16, kAsinh, 3, TH>;
-  return wide ? verify_kernel<float, kAsinh, 0, TH> : verify_kernel<bf16, kAsinh, 0, TH>;
+template <int CL, int TH, typename T>
+auto pick(int32_t kind, int log2n) -> void (*)(VerifyArgs) {
+  if (kind == ALGX_HEAD_CE) return verify_kernel<T, kSoftmax, 0, CL, TH>;
+  return log2n == 3 ? verify_kernel<T, kAsinh, 3, CL, TH> : verify_kernel<T, kAsinh, 0, CL, TH>;
+}
+
+template <int CL, int TH>
+int verify_launch(const VerifyArgs& a, int32_t kind, int32_t dtype, int64_t B, cudaStream_t st) {
+  auto* kern = dtype == ALGX_BF16 ? pick<CL, TH, __nv_bfloat16>(kind, a.log2n) : pick<CL, TH, float>(kind, a.log2n);
+  if (CL > 8)  // clusters above 8 CTAs are this device's, not every one's
+    ALGX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * CL));
+  cfg.blockDim = dim3(TH);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CL;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  ALGX_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  ALGX_LAUNCHED("verify_kernel");
+  return ALGX_OK;
 }
 
 }  // namespace
@@ -398,28 +416,26 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   ALGX_REQUIRE(V >= 1 && V <= INT32_MAX, "the vocabulary must not be empty");
   ALGX_REQUIRE(scale > 0.f, "scale must be positive");
   if (B == 0) return ALGX_OK;
-  ALGX_REQUIRE(B <= INT32_MAX / kCluster, "too many sequences");
+  ALGX_REQUIRE(B <= INT32_MAX / 16, "too many sequences");
   ALGX_REQUIRE(target && race && out && accepted && (K == 0 || (tokens && u)), "NULL tensor");
   ALGX_REQUIRE((((uintptr_t)target | (uintptr_t)draft) & 3) == 0, "logits must be 4-byte aligned");
   VerifyArgs a = {};
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
   a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;
   a.scale = scale;
-  // Few sequences: all rows in one round, whose time is latency. Where the
-  // clusters fill the device, two positions a round: rows behind a refusal are
-  // mostly not read.
-  a.round = B * kCluster <= 148 ? (int)K + 1 : 2;
-  a.slice = ((V + kCluster - 1) / kCluster + 7) / 8 * 8;
   while ((1 << a.log2n) < n) ++a.log2n;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  // 512 threads a CTA while the clusters leave SMs to themselves; above two CTAs
-  // an SM smaller ones, four an SM, which leaves less of a last wave.
-  const bool wide = B * kCluster <= 2 * 148;
-  void (*kern)(VerifyArgs) = wide ? pick_kernel<512>(kind, a.log2n, dtype) : pick_kernel<256>(kind, a.log2n, dtype);
-  const int threads = wide ? 512 : 256;
-  ALGX_CUDA(launch_dependent(kern, dim3((unsigned)(B * kCluster)), dim3(threads), 0, static_cast<cudaStream_t>(stream),
-                             a));
-  ALGX_LAUNCHED("verify_kernel");
-  return ALGX_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Few sequences: all rows in one round, whose time is latency, over as many SMs
+  // as a cluster spans. Where the clusters fill the device, three positions a
+  // round, as rows behind a refusal are mostly not read, and smaller CTAs, four
+  // an SM, which leave less of a last wave.
+  const bool few = B * 16 <= 148, wide = B * 8 <= 2 * 148;
+  const int64_t cluster = few ? 16 : 8;
+  a.round = wide ? (int)K + 1 : 3;
+  a.slice = ((V + cluster - 1) / cluster + 7) / 8 * 8;
+  return few    ? verify_launch<16, 512>(a, kind, dtype, B, st)
+         : wide ? verify_launch<8, 512>(a, kind, dtype, B, st)
+                : verify_launch<8, 256>(a, kind, dtype, B, st);
 }
