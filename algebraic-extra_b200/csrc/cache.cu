@@ -2,6 +2,7 @@
 // tokens (QK norm and rotation on the way in) and evicting slots by accumulated
 // attention weight.
 #include <algorithm>
+#include <atomic>
 
 #include "paged_common.cuh"
 #include "vec_io.cuh"
@@ -130,8 +131,12 @@ int append_launch(const AppendArgs& a, const PagedView& pv, int64_t blocks, cuda
 }
 
 // ------------------------------------------------------------------ eviction
-constexpr int kEvThreads = 1024;
+constexpr int kEvThreads = 512;
 constexpr int kEvWarps = kEvThreads / 32;
+constexpr int kEvChunk = 4 * kEvThreads;     // slots of one sweep of the block, four a thread
+constexpr int kEvCached = 48 * 1024;         // keys kept in shared memory
+constexpr int kBins = 4 * kEvThreads;        // 11 bits a round, 10 in the last
+constexpr int kInplace = 1024;
 
 struct EvictArgs {
   void *k_pages, *v_pages;
@@ -139,10 +144,13 @@ struct EvictArgs {
   const int32_t* positions;
   float* new_scores;
   int32_t *new_positions, *new_lens, *kept;
-  int32_t* holes;  // workspace (B, Hkv, budget)
+  int2* moves;  // workspace (B, Hkv, budget): (to, from) slots
+  int* counts;  // workspace (B, Hkv): moves of each item
   int* err;
   int budget, first, recent;
-  int row_bytes;
+  int lanes;    // 16-byte pieces of a row
+  int cached;   // whether the keys fit shared memory
+  int inplace;  // whether the CTA that chose the rows moves them too
 };
 
 // Order-preserving map of a float to an unsigned key (NaN below everything).
@@ -153,156 +161,243 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum of two counts over the block; totals in tot.
-__device__ __forceinline__ int2 block_scan2(int2 v, int2* warp_sums, int2& tot) {
+// Inclusive sum over the block of one int a thread; the total goes to `total`.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int2 s = v;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, s.x, off), y = __shfl_up_sync(0xffffffffu, s.y, off);
-    if (lane >= off) { s.x += x; s.y += y; }
+    const int x = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += x;
   }
+  if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  if (lane == 31) warp_sums[warp] = s;
-  __syncthreads();
-  if (warp == 0) {
-    int2 t = lane < kEvWarps ? warp_sums[lane] : make_int2(0, 0);
+  int before = 0;
+  total = 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, t.x, off), y = __shfl_up_sync(0xffffffffu, t.y, off);
-      if (lane >= off) { t.x += x; t.y += y; }
-    }
-    warp_sums[lane] = t;
+  for (int i = 0; i < kEvWarps; ++i) {
+    const int x = warp_sums[i];
+    if (i < warp) before += x;
+    total += x;
   }
   __syncthreads();
-  const int2 before = warp > 0 ? warp_sums[warp - 1] : make_int2(0, 0);
-  tot = warp_sums[kEvWarps - 1];
-  return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
+  return before + v;
 }
 
-// One CTA per (sequence, kv head). The budget-th largest key is found by four
-// rounds of 8-bit counting; slots above it stay, and of those equal to it the
-// lowest slots. The kept slots at or above the budget then move, in order, into
-// the holes below it, so a row that is already below the budget never moves.
-__global__ void __launch_bounds__(kEvThreads) cache_evict_kernel(const EvictArgs a, const PagedView pv) {
-  __shared__ int hist[256];
-  __shared__ int2 warp_sums[32];
-  __shared__ int s_newest, s_digit, s_left;
-  const int tid = threadIdx.x;
+// Rows i0, i0 + step, ... of an item's moves, counted in 16-byte pieces: keys and
+// values, kFly pieces of each in flight.
+template <int kFly>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& pv, int64_t bh, int i0, int end, int step) {
+  const int b = (int)(bh / pv.heads), h = (int)(bh - (int64_t)b * pv.heads);
+  const int32_t* table = pv.table + (int64_t)b * pv.max_pages;
+  const int2* moves = a.moves + bh * a.budget;
+  const int row_bytes = a.lanes * 16, row_shift = a.lanes == 8 ? 3 : 4;
+  for (; i0 < end; i0 += step * kFly) {
+    uint4 kv[kFly], vv[kFly];
+    int64_t to[kFly], of[kFly];
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      const int i = i0 + j * step;
+      to[j] = -1;
+      if (i >= end) continue;
+      const int2 move = moves[i >> row_shift];
+      const int pd = table[move.x >> pv.page_shift], ps = table[move.y >> pv.page_shift];
+      if ((unsigned)pd >= (unsigned)pv.num_pages || (unsigned)ps >= (unsigned)pv.num_pages) {
+        atomicOr(a.err, DEV_ERR_BAD_PAGE);
+        continue;
+      }
+      const int part = (i & (a.lanes - 1)) * 16;
+      to[j] = paged_row(pv, pd, h, move.x) / kD * row_bytes + part;
+      of[j] = paged_row(pv, ps, h, move.y) / kD * row_bytes + part;
+    }
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      if (to[j] < 0) continue;
+      kv[j] = ld_stream(static_cast<const char*>(a.k_pages) + of[j]);
+      vv[j] = ld_stream(static_cast<const char*>(a.v_pages) + of[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kFly; ++j) {
+      if (to[j] < 0) continue;
+      *reinterpret_cast<uint4*>(static_cast<char*>(a.k_pages) + to[j]) = kv[j];
+      *reinterpret_cast<uint4*>(static_cast<char*>(a.v_pages) + to[j]) = vv[j];
+    }
+  }
+}
+
+// One CTA per (sequence, kv head). The budget-th largest key is found by three
+// rounds of counting 11 bits; slots above it stay, and of those equal to it the
+// lowest slots. One sweep over the slots then numbers the holes below the budget
+// and the kept slots at or above it: the i-th such slot moves to the i-th hole, so
+// a row that is below the budget never moves. This is a chain of some twenty
+// block-wide steps, whatever the length.
+__global__ void __launch_bounds__(kEvThreads, 2) cache_evict_kernel(const EvictArgs a, const PagedView pv) {
+  extern __shared__ uint4 s_keys[];
+  __shared__ int4 hist[kBins / 4];
+  __shared__ int warp_sums[kEvWarps];
+  __shared__ int s_newest, s_digit, s_left, s_equal;
+  int* const bins = reinterpret_cast<int*>(hist);
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31;
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / pv.heads), h = (int)(bh - (int64_t)b * pv.heads);
   const int len = paged_len(pv, b, a.err);
-  const int64_t S = (int64_t)pv.max_pages << pv.page_shift;
+  const int S = pv.max_pages << pv.page_shift;  // a multiple of 16
   const float* scores = a.scores + bh * S;
   const int32_t* positions = a.positions + bh * S;
   float* new_scores = a.new_scores + bh * S;
   int32_t* new_positions = a.new_positions + bh * S;
   int32_t* kept = a.kept + bh * a.budget;
-  int32_t* holes = a.holes + bh * a.budget;
-  const int out_len = len < a.budget ? len : a.budget;
+  int2* moves = a.moves + bh * a.budget;
+  const int out_len = min(len, a.budget);
   if (h == 0 && tid == 0) a.new_lens[b] = out_len;
-
-  if (len > a.budget) {
-    if (tid == 0) s_newest = -1;
-    __syncthreads();
-    int newest = -1;
-    for (int s = tid; s < len; s += kEvThreads) newest = max(newest, positions[s]);
-    newest = __reduce_max_sync(0xffffffffu, newest);
-    if ((tid & 31) == 0) atomicMax(&s_newest, newest);
-    __syncthreads();
-    newest = s_newest;
-    const int64_t from = (int64_t)newest - a.recent;  // positions above it are recent
-    auto key_at = [&](int s) -> uint32_t {
-      const int p = positions[s];
-      return p < a.first || p > from ? score_key(__int_as_float(0x7f800000)) : score_key(scores[s]);
-    };
-    // the budget-th largest key, and how many of its equals stay
-    uint32_t prefix = 0;
-    int left = a.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kEvThreads) hist[i] = 0;
-      __syncthreads();
-      const uint32_t high = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int s = tid; s < len; s += kEvThreads) {
-        const uint32_t k = key_at(s);
-        if ((k & high) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+  // Everything below the new length first as if nothing moved; the moves write
+  // over their holes later.
+  auto copy_row = [&](int s, const float4& x, const int4& p) {
+    if (s + 4 <= out_len) {
+      *reinterpret_cast<float4*>(new_scores + s) = x;
+      *reinterpret_cast<int4*>(new_positions + s) = p;
+    } else {
+      const float xs[4] = {x.x, x.y, x.z, x.w};
+      const int ps[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        new_scores[s + i] = s + i < out_len ? xs[i] : 0.f;
+        new_positions[s + i] = s + i < out_len ? ps[i] : -1;
       }
-      __syncthreads();
-      if (tid == 0) {
-        int above = 0, d = 255;
-        while (d > 0 && above + hist[d] < left) above += hist[d--];
-        s_digit = d;
-        s_left = left - above;
-      }
-      __syncthreads();
-      prefix |= (uint32_t)s_digit << shift;
-      left = s_left;
-      __syncthreads();
     }
-    // holes below the budget, then movers above it, both in slot order
-    int equal_before = 0, holes_before = 0;
-    for (int s0 = 0; s0 < len; s0 += kEvThreads) {
-      const int s = s0 + tid;
-      const uint32_t k = s < len ? key_at(s) : 0u;
-      const bool equal = s < len && k == prefix;
-      int2 tot;
-      const int2 r = block_scan2(make_int2(equal, 0), warp_sums, tot);
-      const bool keep = s < len && (k > prefix || (equal && equal_before + r.x < left));
-      equal_before += tot.x;
-      const bool hole = s < a.budget && !keep;
-      const bool mover = s >= a.budget && keep;
-      const int2 q = block_scan2(make_int2(hole, mover), warp_sums, tot);
-      // equal counts of holes and movers: the running index serves both lists
-      if (hole) holes[holes_before + q.x] = s;
-      if (s < a.budget && keep) kept[s] = s;
-      holes_before += tot.x;
-      (void)q;
+  };
+  for (int s = tid; s < a.budget; s += kEvThreads) kept[s] = s < out_len ? s : -1;
+  for (int i = tid; i < kBins / 4; i += kEvThreads) hist[i] = make_int4(0, 0, 0, 0);
+  if (tid == 0) s_newest = -1;
+  __syncthreads();
+  int newest = -1;
+#pragma unroll 4
+  for (int s = 4 * tid; s < S; s += kEvChunk) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    int4 p = make_int4(-1, -1, -1, -1);
+    if (s < len) {
+      x = *reinterpret_cast<const float4*>(scores + s);
+      p = *reinterpret_cast<const int4*>(positions + s);
+      newest = max(newest, p.x);
+      if (s + 1 < len) newest = max(newest, p.y);
+      if (s + 2 < len) newest = max(newest, p.z);
+      if (s + 3 < len) newest = max(newest, p.w);
     }
-    __syncthreads();
-    equal_before = 0;
-    int movers_before = 0;
-    for (int s0 = 0; s0 < len; s0 += kEvThreads) {
-      const int s = s0 + tid;
-      const uint32_t k = s < len ? key_at(s) : 0u;
-      const bool equal = s < len && k == prefix;
-      int2 tot;
-      const int2 r = block_scan2(make_int2(equal, 0), warp_sums, tot);
-      const bool keep = s < len && (k > prefix || (equal && equal_before + r.x < left));
-      equal_before += tot.x;
-      const bool mover = s >= a.budget && keep;
-      const int2 q = block_scan2(make_int2(mover, 0), warp_sums, tot);
-      if (mover) kept[holes[movers_before + q.x]] = s;
-      movers_before += tot.x;
-    }
-    __syncthreads();
-    // the rows themselves: 16 bytes a thread
-    const int lanes = a.row_bytes / 16;
-    const int64_t chunks = (int64_t)movers_before * lanes;
-    for (int64_t i = tid; i < chunks; i += kEvThreads) {
-      const int dst = holes[i / lanes], part = (int)(i % lanes);
-      const int src = kept[dst];
-      const int pd = pv.table[(int64_t)b * pv.max_pages + (dst >> pv.page_shift)];
-      const int ps = pv.table[(int64_t)b * pv.max_pages + (src >> pv.page_shift)];
-      if (pd < 0 || pd >= pv.num_pages || ps < 0 || ps >= pv.num_pages) {
-        atomicOr(a.err, DEV_ERR_BAD_PAGE);
-        continue;
-      }
-      const int64_t to = paged_row(pv, pd, h, dst) / kD * a.row_bytes + part * 16;
-      const int64_t of = paged_row(pv, ps, h, src) / kD * a.row_bytes + part * 16;
-      const uint4 kv = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.k_pages) + of);
-      const uint4 vv = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.v_pages) + of);
-      *reinterpret_cast<uint4*>(static_cast<char*>(a.k_pages) + to) = kv;
-      *reinterpret_cast<uint4*>(static_cast<char*>(a.v_pages) + to) = vv;
-    }
-  } else {
-    for (int s = tid; s < len; s += kEvThreads) kept[s] = s;
-    __syncthreads();
+    copy_row(s, x, p);
   }
-  for (int s = out_len + tid; s < a.budget; s += kEvThreads) kept[s] = -1;
-  for (int64_t s = tid; s < S; s += kEvThreads) {
-    const int src = s < out_len ? kept[s] : -1;
-    new_scores[s] = src >= 0 ? scores[src] : 0.f;
-    new_positions[s] = src >= 0 ? positions[src] : -1;
+  int movers = 0;
+  if (len > a.budget) {
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) atomicMax(&s_newest, newest);
+    __syncthreads();
+    const int64_t from = (int64_t)s_newest - a.recent;  // positions above it are recent
+    auto key = [&](float x, int p) { return score_key(p < a.first || p > from ? __int_as_float(0x7f800000) : x); };
+    auto make_keys = [&](int s) {
+      const float4 x = *reinterpret_cast<const float4*>(scores + s);
+      const int4 p = *reinterpret_cast<const int4*>(positions + s);
+      return make_uint4(key(x.x, p.x), key(x.y, p.y), key(x.z, p.z), key(x.w, p.w));
+    };
+
+    // the budget-th largest key, and how many of its equals stay
+    uint32_t limit = 0;
+    int left = a.budget;
+#pragma unroll
+    for (int round = 0; round < 3; ++round) {
+      const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, mask = round == 2 ? 1023 : kBins - 1;
+#pragma unroll 4
+      for (int s = 4 * tid; s < len; s += kEvChunk) {
+        const uint4 k4 = round > 0 && a.cached ? s_keys[s >> 2] : make_keys(s);
+        if (round == 0 && a.cached) s_keys[s >> 2] = k4;  // read by the same thread only
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = s + i < len && (round == 0 || (k[i] >> (round == 1 ? 21 : 10)) == limit);
+          const int bin = (int)((k[i] >> shift) & mask);
+          if (in) atomicAdd(&bins[bin], 1);
+        }
+      }
+      __syncthreads();
+      // the bin where the count from above reaches `left`: four bins a thread
+      const int quad = kEvThreads - 1 - tid;
+      const int4 q = hist[quad];
+      const int c[4] = {q.w, q.z, q.y, q.x};
+      int total;
+      const int mine = c[0] + c[1] + c[2] + c[3], upto = block_scan(mine, warp_sums, total);
+      if (upto >= left && upto - mine < left) {
+        int above = upto - mine, d = 0;
+        while (above + c[d] < left) above += c[d++];
+        s_digit = 4 * quad + 3 - d;
+        s_left = left - above;
+        s_equal = c[d];
+      }
+      hist[quad] = make_int4(0, 0, 0, 0);
+      __syncthreads();
+      limit = round == 0 ? (uint32_t)s_digit : (limit << (round == 1 ? 11 : 10)) | (uint32_t)s_digit;
+      left = s_left;
+    }
+    const bool all_equals = s_equal == left;  // the usual case: no ties at the limit
+
+    int equals = 0, holes = 0;
+    for (int s0 = 0; s0 < len; s0 += kEvChunk) {
+      const int s = s0 + 4 * tid;
+      const uint4 k4 = s < len ? (a.cached ? s_keys[s >> 2] : make_keys(s)) : make_uint4(0, 0, 0, 0);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      bool keep[4];
+      if (all_equals) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keep[i] = s + i < len && k[i] >= limit;
+      } else {
+        int n = 0, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += s + i < len && k[i] == limit;
+        int rank = equals + block_scan(n, warp_sums, total) - n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool equal = s + i < len && k[i] == limit;
+          keep[i] = s + i < len && (k[i] > limit || (equal && rank < left));
+          rank += equal;
+        }
+        equals += total;
+      }
+      int n = 0, total;  // holes in the low half, movers in the high one
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n += s + i < a.budget ? (s + i < len && !keep[i]) : keep[i] << 16;
+      const int upto = block_scan(n, warp_sums, total) - n;
+      int hole = holes + (upto & 0xffff), mover = movers + (upto >> 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s + i < a.budget && s + i < len && !keep[i]) moves[hole++].x = s + i;
+        if (s + i >= a.budget && keep[i]) moves[mover++].y = s + i;
+      }
+      holes += total & 0xffff;
+      movers += total >> 16;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < movers; i += kEvThreads) {
+      const int2 move = moves[i];
+      kept[move.x] = move.y;
+      new_scores[move.x] = scores[move.y];
+      new_positions[move.x] = positions[move.y];
+    }
+    if (a.inplace) move_rows<4>(a, pv, bh, tid, movers * a.lanes, kEvThreads);
+  }
+  if (tid == 0) a.counts[bh] = movers;
+}
+
+// The moves of all items, spread over the device: kMovePieces 16-byte pieces of
+// keys and of values a CTA at a time.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveFly = 4;
+constexpr int kMovePieces = kMoveThreads * kMoveFly;
+
+__global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const EvictArgs a, const PagedView pv, int items,
+                                                                  int chunks) {
+  pdl_wait();
+  for (int64_t i = blockIdx.x; i < (int64_t)items * chunks; i += gridDim.x) {
+    const int chunk = (int)(i / items), item = (int)(i - (int64_t)chunk * items);
+    const int begin = chunk * kMovePieces, end = min(begin + kMovePieces, a.counts[item] * a.lanes);
+    if (begin < end) move_rows<kMoveFly>(a, pv, item, begin + threadIdx.x, end, kMoveThreads);
   }
 }
 
@@ -372,7 +467,7 @@ int algx_cache_append(const void* qkv, const float* gain_q, const float* gain_k,
 }
 
 size_t algx_cache_evict_workspace_size(int64_t B, int64_t Hkv, int64_t budget) {
-  return B > 0 && Hkv > 0 && budget > 0 ? (size_t)(B * Hkv * budget) * sizeof(int32_t) : 0;
+  return B > 0 && Hkv > 0 && budget > 0 ? (size_t)(B * Hkv * budget) * sizeof(int2) + (size_t)(B * Hkv) * sizeof(int) : 0;
 }
 
 int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const int32_t* lens, const float* scores,
@@ -392,19 +487,44 @@ int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const i
                "NULL tensor");
   ALGX_REQUIRE(scores != new_scores && positions != new_positions && lens != new_lens,
                "the new scores, positions and lengths need their own buffers");
-  ALGX_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "tensors must be 16-byte aligned");
+  ALGX_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)scores | (uintptr_t)positions) & 15) == 0 &&
+                   ((uintptr_t)workspace & 7) == 0,
+               "tensors must be 16-byte aligned");
   ALGX_REQUIRE(workspace && workspace_bytes >= algx_cache_evict_workspace_size(B, Hkv, budget),
                "workspace too small");
   EvictArgs a = {};
   a.k_pages = k_pages; a.v_pages = v_pages; a.scores = scores; a.positions = positions;
   a.new_scores = new_scores; a.new_positions = new_positions; a.new_lens = new_lens; a.kept = kept;
-  a.holes = static_cast<int32_t*>(workspace);
+  a.moves = static_cast<int2*>(workspace);
+  a.counts = reinterpret_cast<int*>(a.moves + B * Hkv * budget);
   a.budget = (int)budget; a.first = (int)first; a.recent = (int)recent;
-  a.row_bytes = dtype == ALGX_BF16 ? 128 : 256;
+  a.lanes = dtype == ALGX_BF16 ? 8 : 16;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  cache_evict_kernel<<<(unsigned)(B * Hkv), kEvThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, pv);
+  const int64_t S = page_size * max_pages;
+  // Rows an item can move at most. Up to kInplace of them its own CTA moves them,
+  // which saves a launch; more are spread over the device.
+  const int64_t most = std::min<int64_t>(budget, std::max<int64_t>(0, S - budget));
+  a.inplace = most <= kInplace;
+  a.cached = S <= kEvCached;
+  const size_t smem = a.cached ? (size_t)S * sizeof(uint32_t) : 0;
+  static std::atomic<uint64_t> ready{0};  // one bit per device: its shared memory limit is raised
+  int dev = 0;
+  ALGX_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    ALGX_CUDA(cudaFuncSetAttribute(cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kEvCached * (int)sizeof(uint32_t)));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  ALGX_CUDA(launch_dependent(cache_evict_kernel, dim3((unsigned)(B * Hkv)), dim3(kEvThreads), smem,
+                             static_cast<cudaStream_t>(stream), a, pv));
   ALGX_LAUNCHED("cache_evict_kernel");
+  if (a.inplace) return ALGX_OK;
+  const int64_t items = B * Hkv, chunks = (most * a.lanes + kMovePieces - 1) / kMovePieces;
+  ALGX_CUDA(launch_dependent(cache_move_kernel, dim3((unsigned)std::min<int64_t>(items * chunks, 148 * 8)),
+                             dim3(kMoveThreads), 0, static_cast<cudaStream_t>(stream), a, pv, (int)items, (int)chunks));
+  ALGX_LAUNCHED("cache_move_kernel");
   return ALGX_OK;
 }
 
