@@ -31,43 +31,51 @@ import torch
 
 from .. import _lib as L
 
-_IO = (torch.bfloat16, torch.float32)
+_CODE = {torch.bfloat16: L.ALGX_BF16, torch.float32: L.ALGX_F32}
+_SIZES = frozenset((16, 32, 64, 128, 256))
 _I32, _F32 = torch.int32, torch.float32
 
 
+# A decode step makes these calls once per layer on small tensors, where the
+# host's time is the call's: the checks read each attribute once.
 def _check_cache(k_pages, v_pages, table, lens):
-    """Shapes and dtypes of a paged cache; returns (num_pages, Hkv, page_size, B, max_pages)."""
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    """Shapes and dtypes of a paged cache; returns (num_pages, Hkv, page_size, B, max_pages, dtype code)."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype:
         raise ValueError("k_pages and v_pages must both have shape (num_pages, heads, page_size, 64) and one dtype")
-    num, heads, size, D = k_pages.shape
+    num, heads, size, D = shape
     if D != 64:
         raise ValueError(f"algx paged cache supports head_dim 64, got {D}")
-    if k_pages.dtype not in _IO:
+    code = _CODE.get(dtype)
+    if code is None:
         raise ValueError("paged cache must be bfloat16 or float32")
-    if size < 16 or size > 256 or size & (size - 1):
+    if size not in _SIZES:
         raise ValueError(f"page_size must be a power of two from 16 to 256, got {size}")
     if num < 1 or heads < 1:
         raise ValueError("paged cache has no pages or no heads")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages and v_pages must be contiguous")
-    if table.ndim != 2 or lens.ndim != 1 or lens.shape[0] != table.shape[0] or table.shape[1] < 1:
+    tshape = table.shape
+    if len(tshape) != 2 or lens.shape != tshape[:1] or tshape[1] < 1:
         raise ValueError("table must have shape (B, max_pages) and lens (B,)")
     if table.dtype != _I32 or lens.dtype != _I32:
         raise ValueError("table and lens must be int32")
-    return num, heads, size, table.shape[0], table.shape[1]
+    return num, heads, size, tshape[0], tshape[1], code
 
 
 def _check_state(name, t, shape, dtype):
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of shape {shape}")
 
 
 def _same_device(ref, *tensors):
+    dev = ref.get_device()
     for t in tensors:
-        if t is not None and t.device != ref.device:
-            L.require_cuda(t)
+        if t is not None and t.get_device() != dev:
+            L.require_cuda(ref, t)
             raise ValueError(f"tensors on {ref.device} and {t.device} in one call")
-    L.require_cuda(ref)
+    if dev < 0:
+        L.require_cuda(ref)
 
 
 def _per_sequence(name, t, B):
@@ -91,9 +99,10 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
     ``slot_positions`` (B, Hkv, max_pages * page_size) int32 receives the new
     slots' positions, which ``cache_evict`` reads.
     """
-    num, Hkv, size, B, maxp = _check_cache(k_pages, v_pages, table, lens)
-    if qkv.ndim != 4 or qkv.shape[0] != B or qkv.shape[3] != 64 or qkv.shape[2] < 2 * Hkv:
-        raise ValueError(f"qkv must have shape ({B}, T, Hq + {2 * Hkv}, 64), got {tuple(qkv.shape)}")
+    num, Hkv, size, B, maxp, code = _check_cache(k_pages, v_pages, table, lens)
+    shape = qkv.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != 64 or shape[2] < 2 * Hkv:
+        raise ValueError(f"qkv must have shape ({B}, T, Hq + {2 * Hkv}, 64), got {tuple(shape)}")
     if qkv.dtype != k_pages.dtype:
         raise ValueError(f"qkv ({qkv.dtype}) and the cache ({k_pages.dtype}) must share one dtype")
     if (gain_q is None) != (gain_k is None):
@@ -109,11 +118,12 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
         gain_q, gain_k = gain_q.contiguous(), gain_k.contiguous()
     if rotary is not None:
         cos, sin = rotary
-        if cos.ndim != 2 or cos.shape[1] != 32 or cos.shape != sin.shape or cos.dtype != _F32 or sin.dtype != _F32 \
-                or cos.shape[0] < 1:
+        rshape = cos.shape
+        if len(rshape) != 2 or rshape[1] != 32 or sin.shape != rshape or cos.dtype != _F32 or sin.dtype != _F32 \
+                or rshape[0] < 1:
             raise ValueError("rotary tables must both be float32 of shape (rows, 32)")
         cos, sin = cos.contiguous(), sin.contiguous()
-        rows = cos.shape[0]
+        rows = rshape[0]
     if positions is not None:
         positions = _per_sequence("positions", positions, B)
     if counts is not None:
@@ -122,12 +132,12 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
         _check_state("slot_positions", slot_positions, (B, Hkv, maxp * size), _I32)
     _same_device(qkv, k_pages, v_pages, table, lens, gain_q, gain_k, cos, sin, positions, counts, slot_positions)
     qkv, table, lens = qkv.contiguous(), table.contiguous(), lens.contiguous()
-    T, Hq = qkv.shape[1], qkv.shape[2] - 2 * Hkv
-    q = torch.empty((B, T, Hq, 64), dtype=qkv.dtype, device=qkv.device)
+    T, Hq = shape[1], shape[2] - 2 * Hkv
+    q = qkv.new_empty((B, T, Hq, 64))
     L.check(L.lib().algx_cache_append(
         qkv.data_ptr(), L.ptr(gain_q), L.ptr(gain_k), L.ptr(cos), L.ptr(sin), rows, table.data_ptr(), lens.data_ptr(),
         L.ptr(positions), L.ptr(counts), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), L.ptr(slot_positions),
-        B, T, Hq, Hkv, num, size, maxp, 64, L.dtype_code(qkv.dtype), eps, L.stream_of(qkv)), "algx_cache_append")
+        B, T, Hq, Hkv, num, size, maxp, 64, code, eps, L.stream_of(qkv)), "algx_cache_append")
     return q
 
 
@@ -147,6 +157,12 @@ def paged_config(kind: str, n: int, c: float, window: Optional[int], first: int)
     unit = float(c) if kind == "asinh" else 1.0
     return L.PagedConfig(L.ALGX_ATTN_ASINH if kind == "asinh" else L.ALGX_ATTN_SOFTMAX,
                          int(n) if kind == "asinh" else 2, window or 0, first, 1.0 / (8.0 * unit), 1.0 / unit)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_workspace(*sizes) -> int:
+    """``algx_paged_attn_workspace_size``, a function of its arguments alone."""
+    return max(L.lib().algx_paged_attn_workspace_size(*sizes), 1)
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: str = "softmax", n: int = 16,
@@ -169,20 +185,21 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
     returns ``(o, scores_out)``. The T new slots start from zero, slots beyond
     ``lens`` are set to zero.
     """
-    num, Hkv, size, B, maxp = _check_cache(k_pages, v_pages, table, lens)
-    if q.ndim != 4 or q.shape[0] != B or q.shape[3] != 64 or q.shape[2] < 1 or q.shape[2] % Hkv:
-        raise ValueError(f"q must have shape ({B}, T, Hq, 64) with Hq a multiple of {Hkv}, got {tuple(q.shape)}")
+    num, Hkv, size, B, maxp, code = _check_cache(k_pages, v_pages, table, lens)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != 64 or shape[2] < 1 or shape[2] % Hkv:
+        raise ValueError(f"q must have shape ({B}, T, Hq, 64) with Hq a multiple of {Hkv}, got {tuple(shape)}")
     if q.dtype != k_pages.dtype:
         raise ValueError(f"q ({q.dtype}) and the cache ({k_pages.dtype}) must share one dtype")
     cfg = paged_config(kind, n, c, window, first)
-    T, Hq = q.shape[1], q.shape[2]
+    T, Hq = shape[1], shape[2]
     sink = None
     if sink_logit is not None:
         sink = sink_logit
         if not torch.is_tensor(sink) or sink.dtype != _F32 or sink.shape != (Hq,) or sink.device != q.device:
             sink = torch.as_tensor(sink, dtype=_F32, device=q.device)
             sink = torch.broadcast_to(sink.reshape(-1), (Hq,))
-        sink = sink.detach().contiguous()
+        sink = sink.contiguous()
     if scores is not None:
         scores_out = scores if scores_out is None else scores_out
         _check_state("scores", scores, (B, Hkv, maxp * size), _F32)
@@ -191,16 +208,19 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
         raise ValueError("scores_out without scores")
     _same_device(q, k_pages, v_pages, table, lens, scores, scores_out)
     q, table, lens = q.contiguous(), table.contiguous(), lens.contiguous()
-    lib = L.lib()
     o = torch.empty_like(q)
-    code = L.dtype_code(q.dtype)
-    nbytes = lib.algx_paged_attn_workspace_size(B, T, Hq, Hkv, size, maxp, scores is not None, code)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
-    L.check(lib.algx_paged_attn(
+    nbytes = _attn_workspace(B, T, Hq, Hkv, size, maxp, scores is not None, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    L.check(L.lib().algx_paged_attn(
         cfg, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.ptr(sink),
         L.ptr(scores), L.ptr(scores_out), o.data_ptr(), B, T, Hq, Hkv, num, size, maxp, 64, code, ws.data_ptr(),
         nbytes, L.stream_of(q)), "algx_paged_attn")
     return o if scores is None else (o, scores_out)
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(*sizes) -> int:
+    return max(L.lib().algx_cache_evict_workspace_size(*sizes), 1)
 
 
 def cache_evict(k_pages, v_pages, table, lens, scores, positions, *, budget: int, first: int = 0, recent: int = 0):
@@ -220,7 +240,7 @@ def cache_evict(k_pages, v_pages, table, lens, scores, positions, *, budget: int
     (-1: none). The inputs are not changed, so repeating a call repeats its
     result. The pages beyond the new lengths are free afterwards.
     """
-    num, Hkv, size, B, maxp = _check_cache(k_pages, v_pages, table, lens)
+    num, Hkv, size, B, maxp, code = _check_cache(k_pages, v_pages, table, lens)
     S = maxp * size
     if not 1 <= budget < 2 ** 31:
         raise ValueError("budget must be positive")
@@ -235,12 +255,11 @@ def cache_evict(k_pages, v_pages, table, lens, scores, positions, *, budget: int
     new_scores = torch.empty_like(scores)
     new_positions = torch.empty_like(positions)
     kept = torch.empty((B, Hkv, budget), dtype=_I32, device=dev)
-    lib = L.lib()
-    nbytes = lib.algx_cache_evict_workspace_size(B, Hkv, budget)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    L.check(lib.algx_cache_evict(
+    nbytes = _evict_workspace(B, Hkv, budget)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    L.check(L.lib().algx_cache_evict(
         k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), scores.data_ptr(),
         positions.data_ptr(), budget, first, recent, new_lens.data_ptr(), new_scores.data_ptr(),
-        new_positions.data_ptr(), kept.data_ptr(), B, Hkv, num, size, maxp, 64, L.dtype_code(k_pages.dtype),
-        ws.data_ptr(), nbytes, L.stream_of(k_pages)), "algx_cache_evict")
+        new_positions.data_ptr(), kept.data_ptr(), B, Hkv, num, size, maxp, 64, code, ws.data_ptr(), nbytes,
+        L.stream_of(k_pages)), "algx_cache_evict")
     return new_lens, new_scores, new_positions, kept

@@ -14,7 +14,7 @@ constexpr int kD = 64;
 
 // ------------------------------------------------------------------- append
 constexpr int kAppThreads = 256;
-constexpr int kAppPasses = 4;  // row groups of one warp, loaded together
+constexpr int kAppPasses = 3;  // row groups of one warp, loaded together
 
 struct AppendArgs {
   const void* qkv;
@@ -28,54 +28,57 @@ struct AppendArgs {
   float eps;
 };
 
-// One warp takes `passes` groups of RPW head rows of one token, so the token's
-// slot, page and rotation angles are found once for all of them. y = rms(x) g,
-// then (y1 c - y2 s, y1 s + y2 c), all in fp32 with one rounding at the store:
-// the cache holds the nearest bf16 of the exact key. Bound by memory: each row
-// is read once and written once.
+// One warp takes `passes` groups of head rows of one token, so the token's slot,
+// page and rotation angles are found once for all of them. A lane holds a 16-byte
+// chunk of a row's first half and the chunk 32 elements on, which the rotation
+// pairs: it needs no exchange, and the norm two shuffles (bf16: 4 lanes a row, 8
+// rows a group). y = rms(x) g, then (y1 c - y2 s, y1 s + y2 c), all in fp32 with
+// one rounding at the store: the cache holds the nearest bf16 of the exact key.
+// Bound by memory: each row is read once and written once.
 template <typename T, bool NORM, bool ROT>
 __global__ void __launch_bounds__(kAppThreads) cache_append_kernel(const AppendArgs a, const PagedView pv) {
   using V = Vec<T>;
-  constexpr int kHalfT = V::TPR / 2;
-  const int lane = threadIdx.x & 31, sub = lane % V::TPR, rl = lane / V::TPR;
+  constexpr int N = V::N, kLanes = V::TPR / 2, kRows = 32 / kLanes;
+  pdl_wait();
+  const int lane = threadIdx.x & 31, sub = lane % kLanes, rl = lane / kLanes;
   const int64_t w = (int64_t)blockIdx.x * (kAppThreads / 32) + (threadIdx.x >> 5);
   const int64_t tok = w / a.segs;
   if (tok >= a.tokens) return;
   const int seg = (int)(w - tok * a.segs);
   const int heads = a.Hq + 2 * pv.heads;
-  const int h0 = seg * a.passes * V::RPW + rl;
+  const int h0 = seg * a.passes * kRows + rl;
+  const T* src = static_cast<const T*>(a.qkv) + tok * heads * kD + sub * N;
 
-  uint4 raw[kAppPasses];
+  uint4 raw[kAppPasses][2];
 #pragma unroll
   for (int p = 0; p < kAppPasses; ++p) {
-    const int h = h0 + p * V::RPW;
-    raw[p] = p < a.passes && h < heads
-                 ? ld_stream(static_cast<const T*>(a.qkv) + (tok * heads + h) * kD + sub * V::N)
-                 : make_uint4(0, 0, 0, 0);
+    const int h = h0 + p * kRows;
+    const bool in = p < a.passes && h < heads;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) raw[p][i] = in ? ld_stream(src + h * kD + i * (kD / 2)) : make_uint4(0, 0, 0, 0);
   }
   const int b = (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
-  const int len = pv.lens[b];
+  const int len = pv.lens[b], start = a.positions ? a.positions[b] : len;
   const bool live = a.counts == nullptr || t < a.counts[b];
   const int64_t slot = (int64_t)len + t;
-  int pos = (a.positions ? a.positions[b] : len) + t;
   int pid = -1;
   const bool fits = len >= 0 && slot < ((int64_t)pv.max_pages << pv.page_shift);
   if (live && fits) pid = pv.table[(int64_t)b * pv.max_pages + (slot >> pv.page_shift)];
   const bool stored = live && fits && pid >= 0 && pid < pv.num_pages;
   bool bad = live && !stored;
-  float c[V::N], s[V::N];
+  float2 c[N / 2], s[N / 2];
   if constexpr (ROT) {
+    int64_t pos = (int64_t)start + t;
     if (pos < 0 || pos >= a.rot_rows) {
       bad = bad || live;
       pos = pos < 0 ? 0 : a.rot_rows - 1;
     }
-    const int j0 = (sub % kHalfT) * V::N;
 #pragma unroll
-    for (int i = 0; i < V::N; i += 4) {
-      const float4 cv = *reinterpret_cast<const float4*>(a.rot_cos + (int64_t)pos * (kD / 2) + j0 + i);
-      const float4 sv = *reinterpret_cast<const float4*>(a.rot_sin + (int64_t)pos * (kD / 2) + j0 + i);
-      c[i] = cv.x; c[i + 1] = cv.y; c[i + 2] = cv.z; c[i + 3] = cv.w;
-      s[i] = sv.x; s[i + 1] = sv.y; s[i + 2] = sv.z; s[i + 3] = sv.w;
+    for (int i = 0; i < N / 2; i += 2) {
+      const float4 cv = __ldg(reinterpret_cast<const float4*>(a.rot_cos + pos * (kD / 2) + sub * N) + i / 2);
+      const float4 sv = __ldg(reinterpret_cast<const float4*>(a.rot_sin + pos * (kD / 2) + sub * N) + i / 2);
+      c[i] = make_float2(cv.x, cv.y); c[i + 1] = make_float2(cv.z, cv.w);
+      s[i] = make_float2(sv.x, sv.y); s[i + 1] = make_float2(sv.z, sv.w);
     }
   }
   if (bad && lane == 0) atomicOr(a.err, DEV_ERR_BAD_PAGE);
@@ -83,39 +86,67 @@ __global__ void __launch_bounds__(kAppThreads) cache_append_kernel(const AppendA
 #pragma unroll
   for (int p = 0; p < kAppPasses; ++p) {
     if (p >= a.passes) break;
-    const int h = h0 + p * V::RPW;
+    const int h = h0 + p * kRows;
     const bool is_v = h >= a.Hq + pv.heads;
-    float x[V::N];
-    unpack<T>(raw[p], x);
+    float x0[N], x1[N];
+    unpack<T>(raw[p][0], x0);
+    unpack<T>(raw[p][1], x1);
+    float2 y[2][N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      y[0][i] = make_float2(x0[2 * i], x0[2 * i + 1]);
+      y[1][i] = make_float2(x1[2 * i], x1[2 * i + 1]);
+    }
     if constexpr (NORM) {
-      float ss = 0.f;
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < V::N; ++i) ss = fmaf(x[i], x[i], ss);
-      ss = row_sum<V::TPR>(ss);
-      const float tau = rsqrtf(ss * (1.0f / kD) + a.eps);
-      const float* g = (h < a.Hq ? a.gain_q : a.gain_k) + sub * V::N;
+      for (int i = 0; i < N / 2; ++i) ss = fma2(y[1][i], y[1][i], fma2(y[0][i], y[0][i], ss));
+      const float sum = row_sum<kLanes>(ss.x + ss.y);
+      const float tau = rsqrtf(sum * (1.0f / kD) + a.eps);
+      const float* g = (h < a.Hq ? a.gain_q : a.gain_k) + sub * N;
 #pragma unroll
-      for (int i = 0; i < V::N; ++i) x[i] = (x[i] * tau) * __ldg(g + i);
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 2) {
+          const float4 gv = __ldg(reinterpret_cast<const float4*>(g + half * (kD / 2)) + i / 2);
+          const float2 tt = make_float2(tau, tau);
+          y[half][i] = mul2(mul2(y[half][i], tt), make_float2(gv.x, gv.y));
+          y[half][i + 1] = mul2(mul2(y[half][i + 1], tt), make_float2(gv.z, gv.w));
+        }
     }
     if constexpr (ROT) {
 #pragma unroll
-      for (int i = 0; i < V::N; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, x[i], kHalfT);
-        x[i] = sub < kHalfT ? x[i] * c[i] - other * s[i] : x[i] * c[i] + other * s[i];
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 u = y[0][i], v = y[1][i], minus = make_float2(-v.x, -v.y);
+        y[0][i] = fma2(u, c[i], mul2(minus, s[i]));
+        y[1][i] = fma2(u, s[i], mul2(v, c[i]));
       }
     }
     if (h >= heads) continue;
-    const uint4 y = is_v ? raw[p] : pack<T>(x);
+    uint4 out[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float z[N];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        z[2 * i] = y[half][i].x;
+        z[2 * i + 1] = y[half][i].y;
+      }
+      out[half] = is_v ? raw[p][half] : pack<T>(z);
+    }
+    T* dst = nullptr;
     if (h < a.Hq) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.q) + (tok * a.Hq + h) * kD + sub * V::N) =
-          live ? y : make_uint4(0, 0, 0, 0);
+      dst = static_cast<T*>(a.q) + (tok * a.Hq + h) * kD;
+      if (!live) out[0] = out[1] = make_uint4(0, 0, 0, 0);
     } else if (stored) {
       const int g = h - a.Hq - (is_v ? pv.heads : 0);
-      T* dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) + paged_row(pv, pid, g, (int)slot) + sub * V::N;
-      *reinterpret_cast<uint4*>(dst) = y;
+      dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) + paged_row(pv, pid, g, (int)slot);
       if (!is_v && sub == 0 && a.slot_positions != nullptr)
-        a.slot_positions[((int64_t)b * pv.heads + g) * ((int64_t)pv.max_pages << pv.page_shift) + slot] =
-            (a.positions ? a.positions[b] : len) + t;
+        a.slot_positions[((int64_t)b * pv.heads + g) * ((int64_t)pv.max_pages << pv.page_shift) + slot] = start + t;
+    }
+    if (dst != nullptr) {
+      *reinterpret_cast<uint4*>(dst + sub * N) = out[0];
+      *reinterpret_cast<uint4*>(dst + kD / 2 + sub * N) = out[1];
     }
   }
 }
@@ -125,7 +156,7 @@ int append_launch(const AppendArgs& a, const PagedView& pv, int64_t blocks, cuda
   const bool norm = a.gain_q != nullptr, rot = a.rot_cos != nullptr;
   auto* kern = norm ? (rot ? cache_append_kernel<T, true, true> : cache_append_kernel<T, true, false>)
                     : (rot ? cache_append_kernel<T, false, true> : cache_append_kernel<T, false, false>);
-  kern<<<(unsigned)blocks, kAppThreads, 0, st>>>(a, pv);
+  ALGX_CUDA(launch_dependent(kern, dim3((unsigned)blocks), dim3(kAppThreads), 0, st, a, pv));
   ALGX_LAUNCHED("cache_append_kernel");
   return ALGX_OK;
 }
@@ -443,7 +474,7 @@ int algx_cache_append(const void* qkv, const float* gain_q, const float* gain_k,
   ALGX_REQUIRE(rope_cos == nullptr || (rope_rows >= 1 && rope_rows <= INT32_MAX), "rotary tables have no rows");
   ALGX_REQUIRE(eps > 0.f, "eps must be positive");
   ALGX_REQUIRE(((((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)rope_cos |
-                  (uintptr_t)rope_sin)) & 15) == 0,
+                  (uintptr_t)rope_sin | (uintptr_t)gain_q | (uintptr_t)gain_k)) & 15) == 0,
                "tensors must be 16-byte aligned");
   const int64_t heads = Hq + 2 * Hkv;
   ALGX_REQUIRE(heads <= 65536 && T <= INT32_MAX && B * T <= INT32_MAX, "too many rows");
@@ -454,12 +485,13 @@ int algx_cache_append(const void* qkv, const float* gain_q, const float* gain_k,
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
   a.tokens = B * T; a.T = (int)T; a.Hq = (int)Hq; a.rot_rows = (int)rope_rows; a.eps = eps;
-  const int rpw = dtype == ALGX_BF16 ? 4 : 2;
+  const int rows = dtype == ALGX_BF16 ? 8 : 4;  // of one group
   // Few rows: one group a warp, so the rows spread over the SMs; from 48 warps
   // an SM on, more groups a warp share the token's lookups.
-  const int64_t groups = (heads + rpw - 1) / rpw * a.tokens;
-  a.passes = (int)std::min<int64_t>(kAppPasses, std::max<int64_t>(1, groups / (148 * 48)));
-  a.segs = (int)((heads + rpw * a.passes - 1) / (rpw * a.passes));
+  const int64_t groups = (heads + rows - 1) / rows;
+  const int64_t most = std::min<int64_t>(kAppPasses, std::max<int64_t>(1, groups * a.tokens / (148 * 48)));
+  a.segs = (int)((groups + most - 1) / most);
+  a.passes = (int)((groups + a.segs - 1) / a.segs);
   const int64_t blocks = (a.tokens * a.segs + kAppThreads / 32 - 1) / (kAppThreads / 32);
   ALGX_REQUIRE(blocks <= INT32_MAX, "too many rows");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
