@@ -68,36 +68,30 @@ __device__ __forceinline__ Span item_span(const PagedAttnArgs& a, int len, int t
   return Span(a.sight, a.shift, r.lo, r.hi);
 }
 // Groups of one kv head of a sequence: all tiles', or those before `tiles`.
-__device__ __forceinline__ int64_t head_groups(const PagedAttnArgs& a, int len, int tiles) {
-  int64_t n = 0;
+__device__ __forceinline__ int head_groups(const PagedAttnArgs& a, int len, int tiles) {
+  int n = 0;
   for (int i = 0; i < tiles; ++i) n += item_span(a, len, i).total;
   return n;
 }
 
-// Groups before sequence `upto` and in all, by the whole block.
+// Groups before sequence `upto` and in all, by the whole block. (The host refuses
+// calls whose line could pass 2^31 groups.)
 struct Line {
-  int64_t before, total, share;
+  int before, total, share;
 };
-__device__ __forceinline__ int64_t warp_sum64(int64_t x) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-  return x;
-}
-__device__ __forceinline__ int64_t share_of(const PagedAttnArgs& a, int64_t total) {
-  const int64_t even = (total + a.warps - 1) / a.warps;
-  const int least = kMinSlots >> a.shift;
-  return even < least ? least : even;
+__device__ __forceinline__ int share_of(const PagedAttnArgs& a, int total) {
+  return max(kMinSlots >> a.shift, (int)(((unsigned)total + a.warps - 1) / (unsigned)a.warps));
 }
 __device__ __forceinline__ Line line_before(const PagedAttnArgs& a, const PagedView& pv, int upto) {
-  __shared__ int64_t s_sum[2][kWarps];
-  int64_t before = 0, total = 0;
+  __shared__ int s_sum[2][kWarps];
+  int before = 0, total = 0;
   for (int b = threadIdx.x; b < a.B; b += kThreads) {
-    const int64_t n = head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
+    const int n = head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
     total += n;
     if (b < upto) before += n;
   }
-  before = warp_sum64(before);
-  total = warp_sum64(total);
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
   if ((threadIdx.x & 31) == 0) {
     s_sum[0][threadIdx.x >> 5] = before;
     s_sum[1][threadIdx.x >> 5] = total;
@@ -120,14 +114,13 @@ struct Cursor {
 
   // The `at`-th group, for a warp; `excl` (kThreads) holds the groups before each
   // thread's run of `run` sequences.
-  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, const int64_t* excl, int run,
-                                    int64_t at) : span(a.sight, a.shift, -1, -1) {
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, const int* excl, int run, int at) : span(a.sight, a.shift, -1, -1) {
     int lo = 0;
     for (int step = kThreads / 2; step > 0; step >>= 1)
       if (excl[lo + step] <= at) lo += step;
     b = lo * run;
     at -= excl[lo];
-    int64_t per;
+    int per;
     for (;;) {
       len = paged_len(pv, b, a.err);
       per = head_groups(a, len, a.tiles);
@@ -135,7 +128,7 @@ struct Cursor {
       at -= per * pv.heads;
       ++b;
     }
-    h = (int)(at / per);
+    h = at / per;
     at -= h * per;
     tile = 0;
     for (;;) {
@@ -144,7 +137,7 @@ struct Cursor {
       at -= span.total;
       ++tile;
     }
-    grp = (int)at;
+    grp = at;
     item = (b * pv.heads + h) * a.tiles + tile;
   }
   __device__ __forceinline__ int slot(const PagedAttnArgs& a) const { return span.group(grp) << a.shift; }
@@ -348,7 +341,7 @@ struct MmaEngine {
   using T = __nv_bfloat16;
   // Groups of 32 slots: copies of 4 KB. Read in 2 KB pieces memory gives a tenth
   // less (6.0 TB/s instead of 6.6 in a bare ring of this form).
-  static constexpr int kSlots = 32, kStages = NT <= 2 ? 2 : 3, kCtas = NT <= 2 ? 3 : 2, kRowBytes = kD * 2;
+  static constexpr int kSlots = 32, kStages = NT <= 3 ? 2 : 3, kCtas = NT <= 3 ? 3 : 2, kRowBytes = kD * 2;
   static constexpr int kSub = NT == 1 ? 2 : 1;  // 16-slot steps worked on together
   static constexpr bool kSwizzle = true;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
@@ -358,6 +351,7 @@ struct MmaEngine {
   // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
   float m[NT][2], o[NT][4][4];
   float2 turn[NT], l[NT];
+  int last[NT][2];  // last slot the column's row sees
 
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedView& pv, const Item& w) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -372,6 +366,8 @@ struct MmaEngine {
       m[nt][0] = m[nt][1] = kNegInf;
       turn[nt].x = turn[nt].y = weight_turn<KIND_, false>(kNegInf);
       l[nt] = make_float2(0.f, 0.f);
+      last[nt][0] = w.last_of(a, nt * 8 + 2 * t);
+      last[nt][1] = w.last_of(a, nt * 8 + 2 * t + 1);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -379,12 +375,12 @@ struct MmaEngine {
     }
   }
   // O^T += V^T P^T for 16 slots. PART: values outside keep0, keep1 (bits of slots
-  // 2 t, 2 t + 1 and 2 t + 8, 2 t + 9) are taken as zero, and only the rows whose
-  // last visible slot is `only` receive the sum.
-  template <bool PART>
-  __device__ __forceinline__ void add_values(const PagedAttnArgs& a, const Item& w, uint32_t v_at,
-                                             const uint32_t (&p)[NT][2], uint32_t keep0, uint32_t keep1, int only) {
-    const int t = threadIdx.x & 3;
+  // 2 t, 2 t + 1 and 2 t + 8, 2 t + 9) are taken as zero. ONLY: of the rows, those
+  // whose last visible slot is `only` receive the sum.
+  enum { WHOLE, PART, ONLY };
+  template <int MODE>
+  __device__ __forceinline__ void add_values(uint32_t v_at, const uint32_t (&p)[NT][2], uint32_t keep0, uint32_t keep1,
+                                             int only) {
     uint32_t b[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -395,22 +391,35 @@ struct MmaEngine {
     for (int j = 0; j < 4; ++j) {
       uint32_t v[4];
       load_matrices_trans(v, v_at ^ (j << 5));
-      if constexpr (PART) {
+      if constexpr (MODE != WHOLE) {
         v[0] &= keep0; v[1] &= keep0; v[2] &= keep1; v[3] &= keep1;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (PART) {
+        if constexpr (MODE == ONLY) {
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
           mma_16816(sum, v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (w.last_of(a, nt * 8 + 2 * t + (i & 1)) == only) o[nt][j][i] += sum[i];
+            if (last[nt][i & 1] == only) o[nt][j][i] += sum[i];
         } else {
           mma_16816(o[nt][j], v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
         }
       }
     }
+  }
+  // Whether a kept value of the 16 slots is an infinity or NaN.
+  __device__ __forceinline__ bool odd_values(uint32_t v_at, uint32_t keep0, uint32_t keep1) const {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t v[4];
+      load_matrices_trans(v, v_at ^ (j << 5));
+      v[0] &= keep0; v[1] &= keep0; v[2] &= keep1; v[3] &= keep1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd = odd || (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+    }
+    return __any_sync(0xffffffffu, odd);
   }
   __device__ __forceinline__ float2 pair(const float (&s)[4], int i) const {
     return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]);
@@ -454,7 +463,7 @@ struct MmaEngine {
         for (int i = 0; i < 4; ++i) {
           s[u][nt][i] *= a.scale;
           const int slot = base + u * 16 + g + (i >> 1) * 8;
-          if (!whole && (slot >= live || !a.sight.sees(slot, w.last_of(a, nt * 8 + 2 * t + (i & 1)))))
+          if (!whole && (slot >= live || !a.sight.sees(slot, last[nt][i & 1])))
             s[u][nt][i] = kNegInf;
         }
     if (a.xs != nullptr) {
@@ -523,20 +532,26 @@ struct MmaEngine {
       }
       const uint32_t vu = v_at + u * 16 * kRowBytes;
       if (whole) {
-        add_values<false>(a, w, vu, pk, 0u, 0u, 0);
+        add_values<WHOLE>(vu, pk, 0u, 0u, 0);
         continue;
       }
-      // Slots that a row does not see hold anything: a weight of zero does not hide
-      // an infinity or NaN in a value, so such a group is added token by token with
-      // the values that the token does not see cleared.
-      for (int last = w.lo; last <= w.hi; ++last) {
-        auto keep = [&](int slot) {
-          return (slot < live && a.sight.sees(slot, last) ? 0xffffu : 0u) |
-                 (slot + 1 < live && a.sight.sees(slot + 1, last) ? 0xffff0000u : 0u);
+      // Slots that a row does not see hold anything, and a weight of zero does not
+      // hide an infinity or NaN in a value: values that no row sees are cleared,
+      // and where one of the others is not finite and the rows' tokens differ in
+      // what they see, the 16 slots are added token by token.
+      const int slot = base + u * 16 + 2 * t;
+      auto keep = [&](int slot, int lo, int hi) {  // seen by some query with lo <= last <= hi
+        auto seen = [&](int s) {
+          return s < live && s <= hi && (a.sight.window == 0 || s > lo - a.sight.window || s < a.sight.first);
         };
-        const int slot = base + u * 16 + 2 * t;
-        add_values<true>(a, w, vu, pk, keep(slot), keep(slot + 8), last);
+        return (seen(slot) ? 0xffffu : 0u) | (seen(slot + 1) ? 0xffff0000u : 0u);
+      };
+      const uint32_t keep0 = keep(slot, w.lo, w.hi), keep1 = keep(slot + 8, w.lo, w.hi);
+      if (w.lo == w.hi || !odd_values(vu, keep0, keep1)) {
+        add_values<PART>(vu, pk, keep0, keep1, 0);
+        continue;
       }
+      for (int l = w.lo; l <= w.hi; ++l) add_values<ONLY>(vu, pk, keep(slot, l, l), keep(slot + 8, l, l), l);
     }
   }
   __device__ __forceinline__ void flush(const Item& w, float2* ml, float* dst) {
@@ -580,8 +595,8 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int4 s_meta[kWarps][kStages];  // item, first slot, live slots
-  __shared__ int64_t s_excl[kThreads];
-  __shared__ int64_t s_warp[kWarps];
+  __shared__ int s_excl[kThreads];
+  __shared__ int s_warp[kWarps];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned char* const ring =
@@ -591,24 +606,29 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
 #pragma unroll
     for (int i = 0; i < kStages; ++i) sm100::mbar_init(&full[i], 1);
     sm100::fence_mbar_init();
-    if (warp == 0) abort_flag = 0;
+    if (warp == 0) {
+      abort_flag = 0;
+      sm100::prefetch_tmap(&k_map);
+      sm100::prefetch_tmap(&v_map);
+    }
   }
+  pdl_wait();
   // the line: every thread counts a run of sequences
   const int run = (a.B + kThreads - 1) / kThreads;
-  int64_t mine = 0;
+  int mine = 0;
   for (int i = 0; i < run; ++i) {
     const int b = threadIdx.x * run + i;
     if (b < a.B) mine += head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
   }
-  int64_t sum = mine;
+  int sum = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, sum, off);
+    const int up = __shfl_up_sync(0xffffffffu, sum, off);
     if (lane >= off) sum += up;
   }
   if (lane == 31) s_warp[warp] = sum;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) {
     if (i < warp) before += s_warp[i];
@@ -616,11 +636,11 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   }
   s_excl[threadIdx.x] = before + sum - mine;
   __syncthreads();
-  const int64_t share = share_of(a, total);
+  const int share = share_of(a, total);
   const int wid = warp * gridDim.x + blockIdx.x;  // neighbours in the line sit on different SMs
-  const int64_t start = wid * share;
-  if (start >= total) return;
-  int left = (int)min(share, total - start), to_issue = left;
+  if ((int64_t)wid * share >= total) return;
+  const int start = wid * share;
+  int left = min(share, total - start), to_issue = left;
 
   Cursor at(a, pv, s_excl, run, start);
   // A group lies in one page, or, with pages of 16 slots and groups of 32, in two.
@@ -714,11 +734,11 @@ struct Parts {
                                    int r) {
     const int tile = r / a.tile_rows;
     row = r - tile * a.tile_rows;
-    const int64_t begin = line.before + h * head_groups(a, len, a.tiles) + head_groups(a, len, tile);
+    const int begin = line.before + h * head_groups(a, len, a.tiles) + head_groups(a, len, tile);
     const int groups = item_span(a, len, tile).total;
-    const int64_t lo = begin / line.share, hi = (begin + groups - 1) / line.share;
+    const int lo = begin / line.share, hi = (begin + groups - 1) / line.share;
     first = lo + ((int64_t)b * pv.heads + h) * a.tiles + tile;
-    count = groups ? (int)(hi - lo) + 1 : 0;
+    count = groups ? hi - lo + 1 : 0;
   }
 };
 
@@ -838,7 +858,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool sc
   if (wide) {  // bf16: tiles of up to 32 rows, as even as they come
     const int64_t tiles = (p.rows + 31) / 32;
     p.tile_rows = ((p.rows + tiles - 1) / tiles + 7) / 8 * 8;
-    ctas = p.tile_rows <= 16 ? 3 : 2;
+    ctas = p.tile_rows <= 24 ? 3 : 2;
   } else {
     p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
   }
@@ -873,7 +893,7 @@ int attn_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
   const uint32_t box = std::min(E::kSlots, 1 << pv.page_shift);
   if (int e = make_tmap_2d(&k, a.k, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
   if (int e = make_tmap_2d(&v, a.v, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
-  kern<<<a.warps / kWarps, kThreads, ring_smem<E>(), st>>>(k, v, a, pv);
+  ALGX_CUDA(launch_dependent(kern, dim3(a.warps / kWarps), dim3(kThreads), ring_smem<E>(), st, k, v, a, pv));
   ALGX_LAUNCHED("paged_attn_kernel");
   return ALGX_OK;
 }
@@ -941,7 +961,7 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   ALGX_REQUIRE(T <= INT32_MAX && T * (Hq / Hkv) <= INT32_MAX / 64, "too many rows");
   const int64_t S = page_size * max_pages;
   const Plan p = make_plan(B, T, Hq, Hkv, S, scores != nullptr, dtype == ALGX_BF16);
-  ALGX_REQUIRE(p.items + p.warps <= INT32_MAX, "too many rows");
+  ALGX_REQUIRE(p.items + p.warps <= INT32_MAX && p.items * ((S + 15) / 16) <= INT32_MAX - p.warps, "too many rows");
   ALGX_REQUIRE(workspace && workspace_bytes >= p.bytes, "workspace too small");
   PagedAttnArgs a = {};
   a.q = q; a.k = k_pages; a.v = v_pages; a.sink = sink; a.scores = scores; a.scores_out = scores_out; a.o = o;
