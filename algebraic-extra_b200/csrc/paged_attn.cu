@@ -74,59 +74,52 @@ __device__ __forceinline__ int head_groups(const PagedAttnArgs& a, int len, int 
   return n;
 }
 
-// Groups before sequence `upto` and in all, by the whole block. (The host refuses
-// calls whose line could pass 2^31 groups.)
+// The line as one warp counts it, 32 sequences at a time: its length, and the
+// groups before sequence `upto`. (The host refuses calls whose line could pass
+// 2^31 groups.)
 struct Line {
   int before, total, share;
+  __device__ __forceinline__ Line(const PagedAttnArgs& a, const PagedView& pv, int upto) {
+    before = total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + (threadIdx.x & 31);
+      const int n = b < a.B ? head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads : 0;
+      total += __reduce_add_sync(0xffffffffu, n);
+      before += __reduce_add_sync(0xffffffffu, b < upto ? n : 0);
+    }
+    share = max(kMinSlots >> a.shift, (int)(((unsigned)total + a.warps - 1) / (unsigned)a.warps));
+  }
 };
-__device__ __forceinline__ int share_of(const PagedAttnArgs& a, int total) {
-  return max(kMinSlots >> a.shift, (int)(((unsigned)total + a.warps - 1) / (unsigned)a.warps));
-}
-__device__ __forceinline__ Line line_before(const PagedAttnArgs& a, const PagedView& pv, int upto) {
-  __shared__ int s_sum[2][kWarps];
-  int before = 0, total = 0;
-  for (int b = threadIdx.x; b < a.B; b += kThreads) {
-    const int n = head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
-    total += n;
-    if (b < upto) before += n;
-  }
-  before = __reduce_add_sync(0xffffffffu, before);
-  total = __reduce_add_sync(0xffffffffu, total);
-  if ((threadIdx.x & 31) == 0) {
-    s_sum[0][threadIdx.x >> 5] = before;
-    s_sum[1][threadIdx.x >> 5] = total;
-  }
-  __syncthreads();
-  Line l = {0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    l.before += s_sum[0][i];
-    l.total += s_sum[1][i];
-  }
-  l.share = share_of(a, l.total);
-  return l;
-}
 
 // A place on the line.
 struct Cursor {
   int b, h, tile, item, grp, len;
   Span span;
 
-  // The `at`-th group, for a warp; `excl` (kThreads) holds the groups before each
-  // thread's run of `run` sequences.
-  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, const int* excl, int run, int at) : span(a.sight, a.shift, -1, -1) {
-    int lo = 0;
-    for (int step = kThreads / 2; step > 0; step >>= 1)
-      if (excl[lo + step] <= at) lo += step;
-    b = lo * run;
-    at -= excl[lo];
-    int per;
-    for (;;) {
-      len = paged_len(pv, b, a.err);
-      per = head_groups(a, len, a.tiles);
-      if (at < per * pv.heads) break;
-      at -= per * pv.heads;
-      ++b;
+  // The `at`-th group, found by the whole warp.
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, int at) : span(a.sight, a.shift, -1, -1) {
+    const int lane = threadIdx.x & 31;
+    int per = 0;
+    for (int b0 = 0;; b0 += 32) {
+      const int mine = b0 + lane < a.B ? paged_len(pv, b0 + lane, a.err) : 0;
+      const int each = b0 + lane < a.B ? head_groups(a, mine, a.tiles) : 0, n = each * pv.heads;
+      int upto = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto > at);
+      if (past == 0) {
+        at -= __shfl_sync(0xffffffffu, upto, 31);
+        continue;
+      }
+      const int src = __ffs(past) - 1;
+      at -= __shfl_sync(0xffffffffu, upto - n, src);
+      per = __shfl_sync(0xffffffffu, each, src);
+      len = __shfl_sync(0xffffffffu, mine, src);
+      b = b0 + src;
+      break;
     }
     h = at / per;
     at -= h * per;
@@ -595,8 +588,6 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int4 s_meta[kWarps][kStages];  // item, first slot, live slots
-  __shared__ int s_excl[kThreads];
-  __shared__ int s_warp[kWarps];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned char* const ring =
@@ -612,37 +603,16 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
       sm100::prefetch_tmap(&v_map);
     }
   }
+  __syncthreads();
   pdl_wait();
-  // the line: every thread counts a run of sequences
-  const int run = (a.B + kThreads - 1) / kThreads;
-  int mine = 0;
-  for (int i = 0; i < run; ++i) {
-    const int b = threadIdx.x * run + i;
-    if (b < a.B) mine += head_groups(a, paged_len(pv, b, a.err), a.tiles) * pv.heads;
-  }
-  int sum = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, sum, off);
-    if (lane >= off) sum += up;
-  }
-  if (lane == 31) s_warp[warp] = sum;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += s_warp[i];
-    total += s_warp[i];
-  }
-  s_excl[threadIdx.x] = before + sum - mine;
-  __syncthreads();
-  const int share = share_of(a, total);
+  const Line line(a, pv, 0);
+  const int share = line.share, total = line.total;
   const int wid = warp * gridDim.x + blockIdx.x;  // neighbours in the line sit on different SMs
   if ((int64_t)wid * share >= total) return;
   const int start = wid * share;
   int left = min(share, total - start), to_issue = left;
 
-  Cursor at(a, pv, s_excl, run, start);
+  Cursor at(a, pv, start);
   // A group lies in one page, or, with pages of 16 slots and groups of 32, in two.
   const int boxes = (1 << pv.page_shift) < E::kSlots ? 2 : 1;
   int2 pid = make_int2(0, 0);
@@ -707,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
       parity ^= 1;
     }
   }
-  pdl_trigger();
+  pdl_trigger();  // not earlier: the join's CTAs would only wait beside this kernel's (34.0 us a pass instead of 33.0)
   e.flush(w, a.part_ml + (int64_t)(wid + item) * a.tile_rows, a.part_o + (int64_t)(wid + item) * a.tile_rows * kD);
   if (left > 0) {  // a copy did not arrive in time: let those on their way land, within limits, before the CTA ends
     volatile int quiet = 0;
@@ -773,24 +743,36 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
   const int h = (int)(bh % pv.heads), b = (int)(bh / pv.heads);
   // lengths and sinks were there before the kernel that this one waits for
   const int len = paged_len(pv, b, a.err);
-  const Line line = line_before(a, pv, b);
+  const Line line(a, pv, b);
   if (which < a.rows) {
     __shared__ float4 s_part[kGroups][kQuads];
     const Parts p(a, pv, line, b, h, len, which);
     const float sink = sink_score(a, h, which);
+    const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
+    auto place = [&](int s) { return (p.first + s) * a.tile_rows + p.row; };
     pdl_wait();
+    constexpr int kAhead = 4;  // parts of a thread loaded before the reference is known
+    float ref[kAhead];
+    float4 x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = grp + i * kGroups;
+      ref[i] = s < p.count ? a.part_ml[place(s)].x : kNegInf;
+      x[i] = s < p.count ? reinterpret_cast<const float4*>(a.part_o)[place(s) * kQuads + quad] : make_float4(0, 0, 0, 0);
+    }
     float turn, L;
     join_row<KIND, EXACT>(a, p, sink, turn, L);
-    const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = grp; s < p.count; s += kGroups) {
-      const int64_t at = (p.first + s) * a.tile_rows + p.row;
-      const float2 ml = a.part_ml[at];
-      const float4 x = reinterpret_cast<const float4*>(a.part_o)[at * kQuads + quad];
-      const float f = ml.x == kNegInf && ml.y == 0.f ? 0.f : weight_of<KIND, EXACT>(ml.x, turn, a.log2n);
-      O.x = fmaf(x.x, f, O.x); O.y = fmaf(x.y, f, O.y); O.z = fmaf(x.z, f, O.z); O.w = fmaf(x.w, f, O.w);
-    }
+    // a part that saw nothing has the reference -inf and zeros; one that saw only
+    // NaN has -inf too, and its sums are NaN, which a factor of zero keeps
+    auto add = [&](float r, const float4& y) {
+      const float f = r == kNegInf ? 0.f : weight_of<KIND, EXACT>(r, turn, a.log2n);
+      O.x = fmaf(y.x, f, O.x); O.y = fmaf(y.y, f, O.y); O.z = fmaf(y.z, f, O.z); O.w = fmaf(y.w, f, O.w);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(ref[i], x[i]);
+    for (int s = grp + kAhead * kGroups; s < p.count; s += kGroups)
+      add(a.part_ml[place(s)].x, reinterpret_cast<const float4*>(a.part_o)[place(s) * kQuads + quad]);
     s_part[grp][quad] = O;
     __syncthreads();
     if (threadIdx.x < kD) {
@@ -806,14 +788,24 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
   constexpr int kEach = kScoreSlots / kThreads;
   __shared__ float s_turn[kRowChunk], s_inv[kRowChunk];
   const int64_t s0 = (int64_t)(which - a.rows) * kScoreSlots + threadIdx.x;
-  float old[kEach], sum[kEach];
+  float old[kEach], sum[kEach], next[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int64_t s = s0 + i * kThreads;
     old[i] = s < len - a.T ? a.scores[bh * a.slots + s] : 0.f;
     sum[i] = 0.f;
   }
+  auto read = [&](int r) {  // the scores of row r, one row ahead of their use
+    const float* x = a.xs + (bh * a.rows + r) * a.slots;
+    const int last = len - a.T + r / a.G;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t s = s0 + i * kThreads;
+      next[i] = r < a.rows && s < len && a.sight.sees((int)s, last) ? x[s] : kNegInf;
+    }
+  };
   pdl_wait();
+  read(0);
   for (int r0 = 0; r0 < a.rows; r0 += kRowChunk) {
     const int nr = min(kRowChunk, a.rows - r0);
     __syncthreads();
@@ -825,17 +817,13 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
     }
     __syncthreads();
     for (int r = 0; r < nr; ++r) {
-      const float* x = a.xs + (bh * a.rows + r0 + r) * a.slots;
-      const int last = len - a.T + (r0 + r) / a.G;
-      float xv[kEach];
+      float x[kEach];
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int64_t s = s0 + i * kThreads;
-        xv[i] = s < len && a.sight.sees((int)s, last) ? x[s] : kNegInf;
-      }
+      for (int i = 0; i < kEach; ++i) x[i] = next[i];
+      read(r0 + r + 1);
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        if (xv[i] != kNegInf) sum[i] += weight_of<KIND, EXACT>(xv[i], s_turn[r], a.log2n) * s_inv[r];
+        if (x[i] != kNegInf) sum[i] += weight_of<KIND, EXACT>(x[i], s_turn[r], a.log2n) * s_inv[r];
     }
   }
 #pragma unroll
