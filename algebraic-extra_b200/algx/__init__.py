@@ -6,8 +6,14 @@ Public API, mirroring the reference's ``algebraic.kernels`` modules:
 * ``algx.kernels.fused_head.fused_head``    (kernels/fused_head.py:260)
 * ``algx.kernels.qk_norm.qk_rms_norm``      (kernels/qk_norm.py:62)
 
-All three are torch ``autograd.Function``s over the C ABI of ``libalgx.so``.
-``algx.torch_ops`` registers the same three families as ``torch.library``
+Serving, which the reference has not:
+
+* ``algx.kernels.paged``   paged key/value cache: append, attention, eviction
+* ``algx.kernels.verify``  verification of drafted tokens, sampling
+* ``algx.serve``           the model over its cache: prompts, decoding, drafts
+
+The first three are torch ``autograd.Function``s over the C ABI of ``libalgx.so``.
+``algx.torch_ops`` registers all of these as ``torch.library``
 operators (``torch.ops.algx.*``) for tracers that need opaque nodes.
 """
 

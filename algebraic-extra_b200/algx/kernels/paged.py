@@ -78,6 +78,12 @@ def _same_device(ref, *tensors):
         L.require_cuda(ref)
 
 
+def _ready(t):
+    """``t`` contiguous at a 16-byte boundary, as the kernels load it (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() & 15 == 0 else t.clone()
+
+
 def _per_sequence(name, t, B):
     if t.shape != (B,) or t.dtype != _I32:
         raise ValueError(f"{name} must be int32 of shape ({B},)")
@@ -115,14 +121,14 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
         for g in (gain_q, gain_k):
             if g.shape != (64,) or g.dtype != _F32:
                 raise ValueError("gains must be float32 of shape (64,)")
-        gain_q, gain_k = gain_q.contiguous(), gain_k.contiguous()
+        gain_q, gain_k = _ready(gain_q), _ready(gain_k)
     if rotary is not None:
         cos, sin = rotary
         rshape = cos.shape
         if len(rshape) != 2 or rshape[1] != 32 or sin.shape != rshape or cos.dtype != _F32 or sin.dtype != _F32 \
                 or rshape[0] < 1:
             raise ValueError("rotary tables must both be float32 of shape (rows, 32)")
-        cos, sin = cos.contiguous(), sin.contiguous()
+        cos, sin = _ready(cos), _ready(sin)
         rows = rshape[0]
     if positions is not None:
         positions = _per_sequence("positions", positions, B)
@@ -131,7 +137,7 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
     if slot_positions is not None:
         _check_state("slot_positions", slot_positions, (B, Hkv, maxp * size), _I32)
     _same_device(qkv, k_pages, v_pages, table, lens, gain_q, gain_k, cos, sin, positions, counts, slot_positions)
-    qkv, table, lens = qkv.contiguous(), table.contiguous(), lens.contiguous()
+    qkv, table, lens = _ready(qkv), table.contiguous(), lens.contiguous()
     T, Hq = shape[1], shape[2] - 2 * Hkv
     q = qkv.new_empty((B, T, Hq, 64))
     L.check(L.lib().algx_cache_append(
@@ -207,7 +213,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
     elif scores_out is not None:
         raise ValueError("scores_out without scores")
     _same_device(q, k_pages, v_pages, table, lens, scores, scores_out)
-    q, table, lens = q.contiguous(), table.contiguous(), lens.contiguous()
+    q, table, lens = _ready(q), table.contiguous(), lens.contiguous()
     o = torch.empty_like(q)
     nbytes = _attn_workspace(B, T, Hq, Hkv, size, maxp, scores is not None, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)

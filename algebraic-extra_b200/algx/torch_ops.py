@@ -8,12 +8,18 @@ backward wired through ``torch.library.register_autograd``:
 * ``algx::flash_attention_fwd`` / ``algx::flash_attention_bwd``
 * ``algx::fused_head_fwd`` / ``algx::fused_head_bwd``
 
+and the serving operators, which have no backward:
+
+* ``algx::cache_append``, ``algx::paged_attention``, ``algx::paged_attention_scored``,
+  ``algx::cache_evict`` (the cache's tensors are mutated arguments)
+* ``algx::verify_draft``
+
 To a tracer (``torch.compile``, ``torch.export``, CUDA-graph capture tools)
 each call is one opaque node with known output shapes, where the
 ``autograd.Function`` wrappers of ``algx.kernels`` would be traced through.
 The public functions below take the same arguments, raise the same errors
-and return the same values as ``algx.kernels.{qk_norm,flash,fused_head}``,
-which mirror the reference's kernels/qk_norm.py:62, kernels/flash.py:763 and
+and return the same values as ``algx.kernels.{qk_norm,flash,fused_head,paged,verify}``,
+the first three of which mirror the reference's kernels/qk_norm.py:62, kernels/flash.py:763 and
 kernels/fused_head.py:260.
 """
 
@@ -27,7 +33,9 @@ from torch import Tensor
 from . import _lib as L
 from .kernels import flash as F
 from .kernels import fused_head as FH
+from .kernels import paged as P
 from .kernels import qk_norm as Q
+from .kernels import verify as VD
 
 
 # ------------------------------------------------------------------ QK norm
@@ -264,3 +272,102 @@ def fused_head(h, embed, targets, *, kind="ce", n=16, c=16.0, block_n=128, block
     ints, floats = _head_lists(kind, n, c, embed.shape[0], ignore_index)
     obj, tel, _, _ = _head_fwd_op(h, embed, targets, ints, floats)
     return obj, tel.detach()
+
+
+# ------------------------------------------------------------------ serving
+@torch.library.custom_op("algx::cache_append", mutates_args=("k_pages", "v_pages", "slot_positions"))
+def _cache_append_op(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lens: Tensor,
+                     gain_q: Optional[Tensor], gain_k: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor],
+                     positions: Optional[Tensor], counts: Optional[Tensor], slot_positions: Optional[Tensor],
+                     eps: float) -> Tensor:
+    return P.cache_append(qkv, k_pages, v_pages, table, lens, gain_q, gain_k,
+                          rotary=None if cos is None else (cos, sin), positions=positions, counts=counts,
+                          slot_positions=slot_positions, eps=eps)
+
+
+@_cache_append_op.register_fake
+def _(qkv, k_pages, v_pages, table, lens, gain_q, gain_k, cos, sin, positions, counts, slot_positions, eps):
+    B, T, heads, D = qkv.shape
+    return qkv.new_empty((B, T, heads - 2 * k_pages.shape[1], D))
+
+
+def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *, rotary=None, positions=None,
+                 counts=None, slot_positions=None, eps: float = 1e-5):
+    """``algx.kernels.paged.cache_append`` as one ``algx::cache_append`` node."""
+    cos, sin = (None, None) if rotary is None else rotary
+    return _cache_append_op(qkv, k_pages, v_pages, table, lens, gain_q, gain_k, cos, sin, positions, counts,
+                            slot_positions, float(eps))
+
+
+@torch.library.custom_op("algx::paged_attention", mutates_args=())
+def _paged_attention_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lens: Tensor,
+                        sink: Optional[Tensor], kind: str, n: int, c: float, window: int, first: int) -> Tensor:
+    return P.paged_attention(q, k_pages, v_pages, table, lens, sink, kind=kind, n=n, c=c, window=window or None,
+                             first=first)
+
+
+@_paged_attention_op.register_fake
+def _(q, k_pages, v_pages, table, lens, sink, kind, n, c, window, first):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("algx::paged_attention_scored", mutates_args=("scores",))
+def _paged_attention_scored_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lens: Tensor,
+                               sink: Optional[Tensor], scores: Tensor, kind: str, n: int, c: float, window: int,
+                               first: int) -> Tensor:
+    return P.paged_attention(q, k_pages, v_pages, table, lens, sink, kind=kind, n=n, c=c, window=window or None,
+                             first=first, scores=scores)[0]
+
+
+@_paged_attention_scored_op.register_fake
+def _(q, k_pages, v_pages, table, lens, sink, scores, kind, n, c, window, first):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: str = "softmax", n: int = 16,
+                    c: float = 16.0, window: Optional[int] = None, first: int = 0, scores=None):
+    """``algx.kernels.paged.paged_attention`` as one node; ``scores`` is updated in place and returned beside o."""
+    P.paged_config(kind, n, c, window, first)
+    args = (q, k_pages, v_pages, table, lens, sink_logit)
+    if scores is None:
+        return _paged_attention_op(*args, kind, n, float(c), window or 0, first)
+    return _paged_attention_scored_op(*args, scores, kind, n, float(c), window or 0, first), scores
+
+
+@torch.library.custom_op("algx::cache_evict", mutates_args=("k_pages", "v_pages"))
+def _cache_evict_op(k_pages: Tensor, v_pages: Tensor, table: Tensor, lens: Tensor, scores: Tensor, positions: Tensor,
+                    budget: int, first: int, recent: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    return P.cache_evict(k_pages, v_pages, table, lens, scores, positions, budget=budget, first=first, recent=recent)
+
+
+@_cache_evict_op.register_fake
+def _(k_pages, v_pages, table, lens, scores, positions, budget, first, recent):
+    B, H, _ = scores.shape
+    return (torch.empty_like(lens), torch.empty_like(scores), torch.empty_like(positions),
+            positions.new_empty((B, H, budget)))
+
+
+def cache_evict(k_pages, v_pages, table, lens, scores, positions, *, budget: int, first: int = 0, recent: int = 0):
+    """``algx.kernels.paged.cache_evict`` as one ``algx::cache_evict`` node."""
+    return _cache_evict_op(k_pages, v_pages, table, lens, scores, positions, budget, first, recent)
+
+
+@torch.library.custom_op("algx::verify_draft", mutates_args=())
+def _verify_draft_op(target_logits: Tensor, draft_tokens: Tensor, draft_logits: Optional[Tensor], accept_u: Tensor,
+                     race: Tensor, counts: Optional[Tensor], kind: str, n: int, c: float,
+                     temperature: float) -> Tuple[Tensor, Tensor]:
+    return VD.verify_draft(target_logits, draft_tokens, draft_logits, accept_u, race, kind=kind, n=n, c=c,
+                           temperature=temperature, counts=counts)
+
+
+@_verify_draft_op.register_fake
+def _(target_logits, draft_tokens, draft_logits, accept_u, race, counts, kind, n, c, temperature):
+    B, rows, _ = target_logits.shape
+    return draft_tokens.new_empty((B, rows)), draft_tokens.new_empty((B,))
+
+
+def verify_draft(target_logits, draft_tokens, draft_logits, accept_u, race, *, kind: str = "ce", n: int = 16,
+                 c: float = 16.0, temperature: float = 1.0, counts=None):
+    """``algx.kernels.verify.verify_draft`` as one ``algx::verify_draft`` node."""
+    return _verify_draft_op(target_logits, draft_tokens, draft_logits, accept_u, race, counts, kind, n, float(c),
+                            float(temperature))

@@ -418,7 +418,6 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   if (B == 0) return ALGX_OK;
   ALGX_REQUIRE(B <= INT32_MAX / 16, "too many sequences");
   ALGX_REQUIRE(target && race && out && accepted && (K == 0 || (tokens && u)), "NULL tensor");
-  ALGX_REQUIRE((((uintptr_t)target | (uintptr_t)draft) & 3) == 0, "logits must be 4-byte aligned");
   VerifyArgs a = {};
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
   a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;

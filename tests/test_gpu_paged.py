@@ -338,3 +338,42 @@ def test_evict_of_no_sequences():
     out = cache_evict(k.cuda(), v.cuda(), table, table[:, 0], torch.empty((0, 2, 32), device="cuda"),
                       torch.empty((0, 2, 32), dtype=torch.int32, device="cuda"), budget=4)
     assert [tuple(t.shape) for t in out] == [(0,), (0, 2, 32), (0, 2, 32), (0, 2, 4)]
+
+
+def test_operators_match_the_functions():
+    from algx import torch_ops as T
+    k, v, table, g = make_cache(2, 2, 32, 4, BF16, 70)
+    qkv = torch.randn((2, 3, 8, 64), generator=g).to(BF16).cuda()
+    lens = torch.tensor([60, 5], dtype=torch.int32).cuda()
+    gains = [torch.rand(64, generator=g).cuda() for _ in range(2)]
+    table = table.cuda()
+    caches = [(k.cuda(), v.cuda()) for _ in range(2)]
+    qs = [f(qkv, *c, table, lens, *gains) for f, c in zip((cache_append, T.cache_append), caches)]
+    assert torch.equal(*qs) and all(torch.equal(a, b) for a, b in zip(*caches))
+    after = lens + 3
+    scores = [torch.rand((2, 2, 128), generator=torch.Generator().manual_seed(1)).cuda() for _ in range(2)]
+    a = paged_attention(qs[0], *caches[0], table, after, kind="asinh", c=8.0, scores=scores[0])
+    b = T.paged_attention(qs[0], *caches[1], table, after, kind="asinh", c=8.0, scores=scores[1])
+    assert torch.equal(a[0], b[0]) and torch.equal(scores[0], scores[1])
+    assert torch.equal(paged_attention(qs[0], *caches[0], table, after, window=9),
+                       T.paged_attention(qs[0], *caches[0], table, after, window=9))
+    pos = torch.arange(128, dtype=torch.int32).expand(2, 2, 128).contiguous().cuda()
+    outs = [f(*c, table, after, scores[0], pos, budget=20, recent=4) for f, c in
+            zip((cache_evict, T.cache_evict), caches)]
+    assert all(torch.equal(x, y) for x, y in zip(*outs)) and all(torch.equal(x, y) for x, y in zip(*caches))
+
+
+def test_unaligned_inputs_are_copied():
+    k, v, table, g = make_cache(1, 2, 16, 2, BF16, 71)
+    base = torch.randn(1 + 6 * 64, generator=g).to(BF16).cuda()
+    qkv = base[1:].view(1, 1, 6, 64)
+    gains = torch.rand(130, generator=g).cuda()
+    lens = torch.tensor([3], dtype=torch.int32).cuda()
+    caches = [(k.cuda(), v.cuda()) for _ in range(2)]
+    a = cache_append(qkv, *caches[0], table.cuda(), lens, gains[1:65], gains[65:129])
+    b = cache_append(qkv.clone(), *caches[1], table.cuda(), lens, gains[1:65].clone(), gains[65:129].clone())
+    assert torch.equal(a, b) and torch.equal(caches[0][0], caches[1][0])
+    odd = torch.empty(1 + a.numel(), dtype=BF16, device="cuda")[1:].view(a.shape)
+    odd.copy_(a)
+    assert torch.equal(paged_attention(odd, *caches[0], table.cuda(), lens + 1),
+                       paged_attention(a, *caches[0], table.cuda(), lens + 1))
