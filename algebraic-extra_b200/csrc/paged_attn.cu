@@ -297,8 +297,9 @@ struct FmaEngine {
 // the independence of the warps, which hides the latency of one group's chain
 // (products, weights, products) behind those of the others.
 //
-// Weights are rounded to bf16 for the second product, as the forward kernels
-// round them (kernels/flash.py:262), while their sum keeps the unrounded ones.
+// Weights go into the second product as two bf16 parts each. One part, as the
+// training kernels round them (kernels/flash.py:262), adds 1.6e-3 to the output's
+// relative error of 1.7e-3; the second product's time does not show.
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -310,11 +311,14 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// A pair of floats as the sum of two bf16 pairs (16 bits of each).
+__device__ __forceinline__ void split_pair(float2 x, uint32_t& high, uint32_t& low) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+  const float2 r = sub2(x, __bfloat1622float2(h));
+  const __nv_bfloat162 l = __floats2bfloat162_rn(r.x, r.y);
+  high = *reinterpret_cast<const uint32_t*>(&h);
+  low = *reinterpret_cast<const uint32_t*>(&l);
 }
-
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -372,14 +376,13 @@ struct MmaEngine {
   // whose last visible slot is `only` receive the sum.
   enum { WHOLE, PART, ONLY };
   template <int MODE>
-  __device__ __forceinline__ void add_values(uint32_t v_at, const uint32_t (&p)[NT][2], uint32_t keep0, uint32_t keep1,
+  __device__ __forceinline__ void add_values(uint32_t v_at, const uint32_t (&p)[NT][4], uint32_t keep0, uint32_t keep1,
                                              int only) {
-    uint32_t b[NT][2];
+    uint32_t b[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      b[nt][0] = transpose_8x8(p[nt][0]);
-      b[nt][1] = transpose_8x8(p[nt][1]);
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[nt][i] = transpose_8x8(p[nt][i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t v[4];
@@ -392,11 +395,13 @@ struct MmaEngine {
         if constexpr (MODE == ONLY) {
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
           mma_16816(sum, v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
+          mma_16816(sum, v[0], v[1], v[2], v[3], b[nt][2], b[nt][3]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (last[nt][i & 1] == only) o[nt][j][i] += sum[i];
         } else {
           mma_16816(o[nt][j], v[0], v[1], v[2], v[3], b[nt][0], b[nt][1]);
+          mma_16816(o[nt][j], v[0], v[1], v[2], v[3], b[nt][2], b[nt][3]);
         }
       }
     }
@@ -514,14 +519,14 @@ struct MmaEngine {
     }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      uint32_t pk[NT][2];
+      uint32_t pk[NT][4];  // slots g and g + 8: high parts, low parts
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) l[nt] = add2(l[nt], p[u][nt][i]);
         const float2 x = p[u][nt][0], y = p[u][nt][NP - 1];
-        pk[nt][0] = ONE ? pack_pair(x.x, 0.f) : pack_pair(x.x, x.y);
-        pk[nt][1] = ONE ? pack_pair(x.y, 0.f) : pack_pair(y.x, y.y);
+        split_pair(ONE ? make_float2(x.x, 0.f) : x, pk[nt][0], pk[nt][2]);
+        split_pair(ONE ? make_float2(x.y, 0.f) : y, pk[nt][1], pk[nt][3]);
       }
       const uint32_t vu = v_at + u * 16 * kRowBytes;
       if (whole) {
