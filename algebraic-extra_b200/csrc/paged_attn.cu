@@ -175,8 +175,8 @@ struct Item {
   __device__ __forceinline__ int last_of(const PagedAttnArgs& a, int r) const { return len - a.T + (r0 + r) / a.G; }
 };
 
-// Weights are relative to a per-row reference that moves only when a weight
-// passes 2^8, so most groups need no reduction over lanes at all.
+// Weights are relative to a per-row reference that moves only when a weight (or the
+// sum of a few) passes 2^8, so most groups need no reduction over lanes at all.
 constexpr float kMove = 256.f;
 
 // ------------------------------------------------------- float32, FMA units
@@ -338,7 +338,7 @@ struct MmaEngine {
   using T = __nv_bfloat16;
   // Groups of 32 slots: copies of 4 KB. Read in 2 KB pieces memory gives a tenth
   // less (6.0 TB/s instead of 6.6 in a bare ring of this form).
-  static constexpr int kSlots = 32, kStages = NT <= 3 ? 2 : 3, kCtas = NT <= 3 ? 3 : 2, kRowBytes = kD * 2;
+  static constexpr int kSlots = 32, kStages = NT <= 2 ? 2 : 3, kCtas = NT <= 2 ? 3 : 2, kRowBytes = kD * 2;
   static constexpr int kSub = NT == 1 ? 2 : 1;  // 16-slot steps worked on together
   static constexpr bool kSwizzle = true;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
@@ -347,7 +347,7 @@ struct MmaEngine {
   uint32_t q[NT][8];
   // the lane's two columns of every tile are rows 8 nt + 2 t and + 1
   float m[NT][2], o[NT][4][4];
-  float2 turn[NT], l[NT];
+  float2 turn[NT], l[NT];  // turn: of weight_scaled
   int last[NT][2];  // last slot the column's row sees
 
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const PagedView& pv, const Item& w) {
@@ -361,7 +361,7 @@ struct MmaEngine {
 #pragma unroll
       for (int i = 0; i < 8; ++i) q[nt][i] = r < w.nr ? row[i * 4] : 0u;
       m[nt][0] = m[nt][1] = kNegInf;
-      turn[nt].x = turn[nt].y = weight_turn<KIND_, false>(kNegInf);
+      turn[nt].x = turn[nt].y = signed_turn(weight_turn<KIND_, false>(kNegInf));
       l[nt] = make_float2(0.f, 0.f);
       last[nt][0] = w.last_of(a, nt * 8 + 2 * t);
       last[nt][1] = w.last_of(a, nt * 8 + 2 * t + 1);
@@ -422,12 +422,13 @@ struct MmaEngine {
   __device__ __forceinline__ float2 pair(const float (&s)[4], int i) const {
     return ONE ? make_float2(s[0], s[2]) : make_float2(s[2 * i], s[2 * i + 1]);
   }
+  static __device__ __forceinline__ float signed_turn(float t) { return KIND_ == kSoftmax ? -t : t; }
   __device__ __forceinline__ float2 turns(int nt) const { return ONE ? make_float2(turn[nt].x, turn[nt].x) : turn[nt]; }
 
   __device__ __forceinline__ void compute(const PagedAttnArgs& a, const PagedView& pv, const Item& w,
                                           const unsigned char* group, int base, int live) {
     const bool whole = base + kSlots <= live && a.sight.sees_all(base, kSlots, w.lo, w.hi);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kSlots / 16; i += kSub) step(a, pv, w, sm100::smem_u32(group) + i * 16 * kRowBytes, base + i * 16, live, whole);
   }
   __device__ __forceinline__ void step(const PagedAttnArgs& a, const PagedView& pv, const Item& w, uint32_t at, int base,
@@ -459,7 +460,6 @@ struct MmaEngine {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[u][nt][i] *= a.scale;
           const int slot = base + u * 16 + g + (i >> 1) * 8;
           if (!whole && (slot >= live || !a.sight.sees(slot, last[nt][i & 1])))
             s[u][nt][i] = kNegInf;
@@ -472,20 +472,26 @@ struct MmaEngine {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = nt * 8 + 2 * t + (i & 1), slot = base + u * 16 + g + (i >> 1) * 8;
-            if (r < w.nr && slot < a.slots) w.x_row(a, pv, r)[slot] = s[u][nt][i];
+            if (r < w.nr && slot < a.slots) w.x_row(a, pv, r)[slot] = s[u][nt][i] * a.scale;
           }
     }
-    float2 p[kSub][NT][NP];
-    float high = 0.f;
+    float2 p[kSub][NT][NP], inc[NT];
+    const float2 scale = make_float2(a.scale, a.scale);
+    auto weigh = [&](int nt) {
 #pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          p[u][nt][i] = weight_pair<KIND_, LOG2N>(pair(s[u][nt], i), turns(nt), a.log2n);
-          high = fmaxf(high, fmaxf(p[u][nt][i].x, p[u][nt][i].y));
+          p[u][nt][i] = weight_scaled<KIND_, LOG2N>(pair(s[u][nt], i), scale, turns(nt), a.log2n);
+          inc[nt] = u + i ? add2(inc[nt], p[u][nt][i]) : p[u][nt][i];
         }
+    };
+    float high = 0.f;  // a weight above kMove shows in its sum
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      weigh(nt);
+      high = fmaxf(high, fmaxf(inc[nt].x, inc[nt].y));
+    }
     if (__any_sync(0xffffffffu, high > kMove)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -496,11 +502,12 @@ struct MmaEngine {
           for (int u = 0; u < kSub; ++u) top = fmaxf(top, fmaxf(s[u][nt][c], s[u][nt][c + 2]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          top *= a.scale;
           if (top > m[nt][c]) {
             const float to = weight_turn<KIND_, false>(top);
             const float f = m[nt][c] == kNegInf ? 0.f : weight_of<KIND_, false>(m[nt][c], to, a.log2n);
             m[nt][c] = top;
-            (c ? turn[nt].y : turn[nt].x) = to;
+            (c ? turn[nt].y : turn[nt].x) = signed_turn(to);
             (c ? l[nt].y : l[nt].x) *= f;
             if (ONE) l[nt].y *= f;
 #pragma unroll
@@ -510,20 +517,16 @@ struct MmaEngine {
             }
           }
         }
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int i = 0; i < NP; ++i)
-            p[u][nt][i] = weight_pair<KIND_, LOG2N>(pair(s[u][nt], i), turns(nt), a.log2n);
+        weigh(nt);
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) l[nt] = add2(l[nt], inc[nt]);
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       uint32_t pk[NT][4];  // slots g and g + 8: high parts, low parts
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) l[nt] = add2(l[nt], p[u][nt][i]);
         const float2 x = p[u][nt][0], y = p[u][nt][NP - 1];
         split_pair(ONE ? make_float2(x.x, 0.f) : x, pk[nt][0], pk[nt][2]);
         split_pair(ONE ? make_float2(x.y, 0.f) : y, pk[nt][1], pk[nt][3]);
@@ -851,7 +854,7 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool sc
   if (wide) {  // bf16: tiles of up to 32 rows, as even as they come
     const int64_t tiles = (p.rows + 31) / 32;
     p.tile_rows = ((p.rows + tiles - 1) / tiles + 7) / 8 * 8;
-    ctas = p.tile_rows <= 24 ? 3 : 2;
+    ctas = p.tile_rows <= 16 ? 3 : 2;
   } else {
     p.tile_rows = p.rows <= 1 ? 1 : p.rows <= 2 ? 2 : p.rows <= 4 ? 4 : 8;
   }

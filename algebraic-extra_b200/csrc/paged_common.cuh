@@ -119,6 +119,19 @@ __device__ __forceinline__ float2 weight_pair(float2 x, float2 turn, int log2n) 
   }
 }
 
+// weight_pair of the scores scale x; softmax takes the negative reference, -m.
+template <int KIND, int LOG2N>
+__device__ __forceinline__ float2 weight_scaled(float2 x, float2 scale, float2 turn, int log2n) {
+  if constexpr (KIND == kSoftmax) {
+    float2 y = fma2(x, scale, turn);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(y.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(y.y));
+    return y;
+  } else {
+    return weight_pair<KIND, LOG2N>(mul2(x, scale), turn, log2n);
+  }
+}
+
 // Which slots a query sees. Query token t of T new ones stands at slot
 // last = len - T + t and sees slots s <= last with s > last - window or
 // s < first (window 0: no window).
