@@ -117,22 +117,24 @@ __device__ __forceinline__ uint64_t pack_best(float value, int64_t v) {
   return ((uint64_t)__float_as_uint(value) << 32) | (uint32_t)~(uint32_t)v;
 }
 
-// Columns [begin, end) of a row in blocks of kUnroll 16-byte vectors a lane: the
-// aligned middle, and up to 2 (N - 1) single columns at the ends, which go with
+// Columns [begin, end) of a row: 16-byte vectors in the aligned middle, counted in
+// blocks of kBlock, and up to 2 (N - 1) single columns at the ends, which go with
 // the first block.
-template <typename T, int kUnroll>
+constexpr int kBlock = 64;
+template <typename T>
 struct Columns {
-  static constexpr int N = Vec<T>::N, kBlock = 32 * kUnroll;  // vectors of a block
+  static constexpr int N = Vec<T>::N;
   const T* row;
-  int64_t begin, end, mid, vecs;
+  int64_t begin, end, mid;
+  int vecs;
   __device__ __forceinline__ Columns(const T* r, int64_t b, int64_t e) : row(r), begin(b), end(e) {
     const uintptr_t addr = reinterpret_cast<uintptr_t>(r + b);
     mid = min(e, b + (int64_t)(((16 - (addr & 15)) & 15) / sizeof(T)));
-    vecs = (e - mid) / N;
+    vecs = (int)((e - mid) / N);
   }
-  __device__ __forceinline__ int ends() const { return (int)((mid - begin) + (end - mid - vecs * N)); }
+  __device__ __forceinline__ int ends() const { return (int)((mid - begin) + (end - mid - (int64_t)vecs * N)); }
   __device__ __forceinline__ int64_t end_column(int i) const {
-    return i < mid - begin ? begin + i : mid + vecs * N + (i - (mid - begin));
+    return i < mid - begin ? begin + i : mid + (int64_t)vecs * N + (i - (mid - begin));
   }
 };
 
@@ -140,8 +142,9 @@ template <typename T, int KIND, int LOG2N, int kCluster, int kThreads>
 __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads) verify_kernel(const VerifyArgs a) {
   using V = Vec<T>;
   constexpr int kWarps = kThreads / 32;
-  constexpr int kUnroll = kCluster == 16 ? 8 : 4;  // 16-byte loads of a lane on their way together
-  using Cols = Columns<T, kUnroll>;
+  // 16-byte loads of a lane on their way while as many are worked on
+  constexpr int kFly = kCluster == 16 ? 4 : 2;
+  using Cols = Columns<T>;
   __shared__ float2 s_part[kWarps + kMaxRows];  // (reference, sum) of every (warp, row) that meets, at warp + row
   __shared__ float2 s_row[2][kMaxRows];         // this CTA's (reference, sum) of every row, for two rounds
   __shared__ float s_turn[kMaxRows], s_l[kMaxRows];
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
     const float x = score_of<KIND>(a, z);
     return x > kNegInf ? exact_weight<KIND>(a, x, s_turn[r]) / s_l[r] : 0.f;
   };
-  const int blocks = (int)max((int64_t)1, (end - begin + V::N * Cols::kBlock - 1) / (V::N * Cols::kBlock));
+  const int blocks = (int)max((int64_t)1, (end - begin + V::N * kBlock - 1) / (V::N * kBlock));
 
   // Rounds of a.round positions, up to the first refusal: rows after it are not
   // needed. Row r of a round is target row i0 + r, then draft row i0 + (r - nt).
@@ -209,22 +212,30 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
       const int r = at / blocks;
       const Cols c(r < nt ? target + (int64_t)(i0 + r) * a.V : draft + (int64_t)(i0 + r - nt) * a.V, begin, end);
       const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
-      const int vecs = (int)c.vecs;
       RowSum<KIND, LOG2N> sum;
       sum.clear();
       if (at == r * blocks && lane < c.ends()) {
         const float z[1] = {to_f32(c.row[c.end_column(lane)])};
         sum.add(a, z);
       }
-      for (; at < stop && at < (r + 1) * blocks; ++at) {
-        const int v0 = (at - r * blocks) * Cols::kBlock + lane;
-        uint4 raw[kUnroll];
+      const int to = min(stop, (r + 1) * blocks);
+      int v = (at - r * blocks) * kBlock + lane;
+      const int v_end = min(c.vecs, (to - r * blocks) * kBlock);
+      at = to;
+      uint4 next[kFly];
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i)
-          if (v0 + i * 32 < vecs) raw[i] = __ldg(mid + v0 + i * 32);
+      for (int i = 0; i < kFly; ++i)
+        if (v + i * 32 < v_end) next[i] = __ldg(mid + v + i * 32);
+      for (; v < v_end; v += 32 * kFly) {
+        uint4 raw[kFly];
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i)
-          if (v0 + i * 32 < vecs) {
+        for (int i = 0; i < kFly; ++i) {
+          raw[i] = next[i];
+          if (v + (i + kFly) * 32 < v_end) next[i] = __ldg(mid + v + (i + kFly) * 32);
+        }
+#pragma unroll
+        for (int i = 0; i < kFly; ++i)
+          if (v + i * 32 < v_end) {
             float z[V::N];
             unpack<T>(raw[i], z);
             sum.add(a, z);
@@ -320,22 +331,32 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
     const bool vec = ((reinterpret_cast<uintptr_t>(race + c.mid) & 15) == 0) &&
                      (!rest || (reinterpret_cast<uintptr_t>(row_q + c.mid) & 15) == 0);
     if (vec) {
-#pragma unroll 2
-      for (int64_t i = threadIdx.x; i < c.vecs; i += kThreads) {
-        const int64_t v = c.mid + i * V::N;
-        float z[V::N], zd[V::N], e[V::N];
-        unpack<T>(__ldg(reinterpret_cast<const uint4*>(row_p + v)), z);
-        if (rest) unpack<T>(__ldg(reinterpret_cast<const uint4*>(row_q + v)), zd);
+      struct Three {
+        uint4 p, q;
+        float4 e[V::N / 4];
+      };
+      auto load = [&](Three& x, int i) {
+        if (i >= c.vecs) return;
+        const int64_t v = c.mid + (int64_t)i * V::N;
+        x.p = __ldg(reinterpret_cast<const uint4*>(row_p + v));
+        if (rest) x.q = __ldg(reinterpret_cast<const uint4*>(row_q + v));
 #pragma unroll
-        for (int j = 0; j < V::N; j += 4) {
-          const float4 x = __ldg(reinterpret_cast<const float4*>(race + v + j));
-          e[j] = x.x; e[j + 1] = x.y; e[j + 2] = x.z; e[j + 3] = x.w;
-        }
+        for (int j = 0; j < V::N / 4; ++j) x.e[j] = __ldg(reinterpret_cast<const float4*>(race + v) + j);
+      };
+      Three next;
+      load(next, threadIdx.x);
+      for (int i = threadIdx.x; i < c.vecs; i += kThreads) {
+        const Three x = next;
+        load(next, i + kThreads);
+        float z[V::N], zd[V::N];
+        unpack<T>(x.p, z);
+        if (rest) unpack<T>(x.q, zd);
+        const float* e = reinterpret_cast<const float*>(x.e);
 #pragma unroll
-        for (int j = 0; j < V::N; ++j) enter(v + j, z[j], rest ? zd[j] : kNegInf, e[j]);
+        for (int j = 0; j < V::N; ++j) enter(c.mid + (int64_t)i * V::N + j, z[j], rest ? zd[j] : kNegInf, e[j]);
       }
     } else {
-      for (int64_t v = c.mid + threadIdx.x; v < c.mid + c.vecs * V::N; v += kThreads)
+      for (int64_t v = c.mid + threadIdx.x; v < c.mid + (int64_t)c.vecs * V::N; v += kThreads)
         enter(v, to_f32(row_p[v]), rest ? to_f32(row_q[v]) : kNegInf, race[v]);
     }
     float sure = low;
@@ -427,12 +448,12 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Few sequences: all rows in one round, whose time is latency, over as many SMs
-  // as a cluster spans. Where the clusters fill the device, three positions a
+  // as a cluster spans. Where the clusters fill the device, four positions a
   // round, as rows behind a refusal are mostly not read, and smaller CTAs, four
   // an SM, which leave less of a last wave.
   const bool few = B * 16 <= 148, wide = B * 8 <= 2 * 148;
   const int64_t cluster = few ? 16 : 8;
-  a.round = wide ? (int)K + 1 : 3;
+  a.round = wide ? (int)K + 1 : 4;
   a.slice = ((V + cluster - 1) / cluster + 7) / 8 * 8;
   return few    ? verify_launch<16, 512>(a, kind, dtype, B, st)
          : wide ? verify_launch<8, 512>(a, kind, dtype, B, st)
