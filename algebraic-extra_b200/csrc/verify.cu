@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_common.cuh"
 #include "vec_io.cuh"
@@ -85,31 +86,40 @@ struct RowSum {
     turn = weight_turn<KIND, true>(kNegInf);
     l = make_float2(0.f, 0.f);
   }
-  template <int N>
+  // CLEAN: NaN logits count as -inf. Without it one spoils the sum, which then is
+  // taken again with it.
+  template <bool CLEAN, int N>
   __device__ __forceinline__ void add(const VerifyArgs& a, const float (&z)[N]) {
-    float2 x[(N + 1) / 2], w[(N + 1) / 2];
-    float high = 0.f;
+    constexpr int P = (N + 1) / 2;
+    float2 x[P], w[P];
+    auto weigh = [&]() {
+      float2 sum;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      x[i / 2] = make_float2(fmaxf(z[i], kNegInf), i + 1 < N ? fmaxf(z[i + 1], kNegInf) : kNegInf);
-      if (KIND == kAsinh) x[i / 2] = mul2(x[i / 2], make_float2(a.scale, a.scale));
-      w[i / 2] = fast_weights<KIND, LOG2N>(a, x[i / 2], make_float2(turn, turn));
-      high = fmaxf(high, fmaxf(w[i / 2].x, w[i / 2].y));
+      for (int i = 0; i < P; ++i) {
+        w[i] = fast_weights<KIND, LOG2N>(a, x[i], make_float2(turn, turn));
+        sum = i ? add2(sum, w[i]) : w[i];
+      }
+      return sum;
+    };
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      x[i] = make_float2(z[2 * i], 2 * i + 1 < N ? z[2 * i + 1] : kNegInf);
+      if (CLEAN) x[i] = make_float2(fmaxf(x[i].x, kNegInf), fmaxf(x[i].y, kNegInf));
+      if (KIND == kAsinh) x[i] = mul2(x[i], make_float2(a.scale, a.scale));
     }
-    if (high > kFar) {
+    float2 inc = weigh();
+    if (fmaxf(inc.x, inc.y) > kFar) {  // the reference moves
       float top = m;
 #pragma unroll
-      for (int i = 0; i < (N + 1) / 2; ++i) top = fmaxf(top, fmaxf(x[i].x, x[i].y));
+      for (int i = 0; i < P; ++i) top = fmaxf(top, fmaxf(x[i].x, x[i].y));
       const float to = weight_turn<KIND, true>(top);
       const float f = m == kNegInf ? 0.f : exact_weight<KIND>(a, m, to);
       l = mul2(l, make_float2(f, f));
       m = top;
       turn = to;
-#pragma unroll
-      for (int i = 0; i < (N + 1) / 2; ++i) w[i] = fast_weights<KIND, LOG2N>(a, x[i], make_float2(turn, turn));
+      inc = weigh();
     }
-#pragma unroll
-    for (int i = 0; i < (N + 1) / 2; ++i) l = add2(l, w[i]);
+    l = add2(l, inc);
   }
 };
 
@@ -212,35 +222,41 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
       const int r = at / blocks;
       const Cols c(r < nt ? target + (int64_t)(i0 + r) * a.V : draft + (int64_t)(i0 + r - nt) * a.V, begin, end);
       const uint4* mid = reinterpret_cast<const uint4*>(c.row + c.mid);
-      RowSum<KIND, LOG2N> sum;
-      sum.clear();
-      if (at == r * blocks && lane < c.ends()) {
-        const float z[1] = {to_f32(c.row[c.end_column(lane)])};
-        sum.add(a, z);
-      }
       const int to = min(stop, (r + 1) * blocks);
-      int v = (at - r * blocks) * kBlock + lane;
-      const int v_end = min(c.vecs, (to - r * blocks) * kBlock);
+      const int v_begin = (at - r * blocks) * kBlock + lane, v_end = min(c.vecs, (to - r * blocks) * kBlock);
+      const bool has_ends = at == r * blocks && lane < c.ends();
       at = to;
-      uint4 next[kFly];
-#pragma unroll
-      for (int i = 0; i < kFly; ++i)
-        if (v + i * 32 < v_end) next[i] = __ldg(mid + v + i * 32);
-      for (; v < v_end; v += 32 * kFly) {
-        uint4 raw[kFly];
-#pragma unroll
-        for (int i = 0; i < kFly; ++i) {
-          raw[i] = next[i];
-          if (v + (i + kFly) * 32 < v_end) next[i] = __ldg(mid + v + (i + kFly) * 32);
-        }
+      RowSum<KIND, LOG2N> sum;
+      auto add_up = [&](auto clean) {
+        constexpr bool CLEAN = decltype(clean)::value;
+        sum.clear();
+        int v = v_begin;
+        uint4 next[kFly];
 #pragma unroll
         for (int i = 0; i < kFly; ++i)
-          if (v + i * 32 < v_end) {
-            float z[V::N];
-            unpack<T>(raw[i], z);
-            sum.add(a, z);
+          if (v + i * 32 < v_end) next[i] = __ldg(mid + v + i * 32);
+        if (has_ends) {
+          const float z[1] = {to_f32(c.row[c.end_column(lane)])};
+          sum.template add<CLEAN>(a, z);
+        }
+        for (; v < v_end; v += 32 * kFly) {
+          uint4 raw[kFly];
+#pragma unroll
+          for (int i = 0; i < kFly; ++i) {
+            raw[i] = next[i];
+            if (v + (i + kFly) * 32 < v_end) next[i] = __ldg(mid + v + (i + kFly) * 32);
           }
-      }
+#pragma unroll
+          for (int i = 0; i < kFly; ++i)
+            if (v + i * 32 < v_end) {
+              float z[V::N];
+              unpack<T>(raw[i], z);
+              sum.template add<CLEAN>(a, z);
+            }
+        }
+      };
+      add_up(std::false_type{});
+      if (__any_sync(0xffffffffu, !(sum.l.x + sum.l.y < INFINITY))) add_up(std::true_type{});
       float M = sum.m;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
