@@ -422,7 +422,7 @@ constexpr int kMoveThreads = 256;
 constexpr int kMoveFly = 4;
 constexpr int kMovePieces = kMoveThreads * kMoveFly;
 
-__global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const EvictArgs a, const PagedView pv, int items,
+__global__ void __launch_bounds__(kMoveThreads, 4) cache_move_kernel(const EvictArgs a, const PagedView pv, int items,
                                                                   int chunks) {
   pdl_wait();
   for (int64_t i = blockIdx.x; i < (int64_t)items * chunks; i += gridDim.x) {

@@ -106,8 +106,9 @@ __device__ __forceinline__ float2 weight_pair(float2 x, float2 turn, int log2n) 
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(y.y));
     y.x += fabsf(x.x);
     y.y += fabsf(x.y);
-    y.x = x.x >= 0.f ? y.x : rcp_fast(y.x);
-    y.y = x.y >= 0.f ? y.y : rcp_fast(y.y);
+    const float rx = rcp_fast(y.x), ry = rcp_fast(y.y);
+    y.x = x.x >= 0.f ? y.x : rx;
+    y.y = x.y >= 0.f ? y.y : ry;
     y = mul2(y, turn);
     if constexpr (LOG2N > 0) {
 #pragma unroll
