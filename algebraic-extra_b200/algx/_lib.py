@@ -146,6 +146,28 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The native front-end of the serving operators (``algx._native``, built in-tree
+    beside libalgx.so), bound once to the loaded library's entries."""
+    global _native
+    if _native is None:
+        handle = lib()
+        with _lock:
+            if _native is None:
+                try:
+                    from . import _native as mod
+                except ImportError as e:
+                    raise AlgxError("algx/_native.so is missing or does not load: build it with "
+                                    f"__graft_entry__.build() ({e})") from e
+                names = [n for n in SIGNATURES if hasattr(handle, n)]
+                mod.bind(AlgxError, {n: ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in names})
+                _native = mod
+    return _native
+
+
 def check(status: int, what: str) -> None:
     if status != ALGX_OK:
         msg = lib().algx_last_error().decode(errors="replace")

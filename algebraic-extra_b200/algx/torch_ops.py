@@ -327,7 +327,7 @@ def _(q, k_pages, v_pages, table, lens, sink, scores, kind, n, c, window, first)
 def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: str = "softmax", n: int = 16,
                     c: float = 16.0, window: Optional[int] = None, first: int = 0, scores=None):
     """``algx.kernels.paged.paged_attention`` as one node; ``scores`` is updated in place and returned beside o."""
-    P.paged_config(kind, n, c, window, first)
+    P.paged_options(kind, n, c, window, first)
     args = (q, k_pages, v_pages, table, lens, sink_logit)
     if scores is None:
         return _paged_attention_op(*args, kind, n, float(c), window or 0, first)
