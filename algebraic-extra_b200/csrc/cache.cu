@@ -13,8 +13,8 @@ namespace {
 constexpr int kD = 64;
 
 // ------------------------------------------------------------------- append
-constexpr int kAppThreads = 256;
-constexpr int kAppPasses = 3;  // row groups of one warp, loaded together
+constexpr int kAppThreads = 128;
+constexpr int kAppPasses = 5;  // row groups of one warp, loaded together
 
 struct AppendArgs {
   const void* qkv;
@@ -36,7 +36,7 @@ struct AppendArgs {
 // one rounding at the store: the cache holds the nearest bf16 of the exact key.
 // Bound by memory: each row is read once and written once.
 template <typename T, bool NORM, bool ROT>
-__global__ void __launch_bounds__(kAppThreads, 3) cache_append_kernel(const AppendArgs a, const PagedView pv) {
+__global__ void __launch_bounds__(kAppThreads, 4) cache_append_kernel(const AppendArgs a, const PagedView pv) {
   using V = Vec<T>;
   constexpr int N = V::N, kLanes = V::TPR / 2, kRows = 32 / kLanes;
   pdl_wait();

@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
 // ------------------------------------------------------------------------ join
 // Blocks below `rows` join one row's partial results; the others add the weights
 // of their slots over the rows of one kv head.
-constexpr int kScoreSlots = 512;
+constexpr int kScoreSlots = 1024;
 constexpr int kRowChunk = 64;
 
 // Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
