@@ -26,7 +26,7 @@ constexpr int kD = 64;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
-constexpr int kMinSlots = 64;  // slots a warp takes at least
+constexpr int kMinSlots = 128;  // slots a warp takes at least: fewer make more parts to join (float32 case 21.9 us with 64, 26.3 with 256)
 
 struct PagedAttnArgs {
   const void *q, *k, *v;
