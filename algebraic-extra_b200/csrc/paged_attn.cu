@@ -26,7 +26,11 @@ constexpr int kD = 64;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
-constexpr int kMinSlots = 128;  // slots a warp takes at least: fewer make more parts to join (float32 case 21.9 us with 64, 26.3 with 256)
+// Slots a warp takes at least: fewer make more parts to join, more leave a short
+// cache to few warps. bf16: one user over 2048 slots 10.2 us a pass with 64, 11.4
+// with 128. float32, whose parts are joined with exact roots: 4 users over 4096
+// slots 22.0 us with 64, 19.9 with 128, 26.3 with 256.
+constexpr int kMinSlotsBf16 = 64, kMinSlotsF32 = 128;
 
 struct PagedAttnArgs {
   const void *q, *k, *v;
@@ -39,7 +43,7 @@ struct PagedAttnArgs {
   int* err;
   int64_t slots;    // S: slots of one sequence's table
   int B, T, G, rows, tile_rows, tiles, warps, log2n;
-  int shift;        // log2 of the slots of a group
+  int shift, least;  // log2 of the slots of a group; groups a warp takes at least
   float scale, inv_unit;
   Sight sight;
 };
@@ -87,7 +91,7 @@ struct Line {
       total += __reduce_add_sync(0xffffffffu, n);
       before += __reduce_add_sync(0xffffffffu, b < upto ? n : 0);
     }
-    share = max(kMinSlots >> a.shift, (int)(((unsigned)total + a.warps - 1) / (unsigned)a.warps));
+    share = max(a.least, (int)(((unsigned)total + a.warps - 1) / (unsigned)a.warps));
   }
 };
 
@@ -543,7 +547,7 @@ struct MmaEngine {
       const int slot = base + u * 16 + 2 * t;
       auto keep = [&](int slot, int lo, int hi) {  // seen by some query with lo <= last <= hi
         auto seen = [&](int s) {
-          return s < live && s <= hi && (a.sight.window == 0 || s > lo - a.sight.window || s < a.sight.first);
+          return s < live && s <= hi && (a.sight.window == 0 || s > max(lo, 0) - a.sight.window || s < a.sight.first);
         };
         return (seen(slot) ? 0xffffu : 0u) | (seen(slot + 1) ? 0xffff0000u : 0u);
       };
@@ -882,8 +886,9 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool sc
   }
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
   p.items = B * Hkv * p.tiles;
-  // one wave of CTAs, fewer where even the full tables hold less than kMinSlots a warp
-  const int64_t most = (p.items * ((S + 31) / 32 * 32) + kMinSlots - 1) / kMinSlots;
+  // one wave of CTAs, fewer where even the full tables hold less than the least a warp takes
+  const int64_t least = wide ? kMinSlotsBf16 : kMinSlotsF32;
+  const int64_t most = (p.items * ((S + 31) / 32 * 32) + least - 1) / least;
   p.warps = std::min<int64_t>(kSms * ctas, (most + kWarps - 1) / kWarps) * kWarps;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t parts = (size_t)((p.warps + p.items) * p.tile_rows);
@@ -1000,6 +1005,7 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   a.inv_unit = soft ? cfg->inv_unit * kLog2e : cfg->inv_unit;
   a.sight = {cfg->window, cfg->first};
   a.shift = dtype == ALGX_BF16 ? 5 : 4;
+  a.least = (dtype == ALGX_BF16 ? kMinSlotsBf16 : kMinSlotsF32) >> a.shift;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == ALGX_BF16)
     return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, st) : paged_launch<__nv_bfloat16, kAsinh>(a, pv, st);

@@ -160,7 +160,7 @@ struct Span {
     head_groups = 0;
     skip = 0;
     if (w.window != 0) {
-      const int left = max(0, lo - w.window + 1) >> shift;
+      const int left = max(0, max(lo, 0) - w.window + 1) >> shift;  // queries before slot 0 see nothing
       const int head = (min(w.first, end) + more) >> shift;
       if (head < left) {
         head_groups = head;

@@ -115,6 +115,12 @@ def test_attention_powers_and_score_ranges(kind, n, gain, dtype):
                     gain=gain, sink=True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_widest_window_with_fewer_slots_than_tokens(dtype):
+    check_attention(B=2, T=9, Hq=4, Hkv=2, page=16, lens=[3, 40], dtype=dtype, kind="asinh", seed=8, window=2 ** 31 - 1,
+                    first=2)
+
+
 def test_attention_long_cache_of_many_splits():
     check_attention(B=1, T=1, Hq=2, Hkv=1, page=64, lens=[9001], dtype=BF16, kind="asinh", seed=3, scored=True)
 
@@ -322,6 +328,10 @@ def check_evict(B, Hkv, page, lens, budget, first, recent, dtype, seed, scores=N
 ])
 def test_evict(B, Hkv, page, lens, budget, first, recent, levels, dtype):
     check_evict(B, Hkv, page, lens, budget, first, recent, dtype, 40 + budget, levels=levels)
+
+
+def test_evict_of_more_slots_than_shared_memory_holds():
+    check_evict(1, 1, 256, [51000], 3000, 4, 100, BF16, 60)
 
 
 def test_evict_odd_scores():
