@@ -34,7 +34,9 @@ struct AppendArgs {
 // pairs: it needs no exchange, and the norm two shuffles (bf16: 4 lanes a row, 8
 // rows a group). y = rms(x) g, then (y1 c - y2 s, y1 s + y2 c), all in fp32 with
 // one rounding at the store: the cache holds the nearest bf16 of the exact key.
-// Bound by memory: each row is read once and written once.
+// Bound by memory: each row is read once and written once. Measured: 16384 tokens of
+// 36 rows (155 MB) 30 us, 5.1 TB/s; with a row across 8 lanes, halves exchanged by
+// shuffles, 47 us; three row groups a warp instead of five 34 us.
 template <typename T, bool NORM, bool ROT>
 __global__ void __launch_bounds__(kAppThreads, 4) cache_append_kernel(const AppendArgs a, const PagedView pv) {
   using V = Vec<T>;
@@ -260,7 +262,9 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& p
 // lowest slots. One sweep over the slots then numbers the holes below the budget
 // and the kept slots at or above it: the i-th such slot moves to the i-th hole, so
 // a row that is below the budget never moves. This is a chain of some twenty
-// block-wide steps, whatever the length.
+// block-wide steps, whatever the length. Measured: 12 items of 2560 slots 17 us, with
+// the moves, 192 items of 8192 slots 27 us. (Counting with one addition for all lanes
+// that meet in a bin took 40 us: their matching costs more than the conflicts.)
 __global__ void __launch_bounds__(kEvThreads, 2) cache_evict_kernel(const EvictArgs a, const PagedView pv) {
   extern __shared__ uint4 s_keys[];
   __shared__ int4 hist[kBins / 4];
@@ -417,7 +421,8 @@ __global__ void __launch_bounds__(kEvThreads, 2) cache_evict_kernel(const EvictA
 }
 
 // The moves of all items, spread over the device: kMovePieces 16-byte pieces of
-// keys and of values a CTA at a time.
+// keys and of values a CTA at a time. Bound by memory at single 128-byte rows;
+// measured: 201 MB 41 us, 4.9 TB/s.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveFly = 4;
 constexpr int kMovePieces = kMoveThreads * kMoveFly;
@@ -535,7 +540,9 @@ int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const i
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
   const int64_t S = page_size * max_pages;
   // Rows an item can move at most. Up to kInplace of them its own CTA moves them,
-  // which saves a launch; more are spread over the device.
+  // which saves a launch (12 items of at most 512 rows: 11 us a pass in one launch);
+  // more are spread over the device (192 items of 2050 rows: 69 us a pass in two
+  // launches, 138 in one).
   const int64_t most = std::min<int64_t>(budget, std::max<int64_t>(0, S - budget));
   a.inplace = most <= kInplace;
   a.cached = S <= kEvCached;

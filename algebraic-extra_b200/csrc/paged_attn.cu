@@ -586,7 +586,11 @@ struct MmaEngine {
 // the groups of the warp's share, rows of keys and of values contiguous in a page,
 // kStages - 1 groups ahead into the warp's ring, across the ends of items;
 // the warp takes them from there. (bf16 boxes are swizzled by 128 bytes, so that
-// ldmatrix meets no bank twice.)
+// ldmatrix meets no bank twice.) Three CTAs of four warps with one 8 KB group on its
+// way and one at work keep 96 KB an SM in flight.
+// Measured: 638 MB of 8 ragged sequences up to 32768 slots, 16 heads, 105 us (6.1
+// TB/s; a plain copy reads and writes 6.55); 134 MB of 512 windows of 1024 slots 31
+// us; 20 rows a head over 150 MB 51 us, there bound by issue at 8 warps an SM.
 template <typename E>
 constexpr int group_bytes() { return 2 * E::kSlots * E::kRowBytes; }
 template <typename E>

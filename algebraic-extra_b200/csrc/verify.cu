@@ -14,7 +14,10 @@
 // distributed shared memory, each decides the (same) accepted count, races over
 // its slice of the one row that counts, and the winners meet in CTA 0.
 //
-// Bound by reading the logits once. The sums use the MUFU forms of the weights
+// Bound by reading the logits once where there are many sequences, by the chain of
+// two to four cluster barriers where there are few. Measured: 64 sequences of 7
+// drafts over 50304 float32 logits 55 us a pass (124 MB of them read), one of 4
+// drafts, bf16, 10.5 us. The sums use the MUFU forms of the weights
 // (2^-22 relative error an element, averaged by the sum); everything a decision
 // compares - the drafted tokens' probabilities and the race's candidates - is
 // evaluated with correctly rounded roots and divisions or expf.
@@ -466,7 +469,10 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   // Few sequences: all rows in one round, whose time is latency, over as many SMs
   // as a cluster spans. Where the clusters fill the device, four positions a
   // round, as rows behind a refusal are mostly not read, and smaller CTAs, four
-  // an SM, which leave less of a last wave.
+  // an SM, which leave less of a last wave. (64 sequences of 7 drafts: 87 us with one
+  // position a round, 66, 61, 57 with two, three, four, 60 with all; two CTAs of 512
+  // threads an SM took 100 instead of 74 at an earlier step. One sequence: 25 us over
+  // 8 SMs, 17 over 16.)
   const bool few = B * 16 <= 148, wide = B * 8 <= 2 * 148;
   const int64_t cluster = few ? 16 : 8;
   a.round = wide ? (int)K + 1 : 4;
