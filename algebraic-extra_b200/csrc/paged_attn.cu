@@ -10,6 +10,8 @@
 // with every weight taken relative to a running reference score, so that no sum
 // overflows (algebraic.py:186-204; the shifted form of kernels/flash.py:240-284).
 // A row that sees no slot, or whose weights are all zero, gives zeros.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -18,6 +20,8 @@
 #include "sm100.cuh"
 #include "tmap.h"
 #include "vec_io.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace algx {
 namespace {
@@ -44,6 +48,7 @@ struct PagedAttnArgs {
   int64_t slots;    // S: slots of one sequence's table
   int B, T, G, rows, tile_rows, tiles, warps, log2n;
   int shift, least;  // log2 of the slots of a group; groups a warp takes at least
+  int cluster;       // CTAs of an item where clusters join, 0 where a second launch does
   float scale, inv_unit;
   Sight sight;
 };
@@ -137,6 +142,13 @@ struct Cursor {
     grp = at;
     item = (b * pv.heads + h) * a.tiles + tile;
   }
+  // The grp_-th group of one item.
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, const PagedView& pv, int item_, const Span& span_, int len_,
+                                    int grp_) : item(item_), grp(grp_), len(len_), span(span_) {
+    tile = item % a.tiles;
+    h = item / a.tiles % pv.heads;
+    b = item / a.tiles / pv.heads;
+  }
   __device__ __forceinline__ int slot(const PagedAttnArgs& a) const { return span.group(grp) << a.shift; }
   // On to the next group, if there is one.
   __device__ __forceinline__ void next(const PagedAttnArgs& a, const PagedView& pv) {
@@ -156,6 +168,13 @@ struct Cursor {
     } while (span.total == 0);
   }
 };
+
+// Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
+__device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+__device__ __forceinline__ float sink_score(const PagedAttnArgs& a, int h, int row) {
+  return a.sink ? a.sink[h * a.G + row % a.G] * a.inv_unit : kNegInf;
+}
 
 // What a warp needs to know of the item it works on.
 struct Item {
@@ -191,7 +210,7 @@ constexpr float kMove = 256.f;
 template <int KIND_, int R>
 struct FmaEngine {
   using T = float;
-  static constexpr int kSlots = 16, kStages = 2, kCtas = 3, kRowBytes = kD * 4;
+  static constexpr int kSlots = 16, kStages = 2, kCtas = 3, kRowBytes = kD * 4, kKind = KIND_;
   static constexpr bool kSwizzle = false;
   float4 q[R], acc[R];
   float m[R], turn[R], l[R];
@@ -342,7 +361,8 @@ struct MmaEngine {
   using T = __nv_bfloat16;
   // Groups of 32 slots: copies of 4 KB. Read in 2 KB pieces memory gives a tenth
   // less (6.0 TB/s instead of 6.6 in a bare ring of this form).
-  static constexpr int kSlots = 32, kStages = NT <= 2 ? 2 : 3, kCtas = NT <= 2 ? 3 : 2, kRowBytes = kD * 2;
+  static constexpr int kSlots = 32, kStages = NT <= 2 ? 2 : 3, kCtas = NT <= 2 ? 3 : 2, kRowBytes = kD * 2,
+                       kKind = KIND_;
   static constexpr int kSub = NT == 1 ? 2 : 1;  // 16-slot steps worked on together
   static constexpr bool kSwizzle = true;
   // Scores are worked on in pairs: of both columns of a lane, or, with a single
@@ -596,7 +616,66 @@ constexpr int group_bytes() { return 2 * E::kSlots * E::kRowBytes; }
 template <typename E>
 constexpr int ring_smem() { return 1024 + kWarps * E::kStages * group_bytes<E>(); }
 
+// Joins the CTA's warps' partial results (s_ml, s_o: by warp and row) in one, then
+// the cluster's CTAs', a share of the outputs each.
 template <typename E>
+__device__ __forceinline__ void join_cluster(const PagedAttnArgs& a, const PagedView& pv, const Item& w, float2* s_ml,
+                                             float* s_o) {
+  using T = typename E::T;
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int kKind = E::kKind, kMost = 8;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int R = a.tile_rows, C = a.cluster;
+  float2* const c_ml = s_ml + kWarps * R;
+  float* const c_o = s_o + kWarps * R * kD;
+  for (int i = threadIdx.x; i < w.nr * kD; i += kThreads) {
+    const int r = i / kD, d = i % kD;
+    float M = kNegInf, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) M = fmaxf(M, s_ml[p * R + r].x);
+    const float turn = weight_turn<kKind, EXACT>(M);
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) {
+      const float2 ml = s_ml[p * R + r];
+      const float f = ml.x == kNegInf ? 0.f : weight_of<kKind, EXACT>(ml.x, turn, a.log2n);
+      L = fmaf(ml.y, f, L);
+      O = fmaf(s_o[(p * R + r) * kD + d], f, O);
+    }
+    c_o[i] = O;
+    if (d == 0) c_ml[r] = make_float2(M, L);
+  }
+  cluster.sync();
+  for (int i = (int)cluster.block_rank() * kThreads + threadIdx.x; i < w.nr * kD; i += C * kThreads) {
+    const int r = i / kD, d = i % kD;
+    const float sink = sink_score(a, w.h, w.r0 + r);
+    float2 ml[kMost];
+    float x[kMost];
+    float M = sink;
+#pragma unroll
+    for (int c = 0; c < kMost; ++c)
+      if (c < C) {
+        ml[c] = *cluster.map_shared_rank(c_ml + r, c);
+        x[c] = *cluster.map_shared_rank(c_o + i, c);
+        M = fmaxf(M, ml[c].x);
+      }
+    const float turn = weight_turn<kKind, EXACT>(M);
+    float L = sink == kNegInf ? 0.f : weight_of<kKind, EXACT>(sink, turn, a.log2n), O = 0.f;
+#pragma unroll
+    for (int c = 0; c < kMost; ++c)
+      if (c < C) {
+        const float f = ml[c].x == kNegInf ? 0.f : weight_of<kKind, EXACT>(ml[c].x, turn, a.log2n);
+        L = fmaf(ml[c].y, f, L);
+        O = fmaf(x[c], f, O);
+      }
+    static_cast<T*>(a.o)[w.q_row(a, pv, r) * kD + d] = from_f32<T>(O * row_scale(L));
+  }
+  cluster.sync();  // nobody leaves while others read its shared memory
+}
+
+// CLUSTER: a cluster of a.cluster CTAs takes one item, its groups cut evenly over
+// the cluster's warps, and joins the result itself. For short caches: no line has
+// to be counted and no second launch waits, which are half of their time.
+template <typename E, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, E::kCtas)
     paged_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       const PagedAttnArgs a, const PagedView pv) {
@@ -606,8 +685,8 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   __shared__ int4 s_meta[kWarps][kStages];  // item, first slot, live slots
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned char* const ring =
-      smem_raw + (1024 - (sm100::smem_u32(smem_raw) & 1023)) + warp * kStages * kBytes;
+  unsigned char* const rings = smem_raw + (1024 - (sm100::smem_u32(smem_raw) & 1023));
+  unsigned char* const ring = rings + warp * kStages * kBytes;
   uint64_t* const full = s_full[warp];
   if (lane == 0) {
 #pragma unroll
@@ -621,14 +700,30 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
   }
   __syncthreads();
   pdl_wait();
-  const Line line(a, pv, 0);
-  const int share = line.share, total = line.total;
-  const int wid = warp * gridDim.x + blockIdx.x;  // neighbours in the line sit on different SMs
-  if ((int64_t)wid * share >= total) return;
-  const int start = wid * share;
-  int left = min(share, total - start), to_issue = left;
+  int wid = 0, left = 0, start = 0;
+  if constexpr (!CLUSTER) {
+    const Line line(a, pv, 0);
+    wid = warp * gridDim.x + blockIdx.x;  // neighbours in the line sit on different SMs
+    const int64_t from = (int64_t)wid * line.share;
+    if (from >= line.total) return;  // also where no sequence has a group, which Cursor would look for
+    start = (int)from;
+    left = min(line.share, line.total - start);
+  }
+  Cursor at = [&] {
+    if constexpr (CLUSTER) {
+      const int item = blockIdx.x / (unsigned)a.cluster, rank = blockIdx.x - item * a.cluster;
+      const int len = paged_len(pv, item / a.tiles / pv.heads, a.err);
+      const Span span = item_span(a, len, item % a.tiles);
+      const int n = a.cluster * kWarps, r = rank * kWarps + warp;
+      start = (int)((int64_t)span.total * r / n);
+      left = (int)((int64_t)span.total * (r + 1) / n) - start;
+      return Cursor(a, pv, item, span, len, start);
+    } else {
+      return Cursor(a, pv, start);
+    }
+  }();
+  int to_issue = left;
 
-  Cursor at(a, pv, start);
   // A group lies in one page, or, with pages of 16 slots and groups of 32, in two.
   const int boxes = (1 << pv.page_shift) < E::kSlots ? 2 : 1;
   int2 pid = make_int2(0, 0);
@@ -694,11 +789,20 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
     }
   }
   pdl_trigger();  // not earlier: the join's CTAs would only wait beside this kernel's (34.0 us a pass instead of 33.0)
-  e.flush(w, a.part_ml + (int64_t)(wid + item) * a.tile_rows, a.part_o + (int64_t)(wid + item) * a.tile_rows * kD);
+  if constexpr (!CLUSTER)
+    e.flush(w, a.part_ml + (int64_t)(wid + item) * a.tile_rows, a.part_o + (int64_t)(wid + item) * a.tile_rows * kD);
   if (left > 0) {  // a copy did not arrive in time: let those on their way land, within limits, before the CTA ends
     volatile int quiet = 0;
     for (int i = 0; i < kStages && i < left - to_issue; ++i)
       sm100::mbar_wait(&full[(stage + i) % kStages], parity ^ (stage + i >= kStages), &quiet, nullptr);
+  }
+  if constexpr (CLUSTER) {
+    __syncthreads();  // the rings are free
+    float* const s_o = reinterpret_cast<float*>(rings);
+    float2* const s_ml = reinterpret_cast<float2*>(s_o + (kWarps + 1) * a.tile_rows * kD);
+    e.flush(w, s_ml + warp * a.tile_rows, s_o + warp * a.tile_rows * kD);
+    __syncthreads();
+    join_cluster<E>(a, pv, w, s_ml, s_o);
   }
 }
 
@@ -710,9 +814,6 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
 // rows of 10 parts 57 and 52.
 constexpr int kScoreSlots = 1024;
 constexpr int kRowChunk = 64;
-
-// Final factor of a row: 1 / l with the sink's weight in l, 0 for an empty row.
-__device__ __forceinline__ float row_scale(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // The partial results of one item: indices first .. first + count - 1, and the row
 // in its tile.
@@ -747,10 +848,6 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, const Parts& p,
     if (x.x != kNegInf || x.y != 0.f) L = fmaf(x.y, weight_of<KIND, EXACT>(x.x, turn, a.log2n), L);
   }
   L = row_sum<32>(L);
-}
-
-__device__ __forceinline__ float sink_score(const PagedAttnArgs& a, int h, int row) {
-  return a.sink ? a.sink[h * a.G + row % a.G] * a.inv_unit : kNegInf;
 }
 
 __device__ __forceinline__ void store_row(float* o, int quad, const float4& y) { reinterpret_cast<float4*>(o)[quad] = y; }
@@ -902,11 +999,28 @@ Plan make_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t S, bool sc
   return p;
 }
 
+// Clusters join where the caller's table bounds a warp's work to kFewGroups groups:
+// CTAs an item (at most 8, one wave of them), or 0. One user over 2048 slots: 8.6 us
+// a pass, 9.8 along the line; 512 windows of 1024 slots, 9 groups a warp: 39.9 us by
+// clusters, 33.4 along the line, which balances them.
+constexpr int kFewGroups = 4;
+
 template <typename E>
-int attn_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
-  constexpr int dtype = sizeof(typename E::T) == 2 ? ALGX_BF16 : ALGX_F32;
+int cluster_of(const PagedAttnArgs& a, int64_t items) {
+  if (a.xs != nullptr) return 0;
+  int64_t slots = a.slots;
+  if (a.sight.window) slots = std::min<int64_t>(slots, (int64_t)a.sight.window + a.T + a.sight.first + 2 * E::kSlots);
+  int c = 8;
+  while (c > 1 && items * c > kSms * E::kCtas) c /= 2;
+  const int64_t groups = (slots + E::kSlots - 1) / E::kSlots;
+  return groups <= (int64_t)c * kWarps * kFewGroups && items * c <= INT32_MAX ? c : 0;
+}
+
+template <typename E, bool CLUSTER>
+int attn_kernel(const PagedAttnArgs& a, const PagedView& pv, const CUtensorMap& k, const CUtensorMap& v, int64_t grid,
+                cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};  // one bit per device: its shared memory limit is raised
-  auto* kern = paged_attn_kernel<E>;
+  auto* kern = paged_attn_kernel<E, CLUSTER>;
   int dev = 0;
   ALGX_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
@@ -914,19 +1028,41 @@ int attn_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
     ALGX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_smem<E>()));
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = ring_smem<E>();
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CLUSTER ? a.cluster : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
+  ALGX_CUDA(cudaLaunchKernelEx(&cfg, kern, k, v, a, pv));
+  ALGX_LAUNCHED("paged_attn_kernel");
+  return ALGX_OK;
+}
+
+template <typename E>
+int attn_launch(PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+  constexpr int dtype = sizeof(typename E::T) == 2 ? ALGX_BF16 : ALGX_F32;
   const int64_t rows = ((int64_t)pv.num_pages * pv.heads) << pv.page_shift;
   ALGX_REQUIRE(rows <= INT32_MAX, "paged cache too large");
   CUtensorMap k, v;
   const uint32_t box = std::min(E::kSlots, 1 << pv.page_shift);
   if (int e = make_tmap_2d(&k, a.k, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
   if (int e = make_tmap_2d(&v, a.v, dtype, kD, (uint64_t)rows, E::kRowBytes, kD, box, E::kSwizzle)) return e;
-  ALGX_CUDA(launch_dependent(kern, dim3(a.warps / kWarps), dim3(kThreads), ring_smem<E>(), st, k, v, a, pv));
-  ALGX_LAUNCHED("paged_attn_kernel");
-  return ALGX_OK;
+  const int64_t items = (int64_t)a.B * pv.heads * a.tiles;
+  a.cluster = cluster_of<E>(a, items);
+  return a.cluster ? attn_kernel<E, true>(a, pv, k, v, items * a.cluster, st)
+                   : attn_kernel<E, false>(a, pv, k, v, a.warps / kWarps, st);
 }
 
 template <int KIND, int LOG2N>
-int mma_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+int mma_launch(PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
   return a.rows == 1         ? attn_launch<MmaEngine<KIND, LOG2N, 1, true>>(a, pv, st)
          : a.tile_rows == 8  ? attn_launch<MmaEngine<KIND, LOG2N, 1, false>>(a, pv, st)
          : a.tile_rows == 16 ? attn_launch<MmaEngine<KIND, LOG2N, 2, false>>(a, pv, st)
@@ -935,7 +1071,7 @@ int mma_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
 }
 
 template <typename T, int KIND>
-int paged_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
+int paged_launch(PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
   int e;
   if constexpr (sizeof(T) == 2)
     e = KIND == kAsinh && a.log2n == 4 ? mma_launch<KIND, 4>(a, pv, st) : mma_launch<KIND, 0>(a, pv, st);
@@ -945,6 +1081,7 @@ int paged_launch(const PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
         : a.tile_rows == 4 ? attn_launch<FmaEngine<KIND, 4>>(a, pv, st)
                            : attn_launch<FmaEngine<KIND, 8>>(a, pv, st);
   if (e) return e;
+  if (a.cluster) return ALGX_OK;
   const bool narrow = (int64_t)a.B * pv.heads * a.rows > kSms * 8;
   const int64_t row_blocks = narrow ? (a.rows + kWarps - 1) / kWarps : a.rows;
   const int64_t blocks = row_blocks + (a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0);

@@ -52,7 +52,7 @@ def bound(mag, ref, dtype, n, kind, top, q, k):
 
 
 def check_attention(B, T, Hq, Hkv, page, lens, dtype, kind, seed, n=16, c=8.0, window=None, first=0, sink=False,
-                    scored=False, gain=1.0, in_place=False):
+                    scored=False, gain=1.0, in_place=False, wide=0):
     max_pages = max(1, -(-max(max(lens), 1) // page)) + 1
     k, v, table, g = make_cache(B, Hkv, page, max_pages, dtype, seed, gain)
     k, v = poison(k, table, lens), poison(v, table, lens)
@@ -63,6 +63,7 @@ def check_attention(B, T, Hq, Hkv, page, lens, dtype, kind, seed, n=16, c=8.0, w
     ref, new, mag, top = O.paged_attention(q, k, v, table, lens, s, kind=kind, n=n, c=c, window=window, first=first,
                                            scores=scores)
     dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    table = torch.nn.functional.pad(table, (0, wide))  # pages that no sequence has reached
     lens_d = torch.tensor(lens, dtype=torch.int32).cuda()
     sc = dev(scores)
     out = None if not scored or in_place else torch.full_like(sc, math.nan)
@@ -119,6 +120,29 @@ def test_attention_powers_and_score_ranges(kind, n, gain, dtype):
 def test_attention_widest_window_with_fewer_slots_than_tokens(dtype):
     check_attention(B=2, T=9, Hq=4, Hkv=2, page=16, lens=[3, 40], dtype=dtype, kind="asinh", seed=8, window=2 ** 31 - 1,
                     first=2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("sink", [False, True])
+def test_attention_of_empty_sequences_alone(dtype, sink):
+    for B, T, max_pages in ((1, 1, 1), (3, 2, 200)):
+        k, v, table, g = make_cache(B, 2, 16, max_pages, dtype, 14)
+        q = torch.randn((B, T, 4, 64), generator=g).to(dtype).cuda()
+        lens = torch.zeros(B, dtype=torch.int32).cuda()
+        s = torch.ones(4).cuda() if sink else None
+        o = paged_attention(q, k.cuda(), v.cuda(), table.cuda(), lens, s, kind="asinh")
+        assert bool((o == 0).all())
+        scores = torch.ones((B, 2, 16 * max_pages), device="cuda")
+        o, new = paged_attention(q, k.cuda(), v.cuda(), table.cuda(), lens, s, scores=scores)
+        assert bool((o == 0).all()) and bool((new == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["asinh", "softmax"])
+@pytest.mark.parametrize("i", [i for i, case in enumerate(CASES) if not case.get("scored")])
+def test_attention_with_wide_tables(i, kind, dtype):
+    """Short tables are joined by clusters, wide ones along the line of all groups."""
+    check_attention(dtype=dtype, kind=kind, seed=100 + i, wide=4096, **CASES[i])
 
 
 def test_attention_long_cache_of_many_splits():
