@@ -16,7 +16,7 @@
 //
 // Bound by reading the logits once where there are many sequences, by the chain of
 // two to four cluster barriers where there are few. Measured: 64 sequences of 7
-// drafts over 50304 float32 logits 55 us a pass (124 MB of them read), one of 4
+// drafts over 50304 float32 logits 55 us a pass (119 of 193 MB of them read), one of 4
 // drafts, bf16, 10.5 us. The sums use the MUFU forms of the weights
 // (2^-22 relative error an element, averaged by the sum); everything a decision
 // compares - the drafted tokens' probabilities and the race's candidates - is
@@ -44,7 +44,7 @@ struct VerifyArgs {
   int* err;
   int64_t V, slice;  // slice: vocabulary columns of one CTA
   int K, log2n;
-  int round;  // draft positions looked at in one round
+  int round;  // draft positions looked at in the first round
   float scale;  // 1 / temperature (ce) or 1 / c (alg_ce)
 };
 
@@ -209,13 +209,13 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
   };
   const int blocks = (int)max((int64_t)1, (end - begin + V::N * kBlock - 1) / (V::N * kBlock));
 
-  // Rounds of a.round positions, up to the first refusal: rows after it are not
+  // Two rounds at most, the first of a.round positions: rows after a refusal are not
   // needed. Row r of a round is target row i0 + r, then draft row i0 + (r - nt).
   int acc = -1, i0 = 0, nt = 0;
   for (int turn_no = 0; acc < 0; ++turn_no) {
-    i0 = turn_no * a.round;
-    nt = min(K + 1 - i0, a.round);
-    const int nd = min(K - i0, a.round), rows = nt + (has_draft ? nd : 0);
+    i0 += nt;
+    nt = turn_no == 0 ? min(K + 1, a.round) : K + 1 - i0;
+    const int nd = min(K - i0, nt), rows = nt + (has_draft ? nd : 0);
     float2* const s_mine = s_row[turn_no & 1];
     // the blocks of the round's rows stand in one line, cut into equal shares of the warps
     const int share = (rows * blocks + kWarps - 1) / kWarps;
@@ -467,10 +467,10 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Few sequences: all rows in one round, whose time is latency, over as many SMs
-  // as a cluster spans. Where the clusters fill the device, four positions a
-  // round, as rows behind a refusal are mostly not read, and smaller CTAs, four
-  // an SM, which leave less of a last wave. (64 sequences of 7 drafts: 87 us with one
-  // position a round, 66, 61, 57 with two, three, four, 60 with all; two CTAs of 512
+  // as a cluster spans. Where the clusters fill the device, four positions
+  // first, as rows behind a refusal are mostly not read, and smaller CTAs, four
+  // an SM, which leave less of a last wave. (64 sequences of 7 drafts: 60.8, 55.8,
+  // 56.5, 54.6, 57.3 us with one to five positions first, 60 with all; two CTAs of 512
   // threads an SM took 100 instead of 74 at an earlier step. One sequence: 25 us over
   // 8 SMs, 17 over 16.)
   const bool few = B * 16 <= 148, wide = B * 8 <= 2 * 148;
