@@ -808,12 +808,20 @@ __global__ void __launch_bounds__(kThreads, E::kCtas)
 
 // ------------------------------------------------------------------------ join
 // The first blocks of a kv head join its rows' partial results, the others add the
-// weights of kScoreSlots slots each over the rows. A row takes a CTA (NARROW
-// false), or, where the rows alone fill the device, a warp: 512 rows of 14 parts
+// weights of kScoreSlots slots each over the rows. A row takes a CTA, or, where the
+// rows alone fill the device, a warp: 512 rows of 14 parts
 // 33.4 us a pass with CTAs and 33.7 with warps, 48 rows of 37 parts 21 and 30, 2560
 // rows of 10 parts 57 and 52.
 constexpr int kScoreSlots = 1024;
 constexpr int kRowChunk = 64;
+// Threads of a row: a warp of a CTA of four (kNarrow), a CTA of 128, each of whose
+// warps finds the row's reference and sum for itself (kUsual), or, for few rows, one
+// of 512 that finds them together (kWide), as the way through hundreds of parts is
+// then all latency. 35 rows of 250 parts 32.2 us a pass with kUsual, 17.1 with kWide,
+// 27 rows of 400 parts 21.2 and 16.3, 3 heads of 8 scored rows 19.8 and 15.5; 48 rows
+// of 37 parts 19.5 and 19.9, 512 rows of 14 parts 34.4 and 41.5.
+enum JoinForm { kNarrow, kUsual, kWide };
+constexpr int join_threads(int form) { return form == kWide ? 512 : 128; }
 
 // The partial results of one item: indices first .. first + count - 1, and the row
 // in its tile.
@@ -832,22 +840,37 @@ struct Parts {
   }
 };
 
-// Reference and sum of one row over its parts and the sink, by one warp.
-template <int KIND, bool EXACT>
-__device__ __forceinline__ void join_row(const PagedAttnArgs& a, const Parts& p, float sink, float& turn, float& L) {
-  const int lane = threadIdx.x & 31;
+// Reference and sum of one row over its parts and the sink, by one warp or by all
+// WARPS of the CTA, over shared memory (2 WARPS floats).
+template <int KIND, bool EXACT, int WARPS>
+__device__ __forceinline__ void join_row(const PagedAttnArgs& a, const Parts& p, float sink, float* s_x, float& turn,
+                                         float& L) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = WARPS == 1 ? lane : threadIdx.x;
   const float2* ml = a.part_ml + p.first * a.tile_rows + p.row;
   float M = sink;  // -inf without a sink
-  for (int s = lane; s < p.count; s += 32) M = fmaxf(M, ml[(int64_t)s * a.tile_rows].x);
+  for (int s = at; s < p.count; s += WARPS * 32) M = fmaxf(M, ml[(int64_t)s * a.tile_rows].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  if constexpr (WARPS > 1) {
+    if (lane == 0) s_x[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) M = fmaxf(M, s_x[i]);
+  }
   turn = weight_turn<KIND, EXACT>(M);
-  L = lane == 0 && sink != kNegInf ? weight_of<KIND, EXACT>(sink, turn, a.log2n) : 0.f;
-  for (int s = lane; s < p.count; s += 32) {
+  L = at == 0 && sink != kNegInf ? weight_of<KIND, EXACT>(sink, turn, a.log2n) : 0.f;
+  for (int s = at; s < p.count; s += WARPS * 32) {
     const float2 x = ml[(int64_t)s * a.tile_rows];
     if (x.x != kNegInf || x.y != 0.f) L = fmaf(x.y, weight_of<KIND, EXACT>(x.x, turn, a.log2n), L);
   }
   L = row_sum<32>(L);
+  if constexpr (WARPS > 1) {
+    if (lane == 0) s_x[WARPS + warp] = L;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) L += s_x[WARPS + i];
+  }
 }
 
 __device__ __forceinline__ void store_row(float* o, int quad, const float4& y) { reinterpret_cast<float4*>(o)[quad] = y; }
@@ -857,9 +880,11 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* o, int quad, const floa
       make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-template <typename T, int KIND, bool NARROW>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArgs a, const PagedView pv, int blocks,
-                                                              int row_blocks) {
+template <typename T, int KIND, int FORM>
+__global__ void __launch_bounds__(join_threads(FORM)) paged_join_kernel(const PagedAttnArgs a, const PagedView pv,
+                                                                        int blocks, int row_blocks) {
+  constexpr bool NARROW = FORM == kNarrow;
+  constexpr int kThreads = join_threads(FORM), kWarps = kThreads / 32;
   constexpr bool EXACT = sizeof(T) == 4;
   // 16 lanes hold a part's 64 values; kSets such sets work on a row, each with
   // kAhead parts loaded before the row's reference is known
@@ -886,8 +911,9 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
       ref[i] = s < p.count ? a.part_ml[place(s)].x : kNegInf;
       x[i] = s < p.count ? reinterpret_cast<const float4*>(a.part_o)[place(s) * 16 + quad] : make_float4(0, 0, 0, 0);
     }
+    __shared__ float s_x[2 * kWarps];
     float turn, L;
-    join_row<KIND, EXACT>(a, p, sink, turn, L);
+    join_row<KIND, EXACT, FORM == kWide ? kWarps : 1>(a, p, sink, s_x, turn, L);
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
     // a part that saw nothing has the reference -inf and zeros; one that saw only
     // NaN has -inf too, and its sums are NaN, which a factor of zero keeps
@@ -946,7 +972,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
     __syncthreads();
     for (int r = threadIdx.x >> 5; r < nr; r += kWarps) {
       float turn, L;
-      join_row<KIND, EXACT>(a, Parts(a, pv, line, b, h, len, r0 + r), sink_score(a, h, r0 + r), turn, L);
+      join_row<KIND, EXACT, 1>(a, Parts(a, pv, line, b, h, len, r0 + r), sink_score(a, h, r0 + r), nullptr, turn, L);
       s_turn[r] = turn;
       s_inv[r] = row_scale(L);
     }
@@ -1082,13 +1108,19 @@ int paged_launch(PagedAttnArgs& a, const PagedView& pv, cudaStream_t st) {
                            : attn_launch<FmaEngine<KIND, 8>>(a, pv, st);
   if (e) return e;
   if (a.cluster) return ALGX_OK;
-  const bool narrow = (int64_t)a.B * pv.heads * a.rows > kSms * 8;
-  const int64_t row_blocks = narrow ? (a.rows + kWarps - 1) / kWarps : a.rows;
-  const int64_t blocks = row_blocks + (a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0);
-  const int64_t grid = blocks * a.B * pv.heads;
+  const int64_t heads = (int64_t)a.B * pv.heads;
+  const int64_t score_blocks = a.xs ? (a.slots + kScoreSlots - 1) / kScoreSlots : 0;
+  const bool few = heads * (a.rows + score_blocks) <= kSms && (a.xs || a.warps > 64 * heads * a.tiles);
+  const int form = heads * a.rows > kSms * 8 ? kNarrow : few ? kWide : kUsual;
+  const int64_t row_blocks = form == kNarrow ? (a.rows + kWarps - 1) / kWarps : a.rows;
+  const int64_t blocks = row_blocks + score_blocks;
+  const int64_t grid = blocks * heads;
   ALGX_REQUIRE(grid <= INT32_MAX, "too many rows");
-  ALGX_CUDA(launch_dependent(narrow ? paged_join_kernel<T, KIND, true> : paged_join_kernel<T, KIND, false>,
-                             dim3((unsigned)grid), dim3(kThreads), 0, st, a, pv, (int)blocks, (int)row_blocks));
+  auto* join = form == kNarrow ? paged_join_kernel<T, KIND, kNarrow>
+               : form == kWide ? paged_join_kernel<T, KIND, kWide>
+                               : paged_join_kernel<T, KIND, kUsual>;
+  ALGX_CUDA(launch_dependent(join, dim3((unsigned)grid), dim3(join_threads(form)), 0, st, a, pv, (int)blocks,
+                             (int)row_blocks));
   ALGX_LAUNCHED("paged_join_kernel");
   return ALGX_OK;
 }

@@ -149,6 +149,13 @@ def test_attention_long_cache_of_many_splits():
     check_attention(B=1, T=1, Hq=2, Hkv=1, page=64, lens=[9001], dtype=BF16, kind="asinh", seed=3, scored=True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,T,lens,sink", [(1, 1, [40007], False), (2, 3, [9001, 0], True)])
+def test_attention_few_rows_of_many_parts(B, T, lens, sink, dtype):
+    """A few rows of hundreds of partial results, and of none."""
+    check_attention(B=B, T=T, Hq=2, Hkv=1, page=128, lens=lens, dtype=dtype, kind="asinh", seed=4, sink=sink)
+
+
 def test_attention_rows_see_nothing_of_later_tokens():
     """Infinities and NaN in the newest token's key and value stay out of the earlier tokens' outputs."""
     B, T, H, page = 1, 3, 2, 16
