@@ -473,7 +473,12 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   // 56.5, 54.6, 57.3 us with one to five positions first, 60 with all; two CTAs of 512
   // threads an SM took 100 instead of 74 at an earlier step. One sequence: 25 us over
   // 8 SMs, 17 over 16.)
-  const bool few = B * 16 <= 148, wide = B * 8 <= 2 * 148;
+  //
+  // Clusters of 16 only where a thread of 8 CTAs would read 96 logits or more. (16
+  // CTAs and 8: one user's 4 drafts over 50304 10.9 us and 13.9, 7 drafts over 32000
+  // 10.4 and 12.4; 4 drafts over 32000 with alg_ce 17.8 and 16.6, 9 sequences of one
+  // draft over 3968 24.2 and 10.4.)
+  const bool wide = B * 8 <= 2 * 148, few = B * 16 <= 148 && (2 * K + 1) * V >= 96 * 8 * 512;
   const int64_t cluster = few ? 16 : 8;
   a.round = wide ? (int)K + 1 : 4;
   a.slice = ((V + cluster - 1) / cluster + 7) / 8 * 8;

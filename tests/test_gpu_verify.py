@@ -49,6 +49,13 @@ def test_verify(B, K, V, kind, n, c, dtype):
 
 
 @pytest.mark.parametrize("kind", ["ce", "alg_ce"])
+@pytest.mark.parametrize("B,K,V", [(1, 3, 50304), (3, 31, 6241), (3, 31, 6242), (9, 1, 3968)])
+def test_few_sequences_over_either_size_of_cluster(B, K, V, kind):
+    """The number of CTAs a sequence depends on how much there is to read."""
+    check(*inputs(B, K, V, F32, kind, 2.0, 20 + K, n=8), kind=kind, n=8, c=2.0)
+
+
+@pytest.mark.parametrize("kind", ["ce", "alg_ce"])
 def test_sampling_without_drafts(kind):
     target, tokens, _, u, race = inputs(6, 0, 999, F32, kind, 2.0, 1)
     check(target, tokens, None, u, race, kind=kind, n=8, c=2.0)
