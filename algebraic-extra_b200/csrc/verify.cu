@@ -471,8 +471,7 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   // first, as rows behind a refusal are mostly not read, and smaller CTAs, four
   // an SM, which leave less of a last wave. (64 sequences of 7 drafts: 60.8, 55.8,
   // 56.5, 54.6, 57.3 us with one to five positions first, 60 with all; two CTAs of 512
-  // threads an SM took 100 instead of 74 at an earlier step. One sequence: 25 us over
-  // 8 SMs, 17 over 16.)
+  // threads an SM took 100 instead of 74 at an earlier step.)
   //
   // Clusters of 16 only where a thread of 8 CTAs would read 96 logits or more. (16
   // CTAs and 8: one user's 4 drafts over 50304 10.9 us and 13.9, 7 drafts over 32000
