@@ -524,7 +524,8 @@ int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const i
                "NULL tensor");
   ALGX_REQUIRE(scores != new_scores && positions != new_positions && lens != new_lens,
                "the new scores, positions and lengths need their own buffers");
-  ALGX_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)scores | (uintptr_t)positions) & 15) == 0 &&
+  ALGX_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)scores | (uintptr_t)positions |
+                  (uintptr_t)new_scores | (uintptr_t)new_positions) & 15) == 0 &&
                    ((uintptr_t)workspace & 7) == 0,
                "tensors must be 16-byte aligned");
   ALGX_REQUIRE(workspace && workspace_bytes >= algx_cache_evict_workspace_size(B, Hkv, budget),

@@ -407,7 +407,8 @@ ALGX_API size_t algx_cache_evict_workspace_size(int64_t B, int64_t Hkv, int64_t 
  * (B, Hkv, S; 0 and -1 beyond the new length) describe the result, kept
  * (B, Hkv, budget) the old slot of every new one (-1: none). The new arrays are
  * buffers of their own, so a call repeated on the same inputs gives the same
- * result. No counterpart in the reference. */
+ * result. Scores and positions, old and new, start at 16-byte boundaries. No
+ * counterpart in the reference. */
 ALGX_API int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const int32_t* lens,
                               const float* scores, const int32_t* positions, int64_t budget, int64_t first,
                               int64_t recent, int32_t* new_lens, float* new_scores, int32_t* new_positions,
