@@ -446,7 +446,8 @@ int paged_view(PagedView* pv, const void* table, const void* lens, int64_t B, in
   ALGX_REQUIRE(B >= 0 && Hkv >= 1 && num_pages >= 1 && max_pages >= 1, "paged cache sizes must be positive");
   ALGX_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
                "page_size must be a power of two from 16 to 256");
-  ALGX_REQUIRE(num_pages <= INT32_MAX && max_pages * page_size <= INT32_MAX, "paged cache too large");
+  // slots are counted in 32 bits, up to the end of the group of 32 that holds the last one
+  ALGX_REQUIRE(num_pages <= INT32_MAX && max_pages <= (INT32_MAX - 64) / page_size, "paged cache too large");
   ALGX_REQUIRE(B * Hkv <= INT32_MAX, "too many sequences");
   pv->table = static_cast<const int32_t*>(table);
   pv->lens = static_cast<const int32_t*>(lens);
@@ -519,6 +520,13 @@ int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const i
   ALGX_REQUIRE(budget >= 1 && budget <= INT32_MAX, "budget must be positive");
   ALGX_REQUIRE(first >= 0 && recent >= 0 && first <= budget && recent <= budget - first,
                "first + recent must fit the budget");
+  const int64_t S = page_size * max_pages;
+  // Rows an item can move at most.
+  const int64_t most = std::min<int64_t>(budget, std::max<int64_t>(0, S - budget));
+  // The kernels count slots and 16-byte pieces of moved rows in 32 bits, up to a step past the end.
+  const int64_t lanes = dtype == ALGX_BF16 ? 8 : 16;
+  ALGX_REQUIRE(S <= INT32_MAX - kEvChunk && budget <= INT32_MAX - kEvThreads && most * lanes <= INT32_MAX - 2 * kMovePieces,
+               "paged cache too large");
   if (B == 0) return ALGX_OK;
   ALGX_REQUIRE(k_pages && v_pages && scores && positions && new_lens && new_scores && new_positions && kept,
                "NULL tensor");
@@ -536,15 +544,12 @@ int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const i
   a.moves = static_cast<int2*>(workspace);
   a.counts = reinterpret_cast<int*>(a.moves + B * Hkv * budget);
   a.budget = (int)budget; a.first = (int)first; a.recent = (int)recent;
-  a.lanes = dtype == ALGX_BF16 ? 8 : 16;
+  a.lanes = (int)lanes;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
-  const int64_t S = page_size * max_pages;
-  // Rows an item can move at most. Up to kInplace of them its own CTA moves them,
-  // which saves a launch (12 items of at most 512 rows: 11 us a pass in one launch);
-  // more are spread over the device (192 items of 2050 rows: 69 us a pass in two
-  // launches, 138 in one).
-  const int64_t most = std::min<int64_t>(budget, std::max<int64_t>(0, S - budget));
+  // Up to kInplace rows an item's own CTA moves them, which saves a launch (12
+  // items of at most 512 rows: 11 us a pass in one launch); more are spread over the
+  // device (192 items of 2050 rows: 69 us a pass in two launches, 138 in one).
   a.inplace = most <= kInplace;
   a.cached = S <= kEvCached;
   const size_t smem = a.cached ? (size_t)S * sizeof(uint32_t) : 0;

@@ -341,7 +341,7 @@ ALGX_API int algx_aluglu_bwd(const void* gu, const void* dy, void* dgu, int64_t 
  * 256. table (B, max_pages) int32 names each sequence's pages, lens (B) int32
  * its cached slots; slot s lies in page table[b][s / page_size] at row
  * s % page_size. Entries of the table beyond a sequence's slots are not read.
- * S = max_pages * page_size below. A page number, a length or a rotary position
+ * S = max_pages * page_size below, at most 2^31 - 65. A page number, a length or a rotary position
  * outside its range never leads to an access out of bounds: what it would have
  * touched is skipped (a length is cut to S, a position to the tables' rows) and
  * the device error word gets bit 8. The reference trains only; none of these
@@ -407,8 +407,10 @@ ALGX_API size_t algx_cache_evict_workspace_size(int64_t B, int64_t Hkv, int64_t 
  * (B, Hkv, S; 0 and -1 beyond the new length) describe the result, kept
  * (B, Hkv, budget) the old slot of every new one (-1: none). The new arrays are
  * buffers of their own, so a call repeated on the same inputs gives the same
- * result. Scores and positions, old and new, start at 16-byte boundaries. No
- * counterpart in the reference. */
+ * result. Scores and positions, old and new, start at 16-byte boundaries. Refused
+ * as too large: S above 2^31 - 2049, a budget above 2^31 - 513, or more than
+ * 2^28 - 257 (bf16) or 2^27 - 129 (fp32) rows to move a head (the lesser of
+ * budget and S - budget). No counterpart in the reference. */
 ALGX_API int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table, const int32_t* lens,
                               const float* scores, const int32_t* positions, int64_t budget, int64_t first,
                               int64_t recent, int32_t* new_lens, float* new_scores, int32_t* new_positions,

@@ -35,3 +35,33 @@ def test_evict_needs_aligned_scores_and_positions(name, off):
     """They are read and written four elements at a time."""
     status, message = evict(**{name: off})
     assert status == L.ALGX_ERR_INVALID and "16-byte aligned" in message
+
+
+@pytest.mark.parametrize("page_size,max_pages,budget,dtype", [
+    (256, 2 ** 20, 2 ** 31 - 513, L.ALGX_BF16),
+    (256, 2 ** 23 - 9, 2 ** 28 - 257, L.ALGX_BF16),
+    (256, 2 ** 23 - 9, 2 ** 27 - 129, L.ALGX_F32),
+])
+def test_evict_counts_in_32_bits(page_size, max_pages, budget, dtype):
+    """The largest tables and budgets whose slots and pieces of moved rows the kernels' 32-bit counters hold, and one
+    more (below it a budget leaves rows to move, which bound it earlier)."""
+    sizes = dict(page_size=page_size, max_pages=max_pages, dtype=dtype)
+    assert "workspace too small" in evict(budget=budget, **sizes)[1]
+    status, message = evict(budget=budget + 1, **sizes)
+    assert status == L.ALGX_ERR_INVALID and "too large" in message
+
+
+def test_evict_of_tables_near_32_bits():
+    assert "workspace too small" in evict(page_size=16, max_pages=(2 ** 31 - 2049) // 16, budget=8)[1]
+    assert "too large" in evict(page_size=16, max_pages=(2 ** 31 - 2049) // 16 + 1, budget=8)[1]
+
+
+def test_attention_counts_groups_of_slots_in_32_bits():
+    """A sequence's last group of 32 slots ends below 2^31."""
+    lib = L.lib()
+    cfg = L.PagedConfig(0, 16, 0, 0, 1.0, 1.0)
+    call = lambda pages: lib.algx_paged_attn(cfg, *[None] * 9, 0, 1, 2, 2, 1, 16, pages, 64, L.ALGX_BF16, None, 0,  # noqa: E731
+                                             None)
+    assert call(2 ** 27 - 5) == L.ALGX_OK
+    for pages in (2 ** 27 - 4, 2 ** 27 - 1, 2 ** 60):
+        assert call(pages) == L.ALGX_ERR_INVALID and b"too large" in lib.algx_last_error()
