@@ -994,6 +994,18 @@ __global__ void __launch_bounds__(join_threads(FORM)) paged_join_kernel(const Pa
   }
 }
 
+// Scores of a call without tokens: those of the cached slots stay, the others are zero.
+__global__ void __launch_bounds__(256) paged_scores_kernel(const PagedAttnArgs a, const PagedView pv) {
+  pdl_wait();
+  const int64_t all = (int64_t)a.B * pv.heads * a.slots;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t bh = i / a.slots, s = i - bh * a.slots;
+    const int len = pv.lens[bh / pv.heads];
+    if (s == 0 && len > a.slots) atomicOr(a.err, DEV_ERR_BAD_PAGE);
+    a.scores_out[i] = s < len ? a.scores[i] : 0.f;
+  }
+}
+
 // ------------------------------------------------------------------------ host
 struct Plan {
   int64_t rows, tile_rows, tiles, items, warps;
@@ -1151,9 +1163,21 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
                "n must be a power of two");
   ALGX_REQUIRE(T >= 0 && Hq >= 1 && Hq % Hkv == 0, "query heads must be a multiple of the cache's heads");
   ALGX_REQUIRE(cfg->window >= 0 && cfg->first >= 0, "window and first must not be negative");
-  if (B == 0 || T == 0) return ALGX_OK;
-  ALGX_REQUIRE(q && k_pages && v_pages && o, "NULL tensor");
   ALGX_REQUIRE((scores == nullptr) == (scores_out == nullptr), "give scores and scores_out or neither");
+  if (B == 0 || (T == 0 && scores == nullptr)) return ALGX_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    PagedAttnArgs a = {};
+    a.scores = scores; a.scores_out = scores_out; a.B = (int)B; a.slots = page_size * max_pages;
+    a.err = device_error_word();
+    ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");
+    const int64_t blocks = (B * Hkv * a.slots + 1023) / 1024;
+    ALGX_CUDA(launch_dependent(paged_scores_kernel, dim3((unsigned)std::min<int64_t>(blocks, kSms * 8)), dim3(256), 0, st,
+                               a, pv));
+    ALGX_LAUNCHED("paged_scores_kernel");
+    return ALGX_OK;
+  }
+  ALGX_REQUIRE(q && k_pages && v_pages && o, "NULL tensor");
   ALGX_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)workspace) & 15) == 0,
                "tensors must be 16-byte aligned");
   ALGX_REQUIRE(T <= INT32_MAX && T * (Hq / Hkv) <= INT32_MAX / 64, "too many rows");
@@ -1179,7 +1203,6 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   a.sight = {cfg->window, cfg->first};
   a.shift = dtype == ALGX_BF16 ? 5 : 4;
   a.least = (dtype == ALGX_BF16 ? kMinSlotsBf16 : kMinSlotsF32) >> a.shift;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == ALGX_BF16)
     return soft ? paged_launch<__nv_bfloat16, kSoftmax>(a, pv, st) : paged_launch<__nv_bfloat16, kAsinh>(a, pv, st);
   return soft ? paged_launch<float, kSoftmax>(a, pv, st) : paged_launch<float, kAsinh>(a, pv, st);

@@ -388,7 +388,7 @@ ALGX_API size_t algx_paged_attn_workspace_size(int64_t B, int64_t T, int64_t Hq,
  * gives zeros. scores, scores_out (B, Hkv, S) fp32 or both NULL (they may be
  * the same buffer): scores_out = scores + this call's normalised weights summed
  * over the queries of each kv head; slots of the T new tokens start from 0, and
- * slots beyond lens get 0. No counterpart in the reference for the cache. */
+ * slots beyond lens get 0 (with T = 0 that is all a call does). No counterpart in the reference for the cache. */
 ALGX_API int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_pages, const void* v_pages,
                              const int32_t* table, const int32_t* lens, const float* sink, const float* scores,
                              float* scores_out, void* o, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,

@@ -418,3 +418,21 @@ def test_unaligned_inputs_are_copied():
     odd.copy_(a)
     assert torch.equal(paged_attention(odd, *caches[0], table.cuda(), lens + 1),
                        paged_attention(a, *caches[0], table.cuda(), lens + 1))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_scores_of_a_call_without_tokens(in_place, dtype):
+    """The cached slots' scores as they were, zeros beyond them."""
+    k, v, table, g = make_cache(3, 2, 16, 70, dtype, 15)
+    S = 70 * 16
+    scores = torch.rand((3, 2, S), generator=g)
+    lens = [0, 1, 777]
+    want = torch.where(torch.arange(S) < torch.tensor(lens)[:, None, None], scores, 0.0)
+    sc = scores.cuda()
+    out = sc if in_place else torch.full_like(sc, math.nan)
+    q = torch.empty((3, 0, 4, 64), dtype=dtype, device="cuda")
+    o, got = paged_attention(q, k.cuda(), v.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                             scores=sc, scores_out=out)
+    assert o.shape == (3, 0, 4, 64) and got.data_ptr() == out.data_ptr()
+    assert torch.equal(got.cpu(), want) and L.device_error() == 0
