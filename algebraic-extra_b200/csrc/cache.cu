@@ -326,7 +326,8 @@ __global__ void __launch_bounds__(kEvThreads, 2) cache_evict_kernel(const EvictA
     if (lane == 0) atomicMax(&s_newest, newest);
     __syncthreads();
     const int64_t from = (int64_t)s_newest - a.recent;  // positions above it are recent
-    auto key = [&](float x, int p) { return score_key(p < a.first || p > from ? __int_as_float(0x7f800000) : x); };
+    // protected slots stand above every score, an infinite one too (0xff800000)
+    auto key = [&](float x, int p) { return p < a.first || p > from ? 0xffffffffu : score_key(x); };
     auto make_keys = [&](int s) {
       const float4 x = *reinterpret_cast<const float4*>(scores + s);
       const int4 p = *reinterpret_cast<const int4*>(positions + s);

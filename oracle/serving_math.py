@@ -105,11 +105,11 @@ def evict_plan(scores, positions, length: int, budget: int, first: int, recent: 
         return list(range(length))
     newest = max(int(p) for p in positions[:length])
 
-    def rank(s):
+    def rank(s):  # protected slots, then scores from the highest on, then NaN
         p, x = int(positions[s]), float(scores[s])
         if p < first or p > newest - recent:
-            x = math.inf
-        return (1 if math.isnan(x) else 0, 0.0 if math.isnan(x) else -x, s)
+            return (0, 0.0, s)
+        return (2, 0.0, s) if math.isnan(x) else (1, -x, s)
 
     keep = sorted(sorted(range(length), key=rank)[:budget])
     held = set(keep)

@@ -373,6 +373,14 @@ def test_evict_odd_scores():
     check_evict(2, 2, 16, [128, 77], 50, 1, 3, BF16, 50, scores=scores)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_evict_keeps_protected_slots_above_infinite_scores(dtype):
+    """Infinite scores in the low slots, more of them than the budget has room for beside the protected positions."""
+    scores = torch.rand((2, 2, 160), generator=torch.Generator().manual_seed(2))
+    scores[:, :, :100] = math.inf
+    check_evict(2, 2, 16, [160, 131], 40, 5, 20, dtype, 51, scores=scores)
+
+
 def test_evict_of_no_sequences():
     k, v, _, _ = make_cache(1, 2, 16, 2, BF16, 13)
     table = torch.empty((0, 2), dtype=torch.int32, device="cuda")
