@@ -46,7 +46,22 @@ struct VerifyArgs {
   int K, log2n;
   int round;  // draft positions looked at in the first round
   float scale;  // 1 / temperature (ce) or 1 / c (alg_ce)
+  float margin;  // of the race's fast weights, relative (race_margin)
 };
+
+// How far the race's fast weights may be from the exact ones that decide, relative to
+// themselves, with u = 2^-24. alg_ce: root and reciprocal of 2 u each, a sum and a
+// product of u make 6 u for the fast form of rho(x) turn, 4 u for the exact one, 10 u
+// together, n times that in the power, whose squarings add less than n u a side;
+// 12 n u + 12 u for the factors after it is below 2^-19 n from n = 2 on (measured:
+// 7.5 n u at most). ce: the argument, at most 126 in units of log2(e), is rounded to
+// 2^-18, its factor to 2 u, the exact form's to 2^-18: 2^-16 of a weight, 2^-14 with
+// the factors after it to spare. Below 2^-126 the fast forms flush to zero: kFlushed
+// bounds that.
+constexpr float kFlushed = 0x1p-125f;
+inline float race_margin(int32_t kind, int32_t n) {
+  return kind == ALGX_HEAD_CE ? 0x1p-14f : std::min(1.f, (float)n * 0x1p-19f);
+}
 
 // The score of a logit: the logit itself for ce, so that differences from the
 // maximum are exact, z / c for alg_ce. NaN counts as -inf.
@@ -315,18 +330,17 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
   };
   // pass 0 races over the residual; where nothing of it is left, pass 1 over p
   for (int pass = acc < K ? 0 : 1; pass < 2; ++pass) {
-    // The fast weights err by less than 2^-16 of themselves (2^-22 a factor, 32
-    // factors), which bounds every ratio from both sides. A lane keeps the column
-    // that no other can be above; only where two overlap are they evaluated
-    // exactly, and at the end the lanes that could hold the winner.
+    // The fast weights' error (race_margin) bounds every ratio from both sides. A
+    // lane keeps the column that no other can be above; only where two overlap are
+    // they evaluated exactly, and at the end the lanes that could hold the winner.
     float low = 0.f, up = 0.f, xp_b = kNegInf, xq_b = kNegInf, e_b = 1.f;
     int64_t v_b = min(begin + threadIdx.x, a.V - 1);
     auto enter = [&](int64_t v, float z, float zd, float e) {
       const float xp = score_of<KIND>(a, z), xq = score_of<KIND>(a, zd);
       const float2 f = fast_weights<KIND, LOG2N>(a, make_float2(xp, xq), make_float2(turn_p, turn_q));
       const float p = f.x * inv_p, q = pass == 1 ? 0.f : row_q ? f.y * inv_q : v == drafted ? 1.f : 0.f;
-      const float r = rcp_fast(e), mid = (p - q) * r, off = (p + q) * r * 0x1p-16f;
-      if (!(mid + off > low) || !(mid + off > 0.f)) return;
+      const float r = rcp_fast(e), mid = (p - q) * r, off = fmaf(p + q, a.margin, kFlushed) * r;
+      if (!(mid + off > low) || !(xp > kNegInf)) return;  // the latter: no probability
       bool take = mid - off > up;
       float lo = mid - off, hi = mid + off;
       if (!take) {
@@ -462,6 +476,7 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   a.target = target; a.draft = K > 0 ? draft : nullptr; a.tokens = tokens; a.counts = counts; a.u = u; a.race = race;
   a.out = out; a.accepted = accepted; a.V = V; a.K = (int)K;
   a.scale = scale;
+  a.margin = race_margin(kind, n);
   while ((1 << a.log2n) < n) ++a.log2n;
   a.err = device_error_word();
   ALGX_REQUIRE(a.err != nullptr, "device error word unavailable");

@@ -133,3 +133,55 @@ def test_tokens_have_the_target_distribution():
     freq = torch.bincount(out[:, 0].cpu().long(), minlength=V) / B
     prob = torch.softmax(p, -1)
     assert bool(((freq - prob).abs() < 6 * torch.sqrt(prob * (1 - prob) / B)).all())
+
+
+def test_the_residual_may_be_smaller_than_normal_numbers():
+    """A refusal whose residual is nothing but probabilities below 2^-126: the draw is among those."""
+    V = 3000
+    target, draft = torch.full((2, 2, V), -95.0), torch.full((2, 1, V), -math.inf)
+    target[:, :, 17], draft[:, :, 17] = 0.0, 0.0
+    tokens, u = torch.full((2, 1), 17, dtype=torch.int32), torch.ones((2, 1))
+    race = 0.5 + torch.rand((2, V), generator=torch.Generator().manual_seed(9))
+    race[0, 2001], race[1, 5] = 1e-3, 1e-3
+    check(target, tokens, draft, u, race)
+    assert verify_draft(*(t.cuda() for t in (target, tokens, draft, u, race)))[0][:, 0].tolist() == [2001, 5]
+
+
+def exact_weights(z, n):
+    """(rho(z) rho(-max))^n as float32 arithmetic with correctly rounded operations gives it."""
+    import numpy as np
+
+    def rho32(x):
+        rad = (x.astype(np.float64) ** 2 + 1).astype(np.float32)
+        t = np.abs(x) + np.sqrt(rad)
+        return np.where(x >= 0, t, np.float32(1) / t)
+
+    z = z.numpy()
+    w = rho32(z) * rho32(-z.max(axis=-1, keepdims=True))
+    for _ in range(n.bit_length() - 1):
+        w = w * w
+    assert w.dtype == np.float32
+    return torch.from_numpy(w.astype(np.float64))
+
+
+@pytest.mark.parametrize("n", [8, 32, 64, 256])
+def test_close_races_are_decided_exactly(n):
+    """Columns whose ratios lie within 1e-5 of each other, the winner 4e-6 above the rest (the sum's rounding and
+    those of two divisions are 2e-7): powers above 32 are the C entry's."""
+    B, V = 24, 4000
+    g = torch.Generator().manual_seed(10 + n)
+    half = 0.3 if n <= 64 else 0.1  # no weight below 1e-23
+    z = (2 * half * torch.rand((B, V), generator=g) - half).float()
+    z[:, ::4] = half  # the row's maximum in every 16 bytes: whichever the kernel refers its weights to is this one
+    w = exact_weights(z, n)
+    best = torch.randint(0, V, (B,), generator=g)
+    gap = 4e-6 + 6e-6 * torch.rand((B, V), generator=g, dtype=torch.float64)
+    gap[torch.arange(B), best] = 0.0
+    race = (w / w.sum(dim=-1, keepdim=True) * V * (1 + gap)).float()
+    # the variates' own rounding, 2^-24, is part of the inputs
+    out, accepted = torch.empty((B, 1), dtype=torch.int32, device="cuda"), torch.empty(B, dtype=torch.int32, device="cuda")
+    zd, rd = z[:, None].contiguous().cuda(), race.cuda()
+    torch.cuda.synchronize()
+    L.check(L.lib().algx_verify_draft(L.ALGX_HEAD_ALG_CE, n, 1.0, zd.data_ptr(), None, None, None, None, rd.data_ptr(),
+                                      out.data_ptr(), accepted.data_ptr(), B, 0, V, L.ALGX_F32, L.stream_of(zd)), "verify")
+    assert out[:, 0].tolist() == best.tolist() and accepted.tolist() == [0] * B
