@@ -82,8 +82,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: 
     first ones of the sequence. ``kind``, ``n``, ``c`` and ``sink_logit``
     (broadcastable to (Hq,)) are those of
     ``algx.kernels.flash.flash_attention``; the asinh kind is evaluated against a
-    running maximum, so any score range is safe. A query that sees nothing gives
-    zeros.
+    running maximum, so any score whose square float32 holds (below 2^63) is safe.
+    A query that sees nothing gives zeros.
 
     ``scores`` (B, Hkv, max_pages * page_size) float32: the weight every slot
     has received; the call adds its own normalised weights, summed over the

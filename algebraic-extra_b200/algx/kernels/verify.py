@@ -49,8 +49,8 @@ def verify_draft(target_logits, draft_tokens, draft_logits, accept_u, race, *, k
     first refusal the next token is drawn from max(p - q, 0) of that row, after
     K acceptances from row K, as the argmax of weight / race (ties: the lowest
     index). Probabilities are float32 numbers (below 2^-150: zero); -inf logits
-    have probability 0, and so have NaN ones. ``temperature``
-    divides the logits of the ``ce`` kind. ``counts`` (B,) int32: drafts of each
+    have probability 0, and so have NaN ones; alg_ce takes ``|z / c|`` below 2^63,
+    whose square float32 holds. ``temperature`` divides the logits of the ``ce`` kind. ``counts`` (B,) int32: drafts of each
     sequence where not all have K (row ``counts[b]`` is then the one after).
 
     ``tokens`` (B, K + 1) int32 holds the accepted drafts, the token drawn, then

@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -101,8 +102,13 @@ struct RowSum {
   float2 l;
   __device__ __forceinline__ void clear() {
     m = kNegInf;
-    turn = weight_turn<KIND, true>(kNegInf);
+    turn = KIND == kSoftmax ? -FLT_MAX : weight_turn<KIND, true>(kNegInf);
     l = make_float2(0.f, 0.f);
+  }
+  // The score that l is relative to. Before the reference has moved, ce weights are
+  // relative to the lowest finite logit, so a row of nothing else counts too.
+  __device__ __forceinline__ float reference() const {
+    return KIND == kSoftmax && m == kNegInf && l.x + l.y > 0.f ? -FLT_MAX : m;
   }
   // CLEAN: NaN logits count as -inf. Without it one spoils the sum, which then is
   // taken again with it.
@@ -275,10 +281,11 @@ __global__ void __launch_bounds__(kThreads, kCluster == 16 ? 1 : 1024 / kThreads
       };
       add_up(std::false_type{});
       if (__any_sync(0xffffffffu, !(sum.l.x + sum.l.y < INFINITY))) add_up(std::true_type{});
-      float M = sum.m;
+      const float mine = sum.reference();
+      float M = mine;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-      float L = sum.m == kNegInf ? 0.f : (sum.l.x + sum.l.y) * fast_weight<KIND>(a, sum.m, weight_turn<KIND, true>(M));
+      float L = mine == kNegInf ? 0.f : (sum.l.x + sum.l.y) * fast_weight<KIND>(a, mine, weight_turn<KIND, true>(M));
       L = row_sum<32>(L);
       if (lane == 0) s_part[warp + r] = make_float2(M, L);
     }

@@ -98,6 +98,24 @@ def test_masked_and_odd_logits(kind):
     check(target, tokens, draft, u, race, kind=kind, n=16, c=2.0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("K", [0, 2])
+def test_rows_of_the_lowest_finite_logits(K, dtype):
+    """Masks of the type's lowest value: beside other logits they have no probability, alone they are as likely as
+    each other."""
+    low = torch.finfo(dtype).min
+    target, tokens, draft, u, race = inputs(6, K, 700, dtype, "ce", 1.0, 12)
+    target[0] = low
+    target[1, :, 40:] = low
+    target[2, :, :699] = low
+    target[3, :, ::2], target[3, :, 1::2] = low, -math.inf
+    target[4] = -3e38 if dtype == F32 else low
+    draft[:4:2] = low
+    draft[5, :, 5:] = low
+    check(target, tokens, draft if K else None, u, race)
+    check(target, tokens, draft if K else None, u, race, temperature=1e38)
+
+
 def test_draft_tokens_outside_the_vocabulary_are_refused():
     target, tokens, draft, u, race = inputs(3, 3, 400, BF16, "ce", 1.0, 6)
     tokens[0, 0], tokens[1, 2] = -1, 400
