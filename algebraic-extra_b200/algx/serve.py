@@ -133,7 +133,18 @@ class Decoder:
             self.slot_positions = torch.full(shape, -1, dtype=torch.int32, device=dev)
         if cfg.sink == "const":
             self._sink = torch.full((cfg.n_heads,), cfg.sink_init, dtype=torch.float32, device=dev)
-        self.last = None              # (batch, V) float32 logits of the newest token
+        self._scored = None           # logits (batch, rows, V) of the newest tokens, each sequence's newest row
+
+    @property
+    def last(self):
+        """(batch, V) float32 logits of every sequence's newest token; None before any, and where a rollback
+        went behind the tokens of the last step."""
+        if self._scored is None:
+            return None
+        logits, rows = self._scored
+        if min(rows) == logits.shape[1] - 1:
+            return logits[:, -1]
+        return logits[torch.arange(self.batch, device=logits.device), torch.tensor(rows, device=logits.device)]
 
     # ------------------------------------------------------------ layers
     def _sink_of(self, i):
@@ -199,7 +210,7 @@ class Decoder:
 
         logits = self._logits(self._layers(tokens, attend)).view(B, T, -1)
         self._advance([T] * B)
-        self.last = logits[:, -1]
+        self._scored = logits, [T - 1] * B
         return logits
 
     def _advance(self, by):
@@ -214,6 +225,10 @@ class Decoder:
             raise ValueError("cannot drop more tokens than are cached")
         self._advance([-int(d) for d in drop])
         self.cache.trim(self.lens)
+        if self._scored is not None:
+            logits, rows = self._scored
+            rows = [r - int(d) for r, d in zip(rows, drop)]
+            self._scored = (logits, rows) if min(rows) >= 0 else None
 
     @torch.no_grad()
     def prefill(self, prompts: Sequence[Sequence[int]]):
@@ -253,8 +268,9 @@ class Decoder:
 
         h = self._layers(tokens, attend)
         self._advance(sizes)
-        self.last = self._logits(h[torch.arange(self.batch, device=dev), counts.long() - 1])
-        return self.last
+        last = self._logits(h[torch.arange(self.batch, device=dev), counts.long() - 1])
+        self._scored = last[:, None], [0] * self.batch
+        return last
 
     def _prefill_steps(self, prompts, sizes, chunk: int = 64):
         dev = self.cache.k.device
@@ -278,7 +294,7 @@ class Decoder:
             last = new if last is None else torch.where(fed, new, last)
             done = [d + t for d, t in zip(done, take)]
             self.evict()
-        self.last = last
+        self._scored = last[:, None], [0] * self.batch
         return last
 
     @torch.no_grad()
@@ -323,7 +339,7 @@ def sample(logits, cfg, generator=None, temperature: float = 1.0):
 def generate(dec: Decoder, new_tokens: int, *, generator=None, temperature: float = 1.0):
     """``new_tokens`` sampled tokens per sequence, (B, new_tokens) int32, after ``dec.prefill``."""
     if dec.last is None:
-        raise ValueError("prefill first")
+        raise ValueError("the newest tokens' logits are not known: feed one with step" if any(dec.seen) else "prefill first")
     out = []
     for i in range(new_tokens):
         t = sample(dec.last, dec.cfg, generator, temperature)
