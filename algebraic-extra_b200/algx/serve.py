@@ -134,6 +134,7 @@ class Decoder:
         if cfg.sink == "const":
             self._sink = torch.full((cfg.n_heads,), cfg.sink_init, dtype=torch.float32, device=dev)
         self._scored = None           # logits (batch, rows, V) of the newest tokens, each sequence's newest row
+        self.pending = None           # (batch,) the tokens that generate returned last, not fed yet
 
     @property
     def last(self):
@@ -214,6 +215,7 @@ class Decoder:
         return logits
 
     def _advance(self, by):
+        self.pending = None
         self.lens = [n + t for n, t in zip(self.lens, by)]
         self.seen = [n + t for n, t in zip(self.seen, by)]
         self.cache.lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
@@ -337,7 +339,17 @@ def sample(logits, cfg, generator=None, temperature: float = 1.0):
 
 @torch.no_grad()
 def generate(dec: Decoder, new_tokens: int, *, generator=None, temperature: float = 1.0):
-    """``new_tokens`` sampled tokens per sequence, (B, new_tokens) int32, after ``dec.prefill``."""
+    """``new_tokens`` sampled tokens per sequence, (B, new_tokens) int32, after ``dec.prefill``.
+
+    The last of them is not fed yet: it is ``dec.pending``, which the next call
+    feeds first, so several calls go on where the one before ended. ``step`` and
+    ``rollback`` forget it (a caller who steps feeds it with them).
+    """
+    if new_tokens < 1:
+        return torch.empty((dec.batch, 0), dtype=torch.int32, device=dec.cache.k.device)
+    if dec.pending is not None:
+        dec.step(dec.pending[:, None])
+        dec.evict()
     if dec.last is None:
         raise ValueError("the newest tokens' logits are not known: feed one with step" if any(dec.seen) else "prefill first")
     out = []
@@ -347,6 +359,7 @@ def generate(dec: Decoder, new_tokens: int, *, generator=None, temperature: floa
         if i + 1 < new_tokens:
             dec.step(t[:, None])
             dec.evict()
+    dec.pending = t
     return torch.stack(out, dim=1)
 
 

@@ -137,3 +137,37 @@ def test_logits_of_tokens_before_the_newest_step_are_not_known():
     dec.step(torch.zeros((3, 1), dtype=torch.int64))
     assert torch.equal(dec.last, newest(dec))
     assert generate(dec, 2, generator=gen()).shape == (3, 2)
+
+
+def test_generating_in_pieces_is_generating_at_once():
+    """The token that a call returned last is fed before the next one is drawn."""
+    whole = toy()
+    want = generate(whole, 11, generator=gen(1))
+    dec, g = toy(), gen(1)
+    parts = [generate(dec, n, generator=g) for n in (4, 1, 0, 6)]
+    assert torch.equal(torch.cat(parts, dim=1), want) and want.shape == (3, 11)
+    for d in (whole, dec):
+        assert [d.tokens(b) for b in range(3)] == [p + want[b, :-1].tolist() for b, p in enumerate(PROMPTS)]
+        assert torch.equal(d.pending, want[:, -1])
+
+
+def test_a_token_not_fed_yet_is_forgotten_by_steps_and_rollbacks():
+    dec = toy()
+    out = generate(dec, 3, generator=gen(2))
+    dec.step(torch.full((3, 1), 7))  # the caller goes on with a token of its own
+    assert dec.pending is None and torch.equal(dec.last, newest(dec))
+    generate(dec, 2, generator=gen(3))
+    dec.rollback([1, 0, 0])
+    assert dec.pending is None
+    dec.step(torch.full((3, 1), 8))
+    assert dec.tokens(1)[:-2] == PROMPTS[1] + out[1, :2].tolist() + [7]
+    assert generate(dec, 0).shape == (3, 0)
+
+
+def test_pieces_under_a_budget():
+    kw = dict(max_slots=48, max_positions=200, budget=24, slack=8, first=2, recent=6)
+    whole = toy(**kw)
+    want = generate(whole, 40, generator=gen(4))
+    dec, g = toy(**kw), gen(4)
+    assert torch.equal(torch.cat([generate(dec, n, generator=g) for n in (13, 20, 7)], dim=1), want)
+    assert dec.lens == whole.lens and [dec.held(b) for b in range(3)] == [whole.held(b) for b in range(3)]
