@@ -191,17 +191,26 @@ class Decoder:
 
     # ------------------------------------------------------------ tokens
     @torch.no_grad()
-    def step(self, tokens):
-        """Feed ``tokens`` (B, T) int; float32 logits (B, T, V). The new slots stay until ``rollback``."""
+    def step(self, tokens, idle: Sequence[int] = ()):
+        """Feed ``tokens`` (B, T) int; float32 logits (B, T, V). The new slots stay until ``rollback``.
+
+        The sequences named in ``idle`` sit the step out: they need no slots or
+        positions and keep their weights; their rows of the result mean nothing.
+        """
         cfg, c = self.cfg, self.cache
         B, T = tokens.shape
-        if max(self.seen) + T > self.max_positions:
+        idle = sorted(set(idle))
+        by = [0 if b in idle else T for b in range(B)]
+        if any(n and at + n > self.max_positions for n, at in zip(by, self.seen)):
             raise ValueError(f"positions end at {self.max_positions}")
-        c.reserve([n + T for n in self.lens])
-        after = c.lens + T
+        c.reserve([n + t for n, t in zip(self.lens, by)])
+        counts = torch.tensor(by, dtype=torch.int32, device=c.k.device) if idle else None
+        after = c.lens + (T if counts is None else counts)
+        known = self.last if idle else None
+        held = self.scores[:, idle].clone() if self.scores is not None and idle else None
 
         def attend(i, qkv):
-            q = self._append(i, qkv)
+            q = self._append(i, qkv, counts)
             opts = dict(kind="asinh", n=cfg.attn_n, c=cfg.attn_c)
             if self.window is not None:
                 opts.update(window=self.window, first=self.first)
@@ -210,8 +219,15 @@ class Decoder:
             return paged_attention(q, c.k[i], c.v[i], c.table, after, self._sink_of(i), scores=self.scores[i], **opts)[0]
 
         logits = self._logits(self._layers(tokens, attend)).view(B, T, -1)
-        self._advance([T] * B)
+        if held is not None:
+            self.scores[:, idle] = held
+        self._advance(by)
         self._scored = logits, [T - 1] * B
+        if idle:
+            newest = logits[:, -1].clone()
+            if known is not None:
+                newest[idle] = known[idle]
+            self._scored = None if known is None else (newest[:, None], [0] * B)
         return logits
 
     def _advance(self, by):
@@ -275,29 +291,17 @@ class Decoder:
         return last
 
     def _prefill_steps(self, prompts, sizes, chunk: int = 64):
-        dev = self.cache.k.device
-        done, last = [0] * self.batch, None
+        done = [0] * self.batch
         while any(d < n for d, n in zip(done, sizes)):
-            # the sequences advance together, by what the one nearest its end still has; those
-            # that are done take filler tokens, whose slots and weights are dropped again
-            take = [min(chunk, n - d) for d, n in zip(done, sizes)]
-            T = min(t for t in take if t > 0)
-            take = [min(t, T) for t in take]
-            idle = [b for b, t in enumerate(take) if t == 0]
-            rows = [list(p[d:d + t]) + [0] * (T - t) for p, d, t in zip(prompts, done, take)]
-            held = self.scores[:, idle].clone() if self.scores is not None and idle else None
-            logits = self.step(torch.tensor(rows, device=dev))
-            if held is not None:
-                self.scores[:, idle] = held
-            self.rollback([T - t for t in take])
-            ends = torch.tensor([max(t - 1, 0) for t in take], device=dev)
-            new = logits[torch.arange(self.batch, device=dev), ends]
-            fed = torch.tensor([t > 0 for t in take], device=dev)[:, None]
-            last = new if last is None else torch.where(fed, new, last)
-            done = [d + t for d, t in zip(done, take)]
+            # the sequences advance together, by what the one nearest its end still has
+            left = [n - d for d, n in zip(done, sizes)]
+            T = min(min(chunk, n) for n in left if n > 0)
+            idle = [b for b, n in enumerate(left) if n == 0]
+            rows = [[0] * T if b in idle else list(p[d:d + T]) for b, (p, d) in enumerate(zip(prompts, done))]
+            self.step(torch.tensor(rows, device=self.cache.k.device), idle=idle)
+            done = [d if b in idle else d + T for b, d in enumerate(done)]
             self.evict()
-        self._scored = last[:, None], [0] * self.batch
-        return last
+        return self.last
 
     @torch.no_grad()
     def evict(self, force: bool = False) -> bool:
@@ -372,36 +376,59 @@ def generate_with_draft(dec: Decoder, draft: Decoder, new_tokens: int, *, drafts
     The tokens are distributed as ``generate``'s. Each round the draft model
     samples its tokens one by one, the target scores them and the one before in a
     single pass, and ``verify_draft`` accepts a prefix and draws the token after it.
+    No sequence goes beyond its ``new_tokens``: drafts that would are not accepted,
+    and sequences that are done sit out the others' rounds (with 0 accepted). A
+    round takes slots and positions for ``drafts`` tokens that may be refused. As
+    after ``generate`` the last tokens are both decoders' ``pending``.
     """
     a, b = dec.cfg, draft.cfg
     if (a.vocab_size, a.head, a.head_n, a.head_c) != (b.vocab_size, b.head, b.head_n, b.head_c):
         raise ValueError("the draft model needs the target's vocabulary and head")
-    if dec.last is None or draft.last is None or dec.seen != draft.seen:
+    if not 1 <= drafts <= 31:
+        raise ValueError("drafts must be from 1 to 31")
+    if dec.pending is None or draft.pending is None:
+        ready = dec.pending is draft.pending and dec.last is not None and draft.last is not None
+    else:
+        ready = torch.equal(dec.pending, draft.pending)
+    if not ready or dec.seen != draft.seen:
         raise ValueError("prefill both decoders with the same prompts first")
     B, V, dev = dec.batch, a.vocab_size, dec.cache.k.device
-    newest = sample(dec.last, a, generator, temperature)
-    out = [[t] for t in newest.tolist()]
+    if new_tokens < 1:
+        return torch.empty((B, 0), dtype=torch.int32, device=dev), []
+    newest, out = dec.pending, [[] for _ in range(B)]
+    if newest is None:
+        newest = sample(dec.last, a, generator, temperature)
+        out = [[t] for t in newest.tolist()]
     rounds = []
     while min(len(o) for o in out) < new_tokens:
+        left = [new_tokens - len(o) for o in out]
+        idle = [b for b, n in enumerate(left) if n == 0]
         tokens, logits = [newest], []
         for _ in range(drafts):
-            logits.append(draft.step(tokens[-1][:, None])[:, 0])
+            logits.append(draft.step(tokens[-1][:, None], idle)[:, 0])
             tokens.append(sample(logits[-1], a, generator, temperature))
-        draft.step(tokens[-1][:, None])  # its key and value, should all drafts be accepted
+        draft.step(tokens[-1][:, None], idle)  # its key and value, should all drafts be accepted
         fed = torch.stack(tokens, dim=1)
-        scored = dec.step(fed)
+        scored = dec.step(fed, idle)
         u = torch.rand((B, drafts), device=dev, generator=generator)
+        most = [min(drafts, max(0, n - 1)) for n in left]  # the token after them counts too
+        counts = torch.tensor(most, dtype=torch.int32, device=dev) if min(most) < drafts else None
         got, accepted = verify_draft(scored, fed[:, 1:], torch.stack(logits, dim=1), u, _race(B, V, dev, generator),
-                                     **head_options(a, temperature))
+                                     counts=counts, **head_options(a, temperature))
         took, rows = accepted.tolist(), got.tolist()
-        for o, n, row in zip(out, took, rows):
-            o.extend(row[:n + 1])
-        newest = got.gather(1, accepted[:, None].long())[:, 0]
+        drawn = got.gather(1, accepted[:, None].long())[:, 0]
+        if idle:
+            drawn[idle] = newest[idle]
+        newest = drawn
+        for b, (o, n, row) in enumerate(zip(out, took, rows)):
+            if b not in idle:
+                o.extend(row[:n + 1])
         for d in (dec, draft):
-            d.rollback([drafts - n for n in took])
+            d.rollback([0 if b in idle else drafts - n for b, n in enumerate(took)])
             d.evict()
-        rounds.append(took)
-    return torch.tensor([o[:new_tokens] for o in out], dtype=torch.int32, device=dev), rounds
+        rounds.append([0 if b in idle else n for b, n in enumerate(took)])
+    dec.pending = draft.pending = newest
+    return torch.tensor(out, dtype=torch.int32, device=dev), rounds
 
 
 def main(argv=None) -> None:
@@ -441,7 +468,9 @@ def main(argv=None) -> None:
         out, note = generate(dec, args.new, generator=gen), ""
     else:
         out, rounds = generate_with_draft(dec, draft, args.new, drafts=args.drafts, generator=gen)
-        note = f", {sum(map(sum, rounds)) / (len(rounds) * args.batch):.2f} of {args.drafts} drafts accepted a round"
+        taken = sum(map(sum, rounds))  # each sequence's rounds gave its new tokens but the first, one beside the drafts
+        played = args.batch * (args.new - 1) - taken
+        note = f", {taken / max(1, played):.2f} of {args.drafts} drafts accepted a round"
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     print(f"{out.numel()} tokens in {dt * 1e3:.1f} ms, {out.numel() / dt:.0f} tokens/s{note}")

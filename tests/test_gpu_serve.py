@@ -140,3 +140,41 @@ def test_command_line(capsys):
     from algx.serve import main
     main(["--layers", "1", "--batch", "2", "--prompt", "20", "--new", "8", "--draft-layers", "1", "--drafts", "2"])
     assert "tokens/s" in capsys.readouterr().out
+
+
+def test_drafting_with_another_model_in_no_more_room_than_it_needs(capsys):
+    """Sequences accept differently; the command line's sizes leave one round of drafts beyond the new tokens."""
+    from algx.serve import Decoder, generate_with_draft, main
+    prompts = torch.randint(0, 512, (4, 16), generator=torch.Generator().manual_seed(6)).tolist()
+    target, draft = (Decoder(small(layers=n, seed=n), batch=4, max_slots=16 + 48 + 5) for n in (2, 1))
+    for d in (target, draft):
+        d.prefill(prompts)
+    out, rounds = generate_with_draft(target, draft, 48, generator=torch.Generator(device="cuda").manual_seed(1))
+    assert out.shape == (4, 48) and target.lens == draft.lens == [16 + 47] * 4
+    assert len({sum(r[b] for r in rounds) for b in range(4)}) > 1
+    full = torch.cat([torch.tensor(prompts).cuda(), out[:, :-1]], dim=1)
+    assert rel(target.step(out[:, -1:])[:, 0], full_logits(target.model, torch.nn.functional.pad(
+        torch.cat([full, out[:, -1:]], dim=1), (0, 192)))[:, 63]) < 3e-2
+    main(["--layers", "2", "--batch", "4", "--prompt", "20", "--new", "40", "--draft-layers", "1"])
+    assert "tokens/s" in capsys.readouterr().out and L.device_error() == 0
+
+
+@pytest.mark.parametrize("opts", [dict(), dict(budget=100, slack=16), dict(window=20)])
+def test_idle_sequences_stay_as_they_are(opts):
+    from algx.serve import Decoder
+    model = small()
+    tokens = torch.randint(0, 512, (2, 60), generator=torch.Generator().manual_seed(7)).cuda()
+    a, b = (Decoder(model, batch=2, max_slots=128, **opts) for _ in range(2))
+    for d in (a, b):
+        d.prefill([r[:30].tolist() for r in tokens])
+    a.step(tokens[:, 30:33])
+    b.step(tokens[:, 30:33])
+    last = b.last[1].clone()
+    mixed = torch.stack([tokens[0, 33:38], torch.zeros_like(tokens[1, 33:38])])
+    got, want = b.step(mixed, idle=[1])[0], a.step(tokens[:, 33:38])[0]
+    assert torch.equal(got, want) and torch.equal(b.last[1], last) and b.lens == [38, 33]
+    a.rollback([0, 5])
+    if a.scores is not None:
+        assert torch.equal(b.scores[:, 0], a.scores[:, 0])
+        assert bool((b.scores[:, 1, :, :33].sum(-1) < a.scores[:, 1, :, :33].sum(-1)).all())
+    assert torch.equal(b.step(tokens[:, 38:40])[0], a.step(tokens[:, 38:40])[0]) and L.device_error() == 0

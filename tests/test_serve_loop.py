@@ -13,23 +13,31 @@ import torch
 
 from algx import serve
 from algx.model import config_125m
-from algx.serve import Decoder, generate
+from algx.serve import Decoder, generate, generate_with_draft
 from oracle import serving_math as O
 
 V = 23
 
 
+def logits_of(held, like, seed):
+    """Logits after the cached (position, token) pairs ``held``; ``like`` of them is the same for every seed."""
+    g = torch.Generator().manual_seed(hash(tuple(held)) % 2 ** 62)
+    common = torch.randn(V, generator=g)
+    own = torch.randn(V, generator=g.manual_seed(hash((seed, tuple(held))) % 2 ** 62))
+    return 2 * (like * common + (1 - like) * own)
+
+
 class Toy(Decoder):
     def __init__(self, batch, max_slots, *, like=1.0, seed=0, **kw):
         cfg = config_125m(vocab_size=V, d_model=64, n_heads=1, n_layers=1, d_ff=64)
-        super().__init__(SimpleNamespace(cfg=cfg, flat=SimpleNamespace(data={True: torch.zeros(1)})), batch, max_slots, **kw)
+        model = SimpleNamespace(cfg=cfg, flat=SimpleNamespace(data={True: torch.zeros(1)}), p=lambda name: torch.zeros(1))
+        super().__init__(model, batch, max_slots, **kw)
         self.cache.k = self.cache.k.float()  # (position, token) of every slot
-        self.like, self.seed = like, seed    # how much of the logits all toys share
+        self.toy = like, seed
 
     def held(self, b):
         """(position, token) of the cached slots of sequence b, by position."""
-        rows = O.slots_of(self.cache.k[0], self.cache.table[b], int(self.cache.lens[b]), 0)
-        return sorted((int(r[0]), int(r[1])) for r in rows)
+        return sorted(pairs(self.cache.k[0], self.cache.table[b], int(self.cache.lens[b])))
 
     def tokens(self, b):
         held = self.held(b)
@@ -37,35 +45,61 @@ class Toy(Decoder):
         return [t for _, t in held]
 
     def logits_of(self, held):
-        g = torch.Generator().manual_seed(hash(tuple(held)) % 2 ** 62)
-        common = torch.randn(V, generator=g)
-        own = torch.randn(V, generator=g.manual_seed(hash((self.seed, tuple(held))) % 2 ** 62))
-        return 2 * (self.like * common + (1 - self.like) * own)
+        return logits_of(held, *self.toy)
+
+    def _sink_of(self, i):
+        return self.toy
 
     def _layers(self, tokens, attend):
-        c, size = self.cache, self.cache.page_size
         B, T = tokens.shape
-        out = torch.zeros((B, T, V))
-        for b in range(B):
-            n, start = int(c.lens[b]), int(self.positions[b])
-            slots = [(int(c.table[b, s // size]), s % size) for s in range(n) if s // size < len(c.owned[b])]
-            held = [tuple(int(x) for x in c.k[0, p, 0, r, :2]) for p, r in slots]
-            for t in range(T):
-                s = n + t
-                if s // size < len(c.owned[b]):
-                    page, row = c.owned[b][s // size], s % size
-                    c.k[0, page, 0, row, 0], c.k[0, page, 0, row, 1] = start + t, int(tokens[b, t])
-                    if self.scores is not None:
-                        self.slot_positions[0, b, 0, s] = start + t
-                        self.scores[0, b, 0, s] = 0.0
-                        for i, (p, _) in enumerate(held):
-                            self.scores[0, b, 0, i] += 1 + (7 * p + 3 * start + t) % 5
-                held.append((start + t, int(tokens[b, t])))
-                out[b, t] = self.logits_of(sorted(held))
-        return out
+        return attend(0, tokens[:, :, None, None, None].expand(B, T, 3, 1, 64).float())
 
     def _logits(self, h):
-        return h.reshape(-1, V)
+        return h.reshape(-1, 64)[:, :V]
+
+
+def pairs(k, table, count):
+    return [(int(r[0]), int(r[1])) for r in O.slots_of(k, table, count, 0)]
+
+
+def append(qkv, k, v, table, lens, gain_q, gain_k, *, rotary, positions, counts=None, slot_positions=None, eps):
+    """``cache_append``: tokens and positions in place of keys."""
+    B, T, size = *qkv.shape[:2], k.shape[2]
+    for b in range(B):
+        for t in range(T if counts is None else int(counts[b])):
+            s, at = int(lens[b]) + t, int(positions[b]) + t
+            assert at < rotary[0].shape[0]
+            k[int(table[b, s // size]), 0, s % size, :2] = torch.tensor([float(at), float(qkv[b, t, 0, 0])])
+            if slot_positions is not None:
+                slot_positions[b, 0, s] = at
+    return qkv[:, :, :1]
+
+
+def attention(q, k, v, table, lens, sink, *, scores=None, **kw):
+    """``paged_attention``: the logits of what each query sees in place of its output."""
+    B, T = q.shape[:2]
+    out = torch.zeros((B, T, 1, 64))
+    for b in range(B):
+        n = int(lens[b])
+        held = pairs(k, table[b], n)
+        if scores is not None:
+            scores[b, 0, max(0, n - T):] = 0.0
+        for t in range(T):
+            seen = held[:max(0, n - T + t + 1)]
+            out[b, t, 0, :V] = logits_of(sorted(seen), *sink)
+            if scores is not None:
+                scores[b, 0, :len(seen)] += torch.tensor([float(1 + (7 * p + 3 * len(seen)) % 5) for p, _ in seen])
+    return out if scores is None else (out, scores)
+
+
+def prompt_attention(qkv, gain_q, gain_k, sink, **kw):
+    B, T = qkv.shape[:2]
+    out = torch.zeros((B, T, 1, 64))
+    for b in range(B):
+        row = [(t, int(qkv[b, t, 0, 0, 0])) for t in range(T)]
+        for t in range(T):
+            out[b, t, 0, :V] = logits_of(row[:t + 1], *sink)
+    return out
 
 
 def evict(k, v, table, lens, scores, positions, *, budget, first=0, recent=0):
@@ -89,6 +123,9 @@ def verify(target, tokens, draft, u, race, *, counts=None, **kw):
 def stand_ins(monkeypatch):
     monkeypatch.setattr(serve, "cache_evict", evict)
     monkeypatch.setattr(serve, "verify_draft", verify)
+    monkeypatch.setattr(serve, "cache_append", append)
+    monkeypatch.setattr(serve, "paged_attention", attention)
+    monkeypatch.setattr(serve, "qknorm_flash_attention_packed", prompt_attention)
 
 
 def gen(seed=0):
@@ -171,3 +208,70 @@ def test_pieces_under_a_budget():
     dec, g = toy(**kw), gen(4)
     assert torch.equal(torch.cat([generate(dec, n, generator=g) for n in (13, 20, 7)], dim=1), want)
     assert dec.lens == whole.lens and [dec.held(b) for b in range(3)] == [whole.held(b) for b in range(3)]
+
+
+def drafting(n_new, drafts=4, like=0.6, prompts=PROMPTS, extra=0, **kw):
+    """A target and a draft decoder with no slot to spare: what the longest prompt, the new tokens and one round of
+    drafts take."""
+    slots = max(map(len, prompts)) + n_new + drafts + 1
+    kw = dict(max_slots=slots, max_positions=slots, page_size=16, prompts=prompts, **kw)
+    return toy(like=like, seed=1, **kw), toy(like=like, seed=2, **kw)
+
+
+@pytest.mark.parametrize("like", [0.3, 0.6, 0.9, 1.0])
+@pytest.mark.parametrize("drafts", [1, 4, 7])
+def test_drafting_ends_every_sequence_at_its_last_token(drafts, like):
+    """Sequences of different acceptance: those that are done wait for the others, within slots and positions that
+    hold nothing beyond one round."""
+    n_new = 30
+    dec, draft = drafting(n_new, drafts, like)
+    out, rounds = generate_with_draft(dec, draft, n_new, drafts=drafts, generator=gen(5))
+    assert out.shape == (3, n_new) and out.dtype == torch.int32
+    for d in (dec, draft):
+        assert [d.tokens(b) for b in range(3)] == [p + out[b, :-1].tolist() for b, p in enumerate(PROMPTS)]
+        assert torch.equal(d.pending, out[:, -1])
+    assert all(0 <= n <= drafts for r in rounds for n in r)
+    if like == 1.0:  # equal models: every draft is accepted
+        assert sum(r[0] for r in rounds) == n_new - 1 - len(rounds)
+
+
+def test_drafting_goes_on_after_drafting_and_into_plain_generation():
+    dec, draft = drafting(40)
+    g = gen(6)
+    out = [generate_with_draft(dec, draft, n, generator=g)[0] for n in (9, 1, 12)]
+    out.append(generate(dec, 5, generator=g))
+    out = torch.cat(out, dim=1)
+    assert [dec.tokens(b) for b in range(3)] == [p + out[b, :-1].tolist() for b, p in enumerate(PROMPTS)]
+    with pytest.raises(ValueError, match="same prompts"):
+        generate_with_draft(dec, draft, 3, generator=g)  # the draft model has not seen the last five
+
+
+def test_drafting_refuses_decoders_that_stand_at_different_tokens():
+    dec, draft = drafting(40)
+    generate(dec, 3, generator=gen(7))
+    generate(draft, 3, generator=gen(8))
+    assert dec.seen == draft.seen and not torch.equal(dec.pending, draft.pending)
+    with pytest.raises(ValueError, match="same prompts"):
+        generate_with_draft(dec, draft, 3)
+    dec, draft = drafting(40)
+    for n in (0, 32):
+        with pytest.raises(ValueError, match="drafts"):
+            generate_with_draft(dec, draft, 3, drafts=n)
+    assert generate_with_draft(dec, draft, 0)[0].shape == (3, 0)
+
+
+def test_sequences_that_wait_keep_their_weights():
+    """Under a budget the accumulated weights of a finished sequence stay as they are while the others go on."""
+    prompts = [[1, 2, 3], [4, 5, 6]]
+    kw = dict(max_slots=96, max_positions=96, page_size=16, budget=80, slack=8, prompts=prompts)
+    dec, alone = toy(**kw), toy(**kw)
+    fed = torch.randint(0, V, (2, 6), generator=gen(9))
+    dec.step(fed[:, :3], idle=[])
+    before = dec.scores[:, 1].clone(), dec.last[1].clone()
+    dec.step(fed[:, 3:], idle=[1])
+    assert dec.lens == [9, 6] and dec.seen == [9, 6] and dec.cache.lens.tolist() == [9, 6]
+    assert torch.equal(dec.scores[:, 1], before[0]) and torch.equal(dec.last[1], before[1])
+    alone.step(fed[:, :3])
+    alone.step(fed[:, 3:])
+    assert torch.equal(dec.scores[:, 0], alone.scores[:, 0]) and torch.equal(dec.last[0], alone.last[0])
+    assert dec.tokens(1) == prompts[1] + fed[1, :3].tolist()
