@@ -60,12 +60,21 @@ class PagedCache:
         """Slots of one sequence's table."""
         return self.max_pages * self.page_size
 
+    def _missing(self, need: Sequence[int]) -> int:
+        """Pages that the free list lacks for ``need`` pages of each sequence."""
+        return sum(max(0, n - len(o)) for n, o in zip(need, self.owned)) - len(self.free)
+
+    def fits(self, slots: Sequence[int]) -> bool:
+        """Whether ``reserve(slots)`` would find its slots and pages."""
+        need = [-(-int(n) // self.page_size) for n in slots]
+        return len(need) == len(self.owned) and max(need) <= self.max_pages and self._missing(need) <= 0
+
     def reserve(self, slots: Sequence[int]) -> None:
         """Give sequence b the pages of its first ``slots[b]`` slots."""
         need = [-(-int(n) // self.page_size) for n in slots]
         if len(need) != len(self.owned) or max(need) > self.max_pages:
             raise ValueError(f"at most {self.slots} slots for each of {len(self.owned)} sequences")
-        if sum(max(0, n - len(o)) for n, o in zip(need, self.owned)) > len(self.free):
+        if self._missing(need) > 0:
             raise MemoryError("no free pages")
         changed = False
         for n, own in zip(need, self.owned):
@@ -95,9 +104,10 @@ class Decoder:
     ``max_slots`` bounds the cached tokens of a sequence, ``max_positions`` (default
     the same) their positions, which go on growing when slots are evicted.
     ``budget``: bring every layer's cache down to that many slots per head by
-    accumulated attention weight whenever a sequence holds ``budget + slack``;
-    the ``first`` first positions and the ``recent`` newest always stay (the weights
-    that refused drafts gave stay counted).
+    accumulated attention weight whenever a sequence holds ``budget + slack``, and
+    before a step that would otherwise find no slots or pages; the ``first`` first
+    positions and the ``recent`` newest always stay (the weights that refused
+    drafts gave stay counted).
     ``window``: a sliding window instead, with the ``first`` first slots visible.
     """
 
@@ -109,6 +119,8 @@ class Decoder:
             raise ValueError("eviction moves slots, which a window counts by: give budget or window")
         if budget is not None and not first < budget <= max_slots - slack:
             raise ValueError("budget must exceed first and leave slack below max_slots")
+        if budget is not None and budget >= -(-max_slots // page_size) * page_size:
+            raise ValueError("budget must leave slack: it fills every page of a sequence")
         dev = model.flat.data[True].device
         self.model, self.cfg, self.batch = model, cfg, int(batch)
         self.cache = PagedCache(cfg.n_layers, cfg.n_heads, batch, max_slots, page_size=page_size, pages=pages, device=dev)
@@ -203,6 +215,7 @@ class Decoder:
         by = [0 if b in idle else T for b in range(B)]
         if any(n and at + n > self.max_positions for n, at in zip(by, self.seen)):
             raise ValueError(f"positions end at {self.max_positions}")
+        self.make_room(T, idle)
         c.reserve([n + t for n, t in zip(self.lens, by)])
         counts = torch.tensor(by, dtype=torch.int32, device=c.k.device) if idle else None
         after = c.lens + (T if counts is None else counts)
@@ -229,6 +242,12 @@ class Decoder:
                 newest[idle] = known[idle]
             self._scored = None if known is None else (newest[:, None], [0] * B)
         return logits
+
+    def make_room(self, tokens: int, idle: Sequence[int] = ()) -> None:
+        """Evict now where ``tokens`` more tokens a sequence would find no slots or pages."""
+        if self.budget is not None:
+            if not self.cache.fits([n + (0 if b in idle else tokens) for b, n in enumerate(self.lens)]):
+                self.evict(force=True)
 
     def _advance(self, by):
         self.pending = None
@@ -292,6 +311,8 @@ class Decoder:
 
     def _prefill_steps(self, prompts, sizes, chunk: int = 64):
         done = [0] * self.batch
+        if self.budget is not None:
+            chunk = min(chunk, self.cache.slots - self.budget)
         while any(d < n for d, n in zip(done, sizes)):
             # the sequences advance together, by what the one nearest its end still has
             left = [n - d for d, n in zip(done, sizes)]
@@ -386,6 +407,8 @@ def generate_with_draft(dec: Decoder, draft: Decoder, new_tokens: int, *, drafts
         raise ValueError("the draft model needs the target's vocabulary and head")
     if not 1 <= drafts <= 31:
         raise ValueError("drafts must be from 1 to 31")
+    if any(d.budget is not None and d.cache.slots - d.budget <= drafts for d in (dec, draft)):
+        raise ValueError(f"a round needs room for {drafts + 1} tokens above the budget")
     if dec.pending is None or draft.pending is None:
         ready = dec.pending is draft.pending and dec.last is not None and draft.last is not None
     else:
@@ -404,6 +427,7 @@ def generate_with_draft(dec: Decoder, draft: Decoder, new_tokens: int, *, drafts
         left = [new_tokens - len(o) for o in out]
         idle = [b for b, n in enumerate(left) if n == 0]
         tokens, logits = [newest], []
+        draft.make_room(drafts + 1, idle)  # not between the steps: a rollback cannot go behind an eviction
         for _ in range(drafts):
             logits.append(draft.step(tokens[-1][:, None], idle)[:, 0])
             tokens.append(sample(logits[-1], a, generator, temperature))

@@ -275,3 +275,52 @@ def test_sequences_that_wait_keep_their_weights():
     alone.step(fed[:, 3:])
     assert torch.equal(dec.scores[:, 0], alone.scores[:, 0]) and torch.equal(dec.last[0], alone.last[0])
     assert dec.tokens(1) == prompts[1] + fed[1, :3].tolist()
+
+
+@pytest.mark.parametrize("page_size,max_slots,budget,slack,sizes", [
+    (64, 320, 256, 64, [40, 500]),
+    (16, 164, 100, 64, [400]),
+    (64, 2112, 2048, 64, [2300, 30]),
+    (16, 48, 40, 8, [200, 7, 90]),   # less slack than a chunk of the prompt
+    (16, 41, 40, 1, [60]),
+])
+def test_a_budget_runs_in_the_least_slots(page_size, max_slots, budget, slack, sizes):
+    prompts = [torch.randint(0, V, (n,), generator=gen(n)).tolist() for n in sizes]
+    dec = toy(max_slots, page_size, prompts, max_positions=3000, budget=budget, slack=slack, first=2, recent=5)
+    assert dec.seen == sizes and max(dec.lens) < budget + slack
+    assert torch.equal(dec.last, newest(dec)) or max(sizes) > budget  # an eviction forgets what the logits had seen
+    for b, p in enumerate(prompts):
+        held = dec.held(b)
+        assert len(held) == min(len(p), dec.lens[b]) and all(p[at] == t for at, t in held)
+        assert {at for at, _ in held} >= set(range(min(2, len(p)))) | set(range(max(0, len(p) - 5), len(p)))
+    generate(dec, 2 * slack + 3, generator=gen(10))
+    assert max(dec.lens) < budget + slack
+
+
+def test_drafting_under_a_budget_in_the_least_slots():
+    """Rounds of five tokens meet the end of the tables at every distance."""
+    prompts = [torch.randint(0, V, (n,), generator=gen(n)).tolist() for n in (40, 11)]
+    kw = dict(prompts=prompts, max_slots=48, max_positions=400, page_size=16, budget=40, slack=8, first=2, recent=9)
+    dec, draft = toy(like=0.7, seed=1, **kw), toy(like=0.7, seed=2, **kw)
+    out, _ = generate_with_draft(dec, draft, 90, generator=gen(11))
+    for d in (dec, draft):
+        for b, p in enumerate(prompts):
+            fed = p + out[b, :-1].tolist()
+            assert d.seen[b] == len(fed) and all(fed[at] == t for at, t in d.held(b))
+            assert {at for at, _ in d.held(b)} >= {0, 1} | set(range(len(fed) - 9, len(fed)))
+    with pytest.raises(ValueError, match="room for 9 tokens"):
+        generate_with_draft(dec, draft, 10, drafts=8)
+
+
+def test_an_eviction_makes_room_when_pages_run_out():
+    """Fewer pages than the tables could name: what the budget frees is taken before giving up."""
+    prompts = [torch.randint(0, V, (n,), generator=gen(n)).tolist() for n in (44, 44)]
+    dec = toy(64, 16, prompts, max_positions=200, budget=32, slack=30, first=2, recent=5, pages=6)
+    generate(dec, 30, generator=gen(12))
+    assert dec.seen == [73, 73]
+
+
+def test_a_budget_needs_a_slot_beside_it():
+    with pytest.raises(ValueError, match="leave slack"):
+        toy(48, budget=48, slack=0)
+    assert toy(40, budget=40, slack=0, first=2, recent=4).cache.slots == 48  # the last page's
