@@ -134,6 +134,7 @@ class Decoder:
         self.max_positions = n
         self.lens = [0] * batch       # cached slots, on the host too
         self.seen = [0] * batch       # tokens fed: the next position
+        self.settled = [0] * batch    # first slots that an eviction left in no order of tokens
         self.positions = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.budget, self.slack, self.first = budget, int(slack), int(first)
         self.recent = min(recent if recent is not None else (budget or 0) // 4, (budget or 0) - first) if budget else 0
@@ -257,9 +258,11 @@ class Decoder:
         self.positions.copy_(torch.tensor(self.seen, dtype=torch.int32))
 
     def rollback(self, drop):
-        """Forget the newest ``drop[b]`` tokens of every sequence (refused drafts)."""
+        """Forget the newest ``drop[b]`` tokens of every sequence (refused drafts), fed since it was last evicted from."""
         if any(d < 0 or d > n for d, n in zip(drop, self.lens)):
             raise ValueError("cannot drop more tokens than are cached")
+        if any(d > 0 and n - d < s for d, n, s in zip(drop, self.lens, self.settled)):
+            raise ValueError("cannot drop tokens from before an eviction")
         self._advance([-int(d) for d in drop])
         self.cache.trim(self.lens)
         if self._scored is not None:
@@ -336,6 +339,7 @@ class Decoder:
                                                   recent=self.recent)
             self.scores[i].copy_(scores)
             self.slot_positions[i].copy_(positions)
+        self.settled = [self.budget if n > self.budget else s for n, s in zip(self.lens, self.settled)]
         self.lens = [min(n, self.budget) for n in self.lens]
         c.lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
         c.trim(self.lens)

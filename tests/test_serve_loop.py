@@ -324,3 +324,20 @@ def test_a_budget_needs_a_slot_beside_it():
     with pytest.raises(ValueError, match="leave slack"):
         toy(48, budget=48, slack=0)
     assert toy(40, budget=40, slack=0, first=2, recent=4).cache.slots == 48  # the last page's
+
+
+def test_a_rollback_does_not_go_behind_an_eviction():
+    """Evicted sequences hold their slots in no order of tokens; the others' still are."""
+    prompts = [torch.randint(0, V, (n,), generator=gen(n)).tolist() for n in (36, 9)]
+    dec = toy(64, 16, prompts, max_positions=200, budget=30, slack=10, first=2, recent=5)
+    assert dec.evict(force=True) and dec.lens == [30, 9]
+    dec.step(torch.zeros((2, 3), dtype=torch.int64))
+    before = dec.held(0), dec.held(1)
+    with pytest.raises(ValueError, match="cannot drop tokens from before an eviction"):
+        dec.rollback([4, 0])
+    assert (dec.held(0), dec.held(1)) == before and dec.lens == [33, 12]
+    dec.rollback([3, 8])
+    assert dec.lens == [30, 4] and dec.tokens(1) == prompts[1][:4]
+    assert max(p for p, _ in dec.held(0)) == 35
+    with pytest.raises(ValueError, match="cannot drop more tokens"):
+        dec.rollback([0, 5])
