@@ -350,6 +350,8 @@ def head_options(cfg, temperature: float = 1.0) -> dict:
     """``verify_draft``'s options for a model's likelihood head."""
     if cfg.head == "ce":
         return dict(kind="ce", temperature=temperature)
+    if temperature != 1.0:
+        raise ValueError("temperature is for the ce kind")
     return dict(kind="alg_ce", n=cfg.head_n, c=cfg.head_c)
 
 

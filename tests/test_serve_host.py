@@ -78,3 +78,10 @@ def test_operators_have_shapes_for_tracers():
         assert tokens.shape == (3, 5) and accepted.shape == (3,) and tokens.dtype == accepted.dtype == i32
     with pytest.raises(ValueError, match="window must be positive"):
         T.paged_attention(None, None, None, None, None, window=0)
+
+
+def test_the_algebraic_head_has_no_temperature():
+    """As ``verify_draft`` refuses it: a temperature that is ignored would sample from another distribution than asked."""
+    from algx.model import config_algebraic_125m
+    with pytest.raises(ValueError, match="temperature is for the ce kind"):
+        head_options(config_algebraic_125m(), 0.5)
