@@ -11,7 +11,7 @@ backward wired through ``torch.library.register_autograd``:
 and the serving operators, which have no backward:
 
 * ``algx::cache_append``, ``algx::paged_attention``, ``algx::paged_attention_scored``,
-  ``algx::cache_evict`` (the cache's tensors are mutated arguments)
+  ``algx::paged_attention_scored_into``, ``algx::cache_evict`` (the cache's tensors are mutated arguments)
 * ``algx::verify_draft``
 
 To a tracer (``torch.compile``, ``torch.export``, CUDA-graph capture tools)
@@ -324,14 +324,34 @@ def _(q, k_pages, v_pages, table, lens, sink, scores, kind, n, c, window, first)
     return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
+@torch.library.custom_op("algx::paged_attention_scored_into", mutates_args=("scores_out",))
+def _paged_attention_scored_into_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lens: Tensor,
+                                    sink: Optional[Tensor], scores: Tensor, scores_out: Tensor, kind: str, n: int,
+                                    c: float, window: int, first: int) -> Tensor:
+    return P.paged_attention(q, k_pages, v_pages, table, lens, sink, kind=kind, n=n, c=c, window=window or None,
+                             first=first, scores=scores, scores_out=scores_out)[0]
+
+
+@_paged_attention_scored_into_op.register_fake
+def _(q, k_pages, v_pages, table, lens, sink, scores, scores_out, kind, n, c, window, first):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
 def paged_attention(q, k_pages, v_pages, table, lens, sink_logit=None, *, kind: str = "softmax", n: int = 16,
-                    c: float = 16.0, window: Optional[int] = None, first: int = 0, scores=None):
-    """``algx.kernels.paged.paged_attention`` as one node; ``scores`` is updated in place and returned beside o."""
+                    c: float = 16.0, window: Optional[int] = None, first: int = 0, scores=None, scores_out=None):
+    """``algx.kernels.paged.paged_attention`` as one node; the scores are written in place, or into ``scores_out``."""
     P.paged_options(kind, n, c, window, first)
+    if sink_logit is not None and not isinstance(sink_logit, Tensor):
+        sink_logit = torch.as_tensor(sink_logit, dtype=torch.float32)
+    if scores is None and scores_out is not None:
+        raise ValueError("scores_out without scores")
     args = (q, k_pages, v_pages, table, lens, sink_logit)
+    opts = (kind, n, float(c), window or 0, first)
     if scores is None:
-        return _paged_attention_op(*args, kind, n, float(c), window or 0, first)
-    return _paged_attention_scored_op(*args, scores, kind, n, float(c), window or 0, first), scores
+        return _paged_attention_op(*args, *opts)
+    if scores_out is None or scores_out is scores:
+        return _paged_attention_scored_op(*args, scores, *opts), scores
+    return _paged_attention_scored_into_op(*args, scores, scores_out, *opts), scores_out
 
 
 @torch.library.custom_op("algx::cache_evict", mutates_args=("k_pages", "v_pages"))

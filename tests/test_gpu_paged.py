@@ -412,6 +412,24 @@ def test_operators_match_the_functions():
     assert all(torch.equal(x, y) for x, y in zip(*outs)) and all(torch.equal(x, y) for x, y in zip(*caches))
 
 
+def test_the_attention_operator_takes_what_the_function_takes():
+    """A number for the sink, and scores into a buffer of their own."""
+    from algx import torch_ops as T
+    k, v, table, g = make_cache(2, 2, 32, 4, BF16, 72)
+    k, v, table = k.cuda(), v.cuda(), table.cuda()
+    q = torch.randn((2, 3, 4, 64), generator=g).to(BF16).cuda()
+    lens = torch.tensor([60, 5], dtype=torch.int32).cuda()
+    assert torch.equal(T.paged_attention(q, k, v, table, lens, 1.5, kind="asinh", c=8.0),
+                       paged_attention(q, k, v, table, lens, 1.5, kind="asinh", c=8.0))
+    scores = torch.rand((2, 2, 128), generator=g).cuda()
+    before, out = scores.clone(), [torch.full_like(scores, math.nan) for _ in range(2)]
+    a = paged_attention(q, k, v, table, lens, 0.5, scores=scores, scores_out=out[0])
+    b = T.paged_attention(q, k, v, table, lens, 0.5, scores=scores, scores_out=out[1])
+    assert torch.equal(a[0], b[0]) and b[1] is out[1] and torch.equal(*out) and torch.equal(scores, before)
+    c = T.paged_attention(q, k, v, table, lens, 0.5, scores=scores, scores_out=scores)
+    assert torch.equal(c[0], a[0]) and torch.equal(scores, out[0])
+
+
 def test_unaligned_inputs_are_copied():
     k, v, table, g = make_cache(1, 2, 16, 2, BF16, 71)
     base = torch.randn(1 + 6 * 64, generator=g).to(BF16).cuda()

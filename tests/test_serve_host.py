@@ -85,3 +85,20 @@ def test_the_algebraic_head_has_no_temperature():
     from algx.model import config_algebraic_125m
     with pytest.raises(ValueError, match="temperature is for the ce kind"):
         head_options(config_algebraic_125m(), 0.5)
+
+
+def test_the_attention_operator_has_the_functions_arguments():
+    import inspect
+
+    from algx import torch_ops as T
+    from algx.kernels import paged
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    assert inspect.signature(T.paged_attention) == inspect.signature(paged.paged_attention)
+    with FakeTensorMode():
+        k, table = torch.empty((9, 2, 16, 64)), torch.empty((3, 4), dtype=torch.int32)
+        args = torch.empty((3, 5, 4, 64)), k, k, table, table[:, 0]
+        assert T.paged_attention(*args, 0.5).shape == (3, 5, 4, 64)
+        scores, out = torch.empty((3, 2, 64)), torch.empty((3, 2, 64))
+        assert T.paged_attention(*args, scores=scores, scores_out=out)[1] is out
+    with pytest.raises(ValueError, match="scores_out without scores"):
+        T.paged_attention(None, None, None, None, None, scores_out=out)
