@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <array>
 #include <stdexcept>
 #include <string>
 
@@ -154,6 +155,22 @@ Tensor workspace(size_t bytes, const Tensor& like) {
   return at::empty({(int64_t)(bytes ? bytes : 1)}, like.options().dtype(at::kByte));
 }
 
+// Where the program has other Python threads, allocations and launches run without
+// the interpreter's lock, as torch's own calls do: a launch waits while the stream's
+// queue is full. (One token into the cache: 6.9 us a pass with the lock handed back
+// and taken again, 6.3 without, which is what a program of one thread pays.)
+struct Unlocked {
+  PyThreadState* state = nullptr;
+  Unlocked() {
+    PyThreadState* head = PyInterpreterState_ThreadHead(PyInterpreterState_Get());
+    if (head && PyThreadState_Next(head)) state = PyEval_SaveThread();
+  }
+  ~Unlocked() {
+    if (state) PyEval_RestoreThread(state);
+  }
+  Unlocked(const Unlocked&) = delete;
+};
+
 // ------------------------------------------------------------------ operators
 Tensor append(Args& in) {
   const Tensor &qkv = in.tensor("qkv"), &k = in.tensor("k_pages"), &v = in.tensor("v_pages"), &table = in.tensor("table"),
@@ -178,6 +195,7 @@ Tensor append(Args& in) {
   check_vector("counts", counts, c.B);
   if (where) check_state("slot_positions", *where, {c.B, c.heads, c.max_pages * c.size}, at::kInt);
   same_device(qkv, {&k, &v, &table, &lens, gq, gk, cos, sin, positions, counts, where});
+  Unlocked unlocked;
   c10::cuda::CUDAGuard guard(qkv.device());
   const Tensor x = ready(qkv), tb = table.contiguous(), ln = lens.contiguous();
   Tensor g[2], r[2], pos, cnt;
@@ -218,6 +236,7 @@ Tensor attend(Args& in) {
     check_state("scores_out", *out, {c.B, c.heads, S}, at::kFloat);
   }
   same_device(q, {&k, &v, &table, &lens, scores, out});
+  Unlocked unlocked;
   c10::cuda::CUDAGuard guard(q.device());
   Tensor s;
   if (sink) {
@@ -237,7 +256,7 @@ Tensor attend(Args& in) {
   return o;
 }
 
-PyObject* evict(Args& in) {
+std::array<Tensor, 4> evict(Args& in) {
   const Tensor &k = in.tensor("k_pages"), &v = in.tensor("v_pages"), &table = in.tensor("table"), &lens = in.tensor("lens"),
                &scores = in.tensor("scores"), &positions = in.tensor("positions");
   const int64_t budget = in.integer(), first = in.integer(), recent = in.integer();
@@ -248,6 +267,7 @@ PyObject* evict(Args& in) {
   check_state("scores", scores, {c.B, c.heads, c.max_pages * c.size}, at::kFloat);
   check_state("positions", positions, {c.B, c.heads, c.max_pages * c.size}, at::kInt);
   same_device(k, {&v, &table, &lens, &scores, &positions});
+  Unlocked unlocked;
   c10::cuda::CUDAGuard guard(k.device());
   const Tensor tb = table.contiguous(), ln = lens.contiguous(), sc = ready(scores), po = ready(positions);
   Tensor new_lens = at::empty({c.B}, ln.options());
@@ -260,11 +280,10 @@ PyObject* evict(Args& in) {
                 static_cast<int32_t*>(ptr(new_positions)), static_cast<int32_t*>(ptr(kept)), c.B, c.heads, c.num, c.size,
                 c.max_pages, 64, c.code, ptr(ws), bytes, stream_of(k)),
         "algx_cache_evict");
-  return Py_BuildValue("(NNNN)", THPVariable_Wrap(new_lens), THPVariable_Wrap(new_scores), THPVariable_Wrap(new_positions),
-                       THPVariable_Wrap(kept));
+  return {new_lens, new_scores, new_positions, kept};
 }
 
-PyObject* verify(Args& in) {
+std::array<Tensor, 2> verify(Args& in) {
   const Tensor &target = in.tensor("target_logits"), &tokens = in.tensor("draft_tokens");
   const Tensor* draft = in.maybe("draft_logits");
   const Tensor &u = in.tensor("accept_u"), &race = in.tensor("race");
@@ -287,6 +306,7 @@ PyObject* verify(Args& in) {
   if (!shaped(race, {B, V}, at::kFloat)) bad("race must be float32 of shape " + text({B, V}));
   check_vector("counts", counts, B);
   same_device(target, {draft, &tokens, &u, &race, counts});
+  Unlocked unlocked;
   c10::cuda::CUDAGuard guard(target.device());
   const Tensor t = target.contiguous(), tk = tokens.contiguous(), uu = u.contiguous(), rr = race.contiguous();
   Tensor d, cn;
@@ -297,7 +317,7 @@ PyObject* verify(Args& in) {
                  counts ? ints(cn) : nullptr, static_cast<const float*>(ptr(uu)), static_cast<const float*>(ptr(rr)),
                  static_cast<int32_t*>(ptr(out)), static_cast<int32_t*>(ptr(accepted)), B, K, V, code, stream_of(t)),
         "algx_verify_draft");
-  return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(accepted));
+  return {out, accepted};
 }
 
 // ------------------------------------------------------------------ the module
@@ -328,8 +348,19 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(a, n, [](Args& in) { return THPVariable_Wrap(attend(in)); });
 }
-PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(a, n, evict); }
-PyObject* py_verify(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(a, n, verify); }
+PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, [](Args& in) {
+    const auto t = evict(in);
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(t[0]), THPVariable_Wrap(t[1]), THPVariable_Wrap(t[2]),
+                         THPVariable_Wrap(t[3]));
+  });
+}
+PyObject* py_verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, [](Args& in) {
+    const auto t = verify(in);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(t[0]), THPVariable_Wrap(t[1]));
+  });
+}
 
 // bind(AlgxError, {name: address})
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {

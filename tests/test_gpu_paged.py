@@ -462,3 +462,39 @@ def test_scores_of_a_call_without_tokens(in_place, dtype):
                              scores=sc, scores_out=out)
     assert o.shape == (3, 0, 4, 64) and got.data_ptr() == out.data_ptr()
     assert torch.equal(got.cpu(), want) and L.device_error() == 0
+
+
+def test_other_threads_run_while_a_launch_waits():
+    """The stream's queue is full behind a kernel of some 0.4 s: a thread that looks at the clock every millisecond is
+    not held up as long as the calls are."""
+    import threading
+    import time
+    k, v, table, g = make_cache(1, 2, 16, 4, BF16, 73)
+    k, v, table = k.cuda(), v.cuda(), table.cuda()
+    qkv = torch.randn((1, 1, 6, 64), generator=g).to(BF16).cuda()
+    lens = torch.tensor([5], dtype=torch.int32).cuda()
+    calls = [lambda: cache_append(qkv, k, v, table, lens), lambda: paged_attention(qkv[:, :, :4], k, v, table, lens)]
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        ticks, stop = [], threading.Event()
+
+        def tick():
+            while not stop.is_set():
+                ticks.append(time.perf_counter())
+                time.sleep(1e-3)
+
+        thread = threading.Thread(target=tick)
+        thread.start()
+        torch.cuda._sleep(800_000_000)
+        worst = 0.0
+        for _ in range(3000):
+            t0 = time.perf_counter()
+            call()
+            worst = max(worst, time.perf_counter() - t0)
+        stop.set()
+        thread.join()
+        torch.cuda.synchronize()
+        gap = max(b - a for a, b in zip(ticks, ticks[1:]))
+        assert worst > 0.1, "no call waited: the queue was never full"
+        assert gap < 0.5 * worst
