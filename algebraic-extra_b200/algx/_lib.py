@@ -7,6 +7,7 @@ is missing; there is no CPU fallback anywhere in the package.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import threading
 
@@ -178,6 +179,11 @@ def check(status: int, what: str) -> None:
 
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def has_reciprocal(x: float) -> bool:
+    """Whether x is positive and finite and its reciprocal so in float32, as which it reaches the kernels."""
+    return math.isfinite(x) and x > 0 and 0.0 < ctypes.c_float(1.0 / x).value < math.inf
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

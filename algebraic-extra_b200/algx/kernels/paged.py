@@ -24,7 +24,6 @@ weights (algebraic.py:186-216, standard.py:24-38).
 from __future__ import annotations
 
 import functools
-import math
 from typing import Optional
 
 import torch
@@ -60,7 +59,7 @@ def paged_options(kind: str, n: int, c: float, window: Optional[int], first: int
         raise ValueError(f"unknown attention kernel: {kind}")
     if kind == "asinh" and (n < 2 or n & (n - 1)):
         raise ValueError("asinh kernel needs n to be a power of two")
-    if kind == "asinh" and (not math.isfinite(c) or c <= 0):
+    if kind == "asinh" and not (L.has_reciprocal(c) and L.has_reciprocal(8.0 * c)):
         raise ValueError("asinh scale c must be positive and finite")
     if window is not None and not 1 <= window < 2 ** 31:
         raise ValueError("window must be positive")

@@ -12,7 +12,6 @@ counterpart.
 from __future__ import annotations
 
 import functools
-import math
 
 from .. import _lib as L
 
@@ -25,12 +24,12 @@ def _options(kind: str, n: int, c: float, temperature: float):
     if kind == "alg_ce":
         if n not in (2, 4, 8, 16, 32):
             raise ValueError("algx supports alg_ce powers n in {2, 4, 8, 16, 32}")
-        if not math.isfinite(c) or c <= 0:
+        if not L.has_reciprocal(c):
             raise ValueError("alg_ce scale c must be positive and finite")
         if temperature != 1.0:
             raise ValueError("temperature is for the ce kind")
         return L.ALGX_HEAD_ALG_CE, n, 1.0 / c
-    if not math.isfinite(temperature) or temperature <= 0:
+    if not L.has_reciprocal(temperature):
         raise ValueError("temperature must be positive and finite")
     return L.ALGX_HEAD_CE, 2, 1.0 / temperature
 

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -1162,6 +1163,8 @@ int algx_paged_attn(const algx_paged_config* cfg, const void* q, const void* k_p
   ALGX_REQUIRE(cfg->kind == ALGX_ATTN_SOFTMAX || (cfg->n >= 2 && (cfg->n & (cfg->n - 1)) == 0),
                "n must be a power of two");
   ALGX_REQUIRE(T >= 0 && Hq >= 1 && Hq % Hkv == 0, "query heads must be a multiple of the cache's heads");
+  ALGX_REQUIRE(cfg->scale > 0.f && std::isfinite(cfg->scale) && cfg->inv_unit > 0.f && std::isfinite(cfg->inv_unit),
+               "scale and inv_unit must be positive and finite");
   ALGX_REQUIRE(cfg->window >= 0 && cfg->first >= 0, "window and first must not be negative");
   ALGX_REQUIRE((scores == nullptr) == (scores_out == nullptr), "give scores and scores_out or neither");
   if (B == 0 || (T == 0 && scores == nullptr)) return ALGX_OK;

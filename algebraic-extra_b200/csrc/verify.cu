@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -475,7 +476,7 @@ extern "C" int algx_verify_draft(int32_t kind, int32_t n, float scale, const voi
   ALGX_REQUIRE(kind == ALGX_HEAD_CE || (n >= 2 && (n & (n - 1)) == 0), "n must be a power of two");
   ALGX_REQUIRE(B >= 0 && K >= 0 && K < 32, "at most 31 drafted tokens");
   ALGX_REQUIRE(V >= 1 && V <= INT32_MAX, "the vocabulary must not be empty");
-  ALGX_REQUIRE(scale > 0.f, "scale must be positive");
+  ALGX_REQUIRE(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
   if (B == 0) return ALGX_OK;
   ALGX_REQUIRE(B <= INT32_MAX / 16, "too many sequences");
   ALGX_REQUIRE(target && race && out && accepted && (K == 0 || (tokens && u)), "NULL tensor");

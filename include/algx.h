@@ -370,7 +370,7 @@ typedef struct algx_paged_config {
   int32_t window; /* 0, or the newest slots a query sees, its own among them */
   int32_t first;  /* first slots that stay visible under a window */
   float scale;    /* 1/(sqrt(D)*unit), unit = c (asinh) or 1 (softmax) */
-  float inv_unit; /* 1/unit, multiplies the sink logits */
+  float inv_unit; /* 1/unit, multiplies the sink logits; both positive and finite */
 } algx_paged_config;
 
 /* Bytes of workspace algx_paged_attn needs (no initialisation needed); scored:
@@ -421,7 +421,7 @@ ALGX_API int algx_cache_evict(void* k_pages, void* v_pages, const int32_t* table
 /* Verification of K <= 31 drafted tokens per sequence and the draw of the next
  * one. target (B, K + 1, V) and draft (B, K, V) logits (draft NULL: every draft
  * is a certain proposal, q = 1 at its token); probabilities by softmax of
- * scale * z (ALGX_HEAD_CE) or rho(scale * z)^n normalised (ALGX_HEAD_ALG_CE,
+ * scale * z (ALGX_HEAD_CE; scale positive and finite) or rho(scale * z)^n normalised (ALGX_HEAD_ALG_CE,
  * algebraic.py:266-301), -inf and NaN logits having none. Token i is accepted
  * while u[b][i] q_i(x_i) < p_i(x_i). The next token is
  * argmax_v weight_v / race[b][v], the lowest index on ties, with weight

@@ -65,3 +65,37 @@ def test_attention_counts_groups_of_slots_in_32_bits():
     assert call(2 ** 27 - 5) == L.ALGX_OK
     for pages in (2 ** 27 - 4, 2 ** 27 - 1, 2 ** 60):
         assert call(pages) == L.ALGX_ERR_INVALID and b"too large" in lib.algx_last_error()
+
+
+@pytest.mark.parametrize("scale,inv_unit", [(0.0, 1.0), (-1.0, 1.0), (float("inf"), 1.0), (float("nan"), 1.0),
+                                            (1.0, float("inf")), (1.0, 0.0)])
+def test_attention_needs_a_positive_finite_scale(scale, inv_unit):
+    """The largest score of a group is looked for before scaling, and masked scores are -inf times the scale."""
+    lib = L.lib()
+    cfg = L.PagedConfig(0, 16, 0, 0, scale, inv_unit)
+    status = lib.algx_paged_attn(cfg, *[None] * 9, 0, 1, 2, 2, 1, 16, 1, 64, L.ALGX_BF16, None, 0, None)
+    assert status == L.ALGX_ERR_INVALID and b"positive and finite" in lib.algx_last_error()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -1.0, 0.0])
+def test_verification_needs_a_positive_finite_scale(scale):
+    lib = L.lib()
+    status = lib.algx_verify_draft(L.ALGX_HEAD_CE, 2, scale, *[None] * 8, 0, 1, 9, L.ALGX_F32, None)
+    assert status == L.ALGX_ERR_INVALID and b"positive and finite" in lib.algx_last_error()
+
+
+def test_options_whose_reciprocal_float32_does_not_hold():
+    """1e-39 is positive and finite, 1e39 is not a float32: the logits' differences of zero times it are NaN."""
+    import torch
+
+    from algx.kernels.paged import paged_attention
+    from algx.kernels.verify import verify_draft
+    none = torch.zeros(1)
+    with pytest.raises(ValueError, match="temperature must be"):
+        verify_draft(none, none, None, none, none, temperature=1e-39)
+    with pytest.raises(ValueError, match="positive and finite"):
+        verify_draft(none, none, None, none, none, kind="alg_ce", n=8, c=1e-39)
+    with pytest.raises(ValueError, match="positive and finite"):
+        paged_attention(none, none, none, none, none, kind="asinh", c=1e-39)
+    with pytest.raises(ValueError, match="temperature must be"):  # its reciprocal is zero
+        verify_draft(none, none, None, none, none, temperature=1e60)
