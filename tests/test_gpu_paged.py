@@ -498,3 +498,19 @@ def test_other_threads_run_while_a_launch_waits():
         gap = max(b - a for a, b in zip(ticks, ticks[1:]))
         assert worst > 0.1, "no call waited: the queue was never full"
         assert gap < 0.5 * worst
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["asinh", "softmax"])
+@pytest.mark.parametrize("case", [
+    dict(B=2, T=70, Hq=3, Hkv=3, page=16, lens=[200, 75], sink=True),                     # a chunk of a prompt
+    dict(B=2, T=64, Hq=2, Hkv=2, page=64, lens=[64, 131], scored=True, in_place=True),
+    dict(B=1, T=33, Hq=6, Hkv=2, page=32, lens=[300], window=40, first=3),                # 99 rows a head
+    dict(B=3, T=40, Hq=4, Hkv=2, page=128, lens=[20, 0, 170], scored=True, sink=True),    # fewer slots than tokens
+    dict(B=1, T=17, Hq=2, Hkv=2, page=16, lens=[260], scored=True, window=30, first=2),
+])
+def test_attention_of_prompt_chunks(case, kind, dtype):
+    """More rows than three tiles hold, in both joins."""
+    check_attention(dtype=dtype, kind=kind, seed=300 + case["T"], **case)
+    if not case.get("scored"):
+        check_attention(dtype=dtype, kind=kind, seed=300 + case["T"], wide=4096, **case)

@@ -203,3 +203,11 @@ def test_close_races_are_decided_exactly(n):
     L.check(L.lib().algx_verify_draft(L.ALGX_HEAD_ALG_CE, n, 1.0, zd.data_ptr(), None, None, None, None, rd.data_ptr(),
                                       out.data_ptr(), accepted.data_ptr(), B, 0, V, L.ALGX_F32, L.stream_of(zd)), "verify")
     assert out[:, 0].tolist() == best.tolist() and accepted.tolist() == [0] * B
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["ce", "alg_ce"])
+@pytest.mark.parametrize("B", [1, 40, 64])
+def test_sampling_over_a_real_vocabulary(B, kind, dtype):
+    target, tokens, _, u, race = inputs(B, 0, 50304, dtype, kind, 2.0, 30 + B)
+    check(target, tokens, None, u, race, kind=kind, n=8, c=2.0)
