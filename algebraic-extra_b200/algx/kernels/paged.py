@@ -13,9 +13,10 @@ and, for a cache that must not grow, ``paged_attention(..., scores=scores)``
 accumulates the attention weight every slot received and ``cache_evict`` keeps
 the slots that received most. Everything runs on the current stream without
 host synchronisation, so a step can be captured in a CUDA graph; page numbers,
-lengths and positions are read on the device, and one outside its range is
-skipped and raises the device error word (``algx._lib.device_error()``) instead
-of being followed. No gradients: these are serving operators (the training path
+lengths and positions are read on the device, and one outside its range raises
+the device error word (``algx._lib.device_error()``) and is not followed: slots
+beyond the table or in a page that does not exist are left out, a length is cut
+to the table, a position to the rotary tables' nearest row. No gradients: these are serving operators (the training path
 is ``algx.kernels.flash``). The reference has no cache; the formulas are its
 QK norm (qk_norm.py:29-43), rotation (algebraic.py:172-179) and attention
 weights (algebraic.py:186-216, standard.py:24-38).
@@ -40,7 +41,8 @@ def cache_append(qkv, k_pages, v_pages, table, lens, gain_q=None, gain_k=None, *
     ``lens``: slots held before the call; token t goes to slot ``lens[b] + t``
     and the call changes no length. ``gain_q``, ``gain_k`` (64,) float32 apply
     the QK RMS norm, ``rotary`` = (cos, sin), each (rows, 32) float32, the
-    rotation at position ``positions[b] + t`` (default: the slot). Norm and
+    rotation at position ``positions[b] + t`` (default: the slot; one outside the
+    tables takes their nearest row, and sets the error word). Norm and
     rotation are evaluated in float32 and rounded once. ``counts`` (B,) int32:
     tokens beyond it are padding, stored nowhere, their queries zero.
     ``slot_positions`` (B, Hkv, max_pages * page_size) int32 receives the new

@@ -35,7 +35,8 @@ struct AppendArgs {
 // rows a group). y = rms(x) g, then (y1 c - y2 s, y1 s + y2 c), all in fp32 with
 // one rounding at the store: the cache holds the nearest bf16 of the exact key.
 // Bound by memory: each row is read once and written once. Measured: 16384 tokens of
-// 36 rows (155 MB) 30 us, 5.1 TB/s; with a row across 8 lanes, halves exchanged by
+// 36 rows (155 MB) 32 us a pass, 4.8 TB/s, of 6.55 a plain copy reaches, at 14 warps an
+// SM; with a row across 8 lanes, halves exchanged by
 // shuffles, 47 us; three row groups a warp instead of five 34 us.
 template <typename T, bool NORM, bool ROT>
 __global__ void __launch_bounds__(kAppThreads, 4) cache_append_kernel(const AppendArgs a, const PagedView pv) {
@@ -261,9 +262,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const PagedView& p
 // rounds of counting 11 bits; slots above it stay, and of those equal to it the
 // lowest slots. One sweep over the slots then numbers the holes below the budget
 // and the kept slots at or above it: the i-th such slot moves to the i-th hole, so
-// a row that is below the budget never moves. This is a chain of some twenty
-// block-wide steps, whatever the length. Measured: 12 items of 2560 slots 17 us, with
-// the moves, 192 items of 8192 slots 27 us. (Counting with one addition for all lanes
+// a row that is below the budget never moves. This is a chain of block-wide steps: some
+// twenty, and two barriers (four where scores are equal at the limit) for every 2048
+// slots of the last sweep. Measured: 12 items of 2560 slots, with the moves, 10.9 us a
+// pass (19 as one cold launch under the profiler), 192 items of 8192 slots 27 us. (Counting with one addition for all lanes
 // that meet in a bin took 40 us: their matching costs more than the conflicts.)
 __global__ void __launch_bounds__(kEvThreads, 2) cache_evict_kernel(const EvictArgs a, const PagedView pv) {
   extern __shared__ uint4 s_keys[];
