@@ -14,7 +14,7 @@ def evict(B=1, Hkv=1, page_size=16, max_pages=4, budget=8, dtype=L.ALGX_BF16, **
     room = (ctypes.c_char * 8192)()
     base = (ctypes.addressof(room) + 63) // 64 * 64
     place = dict(k=base, v=base, table=base, lens=base, scores=base, positions=base, new_lens=base + 1024,
-                 new_scores=base + 2048, new_positions=base + 3072, kept=base + 4096, workspace=base)
+                 new_scores=base + 2048, new_positions=base + 4096, kept=base + 5120, workspace=base)
     place.update({name: place[name] + off for name, off in at.items()})
     p = place
     # a workspace of one byte is too small: whatever passes the other checks is refused for that
